@@ -52,6 +52,9 @@ enum {
     MMEB200_FP32_IEEE = 14,
     MMEB200_TF32 = 15
 };
+/* Signed 8-bit integers, a type of the 8-bit layer operators below only (outside the range of EMmeDataType: the
+ * calculator's entry points refuse it). */
+enum { MMEB200_INT8 = 64 };
 
 /* ---- EMmeOpType values (mme_common_enum.h:83-102) ---- */
 enum {
@@ -188,7 +191,8 @@ int mmeb200_set_accumulation(mmeb200_ctx* ctx, int mode);
 int mmeb200_set_option(mmeb200_ctx* ctx, const char* name, int value);
 
 /* Run all later work of this context on the caller's CUDA stream (a cudaStream_t passed as
- * void*); NULL goes back to the context's own stream. */
+ * void*); NULL goes back to the context's own stream, which is not ordered with the legacy default
+ * stream: a caller whose stream is the default one passes cudaStreamLegacy, i.e. (void*)1. */
 int mmeb200_set_stream(mmeb200_ctx* ctx, void* cuda_stream);
 
 /* Replaces CPUCalculator::limitNumOfThreads (mme_reference_impl.cpp:2002-2012): kept for
@@ -359,6 +363,62 @@ int mmeb200_peer_close(mmeb200_ctx* ctx, void* dev_ptr);
 int mmeb200_conv_dedw_allreduce(mmeb200_ctx* ctx, mmeb200_tensor* out, const mmeb200_tensor* x,
                                 const mmeb200_tensor* w, const mmeb200_tensor* y,
                                 const mmeb200_conv_params* params, const mmeb200_peer_group* group);
+
+/* ---- the 8-bit layer: norm -> 8-bit rows -> scaled product ----------------------------------------
+ * No counterpart in the reference's calculator, whose 8-bit operands carry an exponent bias at most. Rows are what runs
+ * along dimension 0: a tensor [cols, r1, r2, r3, r4] has r1*r2*r3*r4 rows, with any strides in dimensions 1..4 (an output's
+ * elements must not share memory; inputs' may). 8-bit codes are int8 (MMEB200_INT8, -127..127), fp8_143 in any Inf/NaN mode
+ * and exponent bias, or fp8_152 in the full Inf/NaN mode. Scales are dense fp32 tensors with one element per row: a row's
+ * values are its codes times its scale.
+ *
+ * How a row v (32 bits) becomes codes: step = max|v| / top, top = 127 or the largest finite value of the fp8 type; every
+ * code is the representable value nearest to the 32-bit quotient v / step, ties to even, limited to +-top. All of it is
+ * correctly rounded 32-bit arithmetic, so codes are reproducible bit for bit. A row of zeros has scale 0; a row with an
+ * infinity or a NaN has scale NaN and codes 0. MMEB200_SCALE_GIVEN reads `scale` instead of writing it (one element per row,
+ * or one for all): code = nearest to v / scale, limited; a NaN becomes int8 0 or the fp8 type's NaN, and a scale that is
+ * zero, negative or no finite number gives codes 0.
+ *
+ * Streams and memory: device-tensor calls are asynchronous on the context's stream and can be captured into a CUDA graph
+ * once each entry point (with these types) has run before; calls that need scratch memory are refused while capturing, see
+ * the entries. The caller's current device is left as it was. An output may be the same tensor as an input (same address,
+ * type and strides) where the entry says so; any other overlap is refused. Host tensors are staged as everywhere else. */
+enum { MMEB200_SCALE_ROW = 0, MMEB200_SCALE_GIVEN = 1 };
+
+/* RMS norm of every row, with the residual's addition: h = x + residual, rounded to the residual's type and written to
+ * `sum`; out = h / sqrt(mean(h^2) + eps) * gamma, all in 32 bits and rounded once.
+ *   x, residual, gamma: bf16 or fp32 each; residual, sum and gamma may be NULL (no addition; h not kept; ones). sum has the
+ *   residual's type, and may be the same tensor as x or residual; out may be the same tensor as x or residual.
+ *   out: bf16, fp32 (scale must be NULL), or 8-bit codes with `scale` (see above; the codes of h * gamma, whose scale then
+ *   carries the factor 1 / sqrt(...); with MMEB200_SCALE_GIVEN the codes of the finished rows).
+ *   gamma: dense, one element per column. eps: finite, >= 0. */
+int mmeb200_rms_norm(mmeb200_ctx* ctx, mmeb200_tensor* out, mmeb200_tensor* scale, mmeb200_tensor* sum, const mmeb200_tensor* x,
+                     const mmeb200_tensor* residual, const mmeb200_tensor* gamma, float eps, int scale_mode);
+
+/* Gradient of mmeb200_rms_norm; `x` is what was normed (the forward call's x, or its `sum`), dy the gradient of out, dsum
+ * (may be NULL) the gradient that reaches `sum` along the residual stream. With u = x / sqrt(mean(x^2) + eps), a = dy * gamma:
+ *   dx = (a - u * mean(a * u)) / sqrt(...) + dsum   -- the gradient of x and of the residual alike
+ *   dgamma = sum over rows of dy * u                -- fp32, dense; may be NULL
+ * dx, dy, x and dsum have one type (bf16 or fp32); dx may be the same tensor as any of the others. The gradient of an 8-bit
+ * output's rounding is taken as one. Sums have a fixed order: results are equal run to run.
+ *   workspace: fp32 device tensor of mmeb200_rms_norm_grad_workspace bytes for the partial sums of dgamma, not shared by calls
+ *   that may overlap; NULL takes the context's scratch memory (refused while capturing). */
+int mmeb200_rms_norm_grad(mmeb200_ctx* ctx, mmeb200_tensor* dx, mmeb200_tensor* dgamma, const mmeb200_tensor* dy, const mmeb200_tensor* x,
+                          const mmeb200_tensor* gamma, const mmeb200_tensor* dsum, float eps, mmeb200_tensor* workspace);
+size_t mmeb200_rms_norm_grad_workspace(const mmeb200_ctx* ctx, uint64_t rows, uint64_t cols);
+
+/* 8-bit codes of x (bf16 or fp32). op MMEB200_OP_MEMCPY: out has x's sizes, one scale per row. MMEB200_OP_TRANS (2-D): out is
+ * x transposed, one scale per column of x -- a weight stored with its output channels contiguous becomes the operand
+ * mmeb200_scaled_gemm takes. */
+int mmeb200_quantize(mmeb200_ctx* ctx, mmeb200_tensor* out, mmeb200_tensor* scale, const mmeb200_tensor* x, int op, int scale_mode);
+
+/* Product of 8-bit operands with a scale for each token and channel, both [K, rows] with K contiguous (op MMEB200_OP_ABT):
+ *   out[n, m] = (sum_k x[k, m] * w[k, n]) * x_scale[m] * w_scale[n] + bias[n],  rounded once.
+ *   x, w: both int8 (any code, -128 included; the sum is exact, K <= 131071), or both fp8 (1-4-3 'minimal' or 1-5-2 'full', any
+ *   exponent bias; fp32 sum on the tensor cores). x_scale, w_scale: dense fp32, one element per row or one for all.
+ *   bias: bf16 or fp32, dense, may be NULL. out: bf16 or fp32, any row pitch. K = 0 gives the bias, or zeros.
+ * Operands whose rows do not start on 16-byte boundaries are copied to scratch memory first (refused while capturing). */
+int mmeb200_scaled_gemm(mmeb200_ctx* ctx, mmeb200_tensor* out, const mmeb200_tensor* x, const mmeb200_tensor* x_scale, const mmeb200_tensor* w,
+                        const mmeb200_tensor* w_scale, const mmeb200_tensor* bias, int op);
 
 /* Number of kernels this library has launched on the context since creation. */
 uint64_t mmeb200_launch_count(const mmeb200_ctx* ctx);

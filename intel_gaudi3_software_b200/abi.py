@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libmme_b200.so")
 
 # EMmeDataType values (mme/include/mme_common/mme_common_enum.h:32-62)
 FP8_143, FP8_152, FP16, BF16, FP32, FP32_IEEE, TF32 = 9, 10, 11, 12, 13, 14, 15
+INT8 = 64   # a type of the 8-bit layer operators only
 # EMmeOpType values (mme_common_enum.h:83-102)
 OP_FWD, OP_DEDX, OP_DEDW, OP_DET_DEDW, OP_TRANSPOSED_DEDX = 0, 1, 2, 3, 4
 OP_AB, OP_ABT, OP_ATB, OP_ATBT = 5, 6, 7, 8
@@ -26,12 +27,14 @@ RED_ADD, RED_SUB, RED_MIN, RED_MAX, RED_MAX_0, RED_NONE = 0, 1, 2, 3, 4, 5
 CHIP_GAUDI, CHIP_GAUDI2, CHIP_GAUDI3 = 0, 1, 2
 MEM_HOST, MEM_DEVICE = 0, 1
 RNG_LFSR, RNG_PHILOX = 0, 1
+SCALE_ROW, SCALE_GIVEN = 0, 1
+STREAM_LEGACY = 1   # cudaStreamLegacy, for set_stream: the default stream's handle, 0, means the context's own stream there
 
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_TIMEOUT, ERR_NO_DEVICE, ERR_DEVICE_WAIT = 0, -1, -2, -3, -4, -5, -6
 
-ELEM_SIZE = {FP8_143: 1, FP8_152: 1, BF16: 2, FP16: 2, FP32: 4, FP32_IEEE: 4, TF32: 4}
+ELEM_SIZE = {FP8_143: 1, FP8_152: 1, BF16: 2, FP16: 2, FP32: 4, FP32_IEEE: 4, TF32: 4, INT8: 1}
 NP_DTYPE = {FP8_143: np.uint8, FP8_152: np.uint8, BF16: np.uint16, FP16: np.uint16, FP32: np.float32,
-            FP32_IEEE: np.float32, TF32: np.float32}
+            FP32_IEEE: np.float32, TF32: np.float32, INT8: np.int8}
 
 
 class Tensor(C.Structure):
@@ -176,6 +179,11 @@ SYMBOLS = {
     "mmeb200_peer_open": (C.c_int, [C.c_void_p, C.c_char_p, P(C.c_void_p)]),
     "mmeb200_peer_close": (C.c_int, [C.c_void_p, C.c_void_p]),
     "mmeb200_conv_dedw_allreduce": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(ConvParams), P(PeerGroup)]),
+    "mmeb200_rms_norm": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), C.c_float, C.c_int]),
+    "mmeb200_rms_norm_grad": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), C.c_float, P(Tensor)]),
+    "mmeb200_rms_norm_grad_workspace": (C.c_size_t, [C.c_void_p, C.c_uint64, C.c_uint64]),
+    "mmeb200_quantize": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), C.c_int, C.c_int]),
+    "mmeb200_scaled_gemm": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), P(Tensor), C.c_int]),
     "mmeb200_gemm_splitk_static": (C.c_int, [C.c_void_p, P(Tensor), P(Tensor), P(Tensor), C.c_int, C.c_int]),
 }
 

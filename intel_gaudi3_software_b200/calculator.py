@@ -141,6 +141,27 @@ class Calculator:
         that may not allocate (see include/mme_b200.h). Device tensors only."""
         self._check(self.lib.mmeb200_gemm_splitk_static(self.ctx, out, x, w, op, splits))
 
+    # ---- the 8-bit layer (include/mme_b200.h has the definitions) ---------------------------
+    def rms_norm(self, out, x, gamma, eps, residual=None, sum=None, scale=None, scale_mode=abi.SCALE_ROW):
+        """out = h / sqrt(mean(h^2) + eps) * gamma for the rows h = x + residual (kept in `sum`); an 8-bit out has a `scale` per row."""
+        self._check(self.lib.mmeb200_rms_norm(self.ctx, out, scale, sum, x, residual, gamma, eps, scale_mode))
+
+    def rms_norm_grad(self, dx, dgamma, dy, x, gamma, eps, dsum=None, workspace=None):
+        """Gradient of rms_norm at what was normed (`x`, or the forward call's `sum`): dx, and dgamma unless it is None."""
+        self._check(self.lib.mmeb200_rms_norm_grad(self.ctx, dx, dgamma, dy, x, gamma, dsum, eps, workspace))
+
+    def rms_norm_grad_workspace(self, rows, cols):
+        """Bytes of the workspace that a captured rms_norm_grad takes."""
+        return int(self.lib.mmeb200_rms_norm_grad_workspace(self.ctx, rows, cols))
+
+    def quantize(self, out, scale, x, op=abi.OP_MEMCPY, scale_mode=abi.SCALE_ROW):
+        """8-bit codes of x with a scale per row; OP_TRANS: of x transposed, with a scale per column of x."""
+        self._check(self.lib.mmeb200_quantize(self.ctx, out, scale, x, op, scale_mode))
+
+    def scaled_gemm(self, out, x, x_scale, w, w_scale, bias=None, op=abi.OP_ABT):
+        """out[m][n] = (sum_k x[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n] for int8 or fp8 operands."""
+        self._check(self.lib.mmeb200_scaled_gemm(self.ctx, out, x, x_scale, w, w_scale, bias, op))
+
     # ---- state and plumbing -----------------------------------------------------------------
     def get_lfsr(self, n=256):
         regs = np.zeros(n, dtype=np.uint32)

@@ -15,9 +15,11 @@
 
 #include "gemm_launch.h"
 #include "gemm_sm100.cuh"
+#include "gemm_tokens.h"
 #include "gaudi3_exact.cuh"
 #include "kernels.cuh"
 #include "mme_b200.h"
+#include "norm_quant.h"
 
 using namespace mmeb200;
 
@@ -78,6 +80,10 @@ struct mmeb200_ctx {
     float* sk_ws = nullptr;
     uint32_t* sk_flags = nullptr;
     uint32_t sk_slots_cap = 0, sk_gen = 0;
+    // scratch of the 8-bit layer operators (layer_api.cuh); the event marks its last use, whatever stream that was on
+    void* layer_ws = nullptr;
+    size_t layer_ws_bytes = 0;
+    cudaEvent_t layer_ws_used = nullptr;
 
     int fail(int code, const char* fmt, ...) {
         char buf[512];
@@ -187,7 +193,7 @@ struct Staged {
 static int stage_in(mmeb200_ctx* c, const mmeb200_tensor* src, Staged* s, bool copy_contents) {
     s->t = *src;
     s->host = nullptr;
-    s->bytes = span_elems(src) * dtype_size(src->dtype);
+    s->bytes = span_elems(src) * (src->dtype == MMEB200_INT8 ? 1 : dtype_size(src->dtype));
     if (src->mem_space == MMEB200_MEM_DEVICE) return 0;
     void* d = nullptr;
     TRY(arena_alloc(c, &d, s->bytes));
@@ -1159,6 +1165,11 @@ void mmeb200_destroy(mmeb200_ctx* c) {
     if (c->aux) cudaFree(c->aux);
     if (c->sk_ws) cudaFree(c->sk_ws);
     if (c->sk_flags) cudaFree(c->sk_flags);
+    if (c->layer_ws_used) {
+        cudaEventSynchronize(c->layer_ws_used);
+        cudaEventDestroy(c->layer_ws_used);
+    }
+    if (c->layer_ws) cudaFree(c->layer_ws);
     if (c->d_status) cudaFree(c->d_status);
     if (c->h_status) cudaFreeHost(c->h_status);
     if (c->d_jump) cudaFree(c->d_jump);
@@ -2240,3 +2251,5 @@ extern "C" int mmeb200_gemm_splitk_static(mmeb200_ctx* c, mmeb200_tensor* out, c
     CUDA_OK(c, cudaGetLastError());
     return 0;
 }
+
+#include "layer_api.cuh"

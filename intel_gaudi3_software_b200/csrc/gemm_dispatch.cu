@@ -17,6 +17,11 @@ LaunchResult launch_gemm_pair(const LaunchEnv& env, uint32_t kind, int epi_group
     return kind == KIND_F16 ? launch_pair_f16_e1(env, p, tiles) : kind == KIND_TF32 ? launch_pair_tf32_e1(env, p, tiles) : launch_pair_f8_e1(env, p, tiles);
 }
 
+LaunchResult launch_gemm_pair_scaled(const LaunchEnv& env, uint32_t kind, int epi_groups, const GemmParams& p, uint64_t tiles) {
+    if (epi_groups == 2) return kind == KIND_I8 ? launch_scaled_i8_e2(env, p, tiles) : launch_scaled_f8_e2(env, p, tiles);
+    return kind == KIND_I8 ? launch_scaled_i8_e1(env, p, tiles) : launch_scaled_f8_e1(env, p, tiles);
+}
+
 int gemm_pair_capacity(const LaunchEnv& env, uint32_t kind, int epi_groups) {
     if (epi_groups == 2)
         return kind == KIND_F16 ? launch_pair_f16_e2_capacity(env) : kind == KIND_TF32 ? launch_pair_tf32_e2_capacity(env) : launch_pair_f8_e2_capacity(env);

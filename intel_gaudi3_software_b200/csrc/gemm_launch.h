@@ -35,6 +35,9 @@ LaunchResult launch_gemm_pair(const LaunchEnv& env, uint32_t kind, int epi_group
 // Number of CTA pairs the device can hold at once for the given variant (0 on failure).
 int gemm_pair_capacity(const LaunchEnv& env, uint32_t kind, int epi_groups);
 
+// Scaled products (8-bit operands, p.scaled applied in the epilogue), CTA-pair kernel: kind is KIND_F8 or KIND_I8.
+LaunchResult launch_gemm_pair_scaled(const LaunchEnv& env, uint32_t kind, int epi_groups, const GemmParams& p, uint64_t tiles);
+
 #define MMEB200_DECLARE_SINGLE(NAME) LaunchResult NAME(const LaunchEnv& env, const GemmParams& p, unsigned grid);
 #define MMEB200_DECLARE_PAIR(NAME)                                                      \
     LaunchResult NAME(const LaunchEnv& env, const GemmParams& p, uint64_t tiles);        \
@@ -54,6 +57,10 @@ MMEB200_DECLARE_PAIR(launch_pair_f8_e2)
 MMEB200_DECLARE_PAIR(launch_pair_f16_e2_cut)
 MMEB200_DECLARE_PAIR(launch_pair_tf32_e2_cut)
 MMEB200_DECLARE_PAIR(launch_pair_f8_e2_cut)
+MMEB200_DECLARE_PAIR(launch_scaled_f8_e1)
+MMEB200_DECLARE_PAIR(launch_scaled_i8_e1)
+MMEB200_DECLARE_PAIR(launch_scaled_f8_e2)
+MMEB200_DECLARE_PAIR(launch_scaled_i8_e2)
 #undef MMEB200_DECLARE_SINGLE
 #undef MMEB200_DECLARE_PAIR
 

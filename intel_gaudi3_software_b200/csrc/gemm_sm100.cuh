@@ -32,7 +32,7 @@ constexpr int kGemmThreads = 256;
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s
 
 enum : uint32_t { A_TILED = 0, A_IM2COL = 1 };
-enum : uint32_t { KIND_F16 = 0, KIND_TF32 = 1, KIND_F8 = 2 };
+enum : uint32_t { KIND_F16 = 0, KIND_TF32 = 1, KIND_F8 = 2, KIND_I8 = 3 };
 enum : uint32_t { EPI_GENERIC = 0, EPI_F32 = 1, EPI_BF16_RNE = 2, EPI_FP8_HW = 3 };
 enum : uint32_t {
     WAIT_OK = 0,
@@ -65,6 +65,16 @@ struct ConvGeom {
     // out_h x out_w grid is stored at element out_base + n * out_stride_n + i * out_stride_h + j * out_stride_w.
     int32_t out_grid;            // 0: rows are out_ld apart
     int64_t out_base, out_stride_n, out_stride_h, out_stride_w;
+};
+
+// What the epilogue of a scaled product reads beside the accumulator. Strides are 0 (one scale for all) or 1.
+struct ScaledOut {
+    const float* row_scale;
+    const float* col_scale;
+    const void* col_bias;       // nullptr: none
+    uint32_t row_stride, col_stride;
+    uint32_t bias_bf16;         // element type of col_bias: bf16, else fp32
+    uint32_t col_vec;           // col_scale and col_bias may be read 16 bytes at a time
 };
 
 struct GemmParams {
@@ -117,6 +127,8 @@ struct GemmParams {
     float* sk_ws;            // [slot][CTA of the pair][column 0..255][row 0..127] floats: 128 KB per CTA
     uint32_t* sk_flags;      // [slot][CTA of the pair][16]: one word per epilogue warp of the writer
     uint32_t sk_gen;         // differs from every earlier launch that used the same flags; never 0
+    // Scaled products (the SCALED instantiations): out = acc * row_scale[m] * col_scale[n] + col_bias[n]
+    ScaledOut scaled;
 };
 constexpr uint32_t kSkSlotFloats = 8 * kBlockM * 32;   // one CTA's 128 x 256 partial accumulator
 constexpr uint32_t kSkFlagsPerCta = 16;
@@ -582,10 +594,71 @@ __device__ __forceinline__ void store_row32(const uint32_t (&v)[32], uint8_t* ds
     }
 }
 
+__device__ __forceinline__ float scaled_bias(const ScaledOut& so, uint32_t n) {
+    return so.bias_bf16 ? __uint_as_float(uint32_t(static_cast<const uint16_t*>(so.col_bias)[n]) << 16) : static_cast<const float*>(so.col_bias)[n];
+}
+// The accumulator as a number: integer accumulators are exact and rounded once here (24 bits hold what the output keeps).
+template <int KIND>
+__device__ __forceinline__ float scaled_acc(uint32_t v) {
+    if constexpr (KIND == KIND_I8) return __int2float_rn(int(v));
+    else return __uint_as_float(v);
+}
+// 32 accumulator columns from col0 on of a row whose scale is xs -> packed bf16 or fp32 outputs, rounded once.
+// Only the first `ncols` columns exist; the rest of v is left undefined.
+template <int KIND>
+__device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const GemmParams& p, float xs, uint32_t col0, uint32_t out_elem) {
+    const ScaledOut& so = p.scaled;
+    const bool whole = so.col_vec && col0 + 32 <= p.N;
+    const float same = so.col_stride ? 0.0f : so.col_scale[0];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        float w[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (whole) {
+            const float4 t = __ldg(reinterpret_cast<const float4*>(so.col_scale + col0) + q);
+            w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
+            if (so.col_bias) {
+                if (so.bias_bf16) {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(so.col_bias) + col0) + q);
+                    b[0] = __uint_as_float(u.x << 16); b[1] = __uint_as_float(u.x & 0xFFFF0000u);
+                    b[2] = __uint_as_float(u.y << 16); b[3] = __uint_as_float(u.y & 0xFFFF0000u);
+                } else {
+                    const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(so.col_bias) + col0) + q);
+                    b[0] = u.x; b[1] = u.y; b[2] = u.z; b[3] = u.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t n = col0 + 4 * q + e;
+                w[e] = same;
+                if (n < p.N) {
+                    if (so.col_stride) w[e] = so.col_scale[n];
+                    if (so.col_bias) b[e] = scaled_bias(so, n);
+                }
+            }
+        }
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = scaled_acc<KIND>(v[4 * q + e]) * xs * w[e];
+        if (so.col_bias) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] += b[e];
+        }
+        if (out_elem == 2) {   // words 2q, 2q + 1 lie below every value still to be read
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q]) : "f"(y[1]), "f"(y[0]));
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q + 1]) : "f"(y[3]), "f"(y[2]));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * q + e] = __float_as_uint(y[e]);
+        }
+    }
+}
+
 // Epilogue of one output tile, run by one epilogue warp for its 32 rows: reads `tile_cols` accumulator columns (a
 // multiple of 32) from tensor memory (tmem_acc = the warp's lane window of the tile's accumulator), converts and stores
 // them. m0 is the first row of the CTA's 128-row block, n0 the first column.
-template <bool FIX = false>
+// SCALED: -1, or the KIND_* of a scaled product (epilogue_scaled takes the place of the cast).
+template <bool FIX = false, int SCALED = -1>
 __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile_cols, uint32_t m0, uint32_t n0, uint32_t batch, uint32_t split,
                                               uint32_t tmem_acc, uint8_t* stage_out, uint32_t& store_buf, uint32_t sub, uint32_t lane,
                                               uint32_t out_elem, const SkFix& fix = SkFix{nullptr, 0u, 0u}) {
@@ -610,6 +683,10 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile
         flat_row = base_off;
     } else {
         base_off = bi[0] * p.out_bstride[0] + bi[1] * p.out_bstride[1] + bi[2] * p.out_bstride[2] + uint64_t(row) * p.out_ld;
+    }
+    float xs = 0.0f;
+    if constexpr (SCALED >= 0) {
+        if (row < p.M) xs = p.scaled.row_scale[uint64_t(row) * p.scaled.row_stride] * p.scale;   // p.scale: the power of two of the operands' exponent biases
     }
     uint32_t done_cols = 0;   // columns of the tile already stored
     if (p.tma_store) {
@@ -637,7 +714,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile
                 tmem_ld_32x32b_x32(tmem_acc + ch * cols_per_chunk + l * 32, v);
                 if constexpr (FIX) tmem_ld_wait_add(v, fix, fix.col0 + ch * cols_per_chunk + l * 32, sub * 32 + lane);
                 else tmem_ld_wait();
-                epilogue_convert(v, p, out_elem, flat_row + col0 + l * 32);
+                if constexpr (SCALED >= 0) epilogue_scaled<SCALED>(v, p, xs, col0 + l * 32, out_elem);
+                else epilogue_convert(v, p, out_elem, flat_row + col0 + l * 32);
                 if (out_elem == 4) {
 #pragma unroll
                     for (uint32_t q = 0; q < 8; ++q)
@@ -679,7 +757,8 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile
         } else {
             elem = out_elem;
             dst = reinterpret_cast<uint8_t*>(p.out) + (base_off + col0) * out_elem;
-            epilogue_convert(v, p, out_elem, flat_row + col0);
+            if constexpr (SCALED >= 0) epilogue_scaled<SCALED>(v, p, xs, col0, out_elem);
+            else epilogue_convert(v, p, out_elem, flat_row + col0);
         }
         store_row32(v, dst, elem, ncols);   // v[0 .. 8*elem) holds 32 packed outputs
     }

@@ -45,7 +45,8 @@ struct PairSmem {
 // columns from rank * tile_n / 2 on (whole 128-byte groups of an MN-major B: up to 16 bytes' worth of columns more than it
 // needs), and the epilogue leaves the columns after tile_n to the next tile.
 // CUT: the instantiation that can run a cut tail (p.sk_tiles != 0); the others carry none of its code.
-template <int KIND, int EPI_GROUPS, bool CUT = false>
+// SCALED: the epilogue applies p.scaled (8-bit products with a scale for each row and column) in place of a cast.
+template <int KIND, int EPI_GROUPS, bool CUT = false, bool SCALED = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairSmem<EPI_GROUPS>::kThreads, 1)
     gemm_tcgen05_pair_kernel(const __grid_constant__ GemmParams p) {
     using S = PairSmem<EPI_GROUPS>;
@@ -235,8 +236,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairSmem<EPI_GROUPS>
                                         stage_out, store_buf, sub, lane, out_elem, fix);
                 }
             } else {
-                epilogue_tile(p, group_cols, tc.m0 * 2 + rank * kBlockM, tc.n0 * p.tile_n + grp * kGroupCols, tc.batch, tc.split, tmem_acc,
-                              stage_out, store_buf, sub, lane, out_elem);
+                epilogue_tile<false, SCALED ? KIND : -1>(p, group_cols, tc.m0 * 2 + rank * kBlockM, tc.n0 * p.tile_n + grp * kGroupCols, tc.batch, tc.split,
+                                                         tmem_acc, stage_out, store_buf, sub, lane, out_elem);
             }
             tc_fence_before_sync();
             __syncwarp();

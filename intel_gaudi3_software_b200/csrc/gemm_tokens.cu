@@ -1,0 +1,77 @@
+// Launcher of the few-token product kernel; see gemm_tokens.h.
+#include "gemm_tokens.cuh"
+
+#include <cstring>
+
+namespace mmeb200 {
+
+constexpr int kTokenSmem = 227 * 1024;
+
+static uint32_t stages_for(uint32_t tok) {
+    const uint32_t bytes = kTokenWBytes + tok * kRowBytes, n = (kTokenSmem - kTokenBarrierBytes) / bytes;
+    return n < kTokenMaxStages ? n : kTokenMaxStages;
+}
+
+template <int KIND>
+static cudaError_t configure(const LaunchEnv& env, uint32_t tok, uint32_t splits, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs) {
+    static bool done[64] = {};
+    if (!done[env.device & 63]) {
+        const cudaError_t e = cudaFuncSetAttribute(gemm_tokens_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTokenSmem);
+        if (e != cudaSuccess) return e;
+        done[env.device & 63] = true;
+    }
+    memset(cfg, 0, sizeof *cfg);
+    cfg->blockDim = dim3(kTokenThreads);
+    cfg->dynamicSmemBytes = stages_for(tok) * (kTokenWBytes + tok * kRowBytes) + kTokenBarrierBytes;
+    cfg->stream = env.stream;
+    attrs[0].id = cudaLaunchAttributeClusterDimension;
+    attrs[0].val.clusterDim.x = splits; attrs[0].val.clusterDim.y = 1; attrs[0].val.clusterDim.z = 1;
+    attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg->attrs = attrs;
+    cfg->numAttrs = env.dependent_launch ? 2 : 1;
+    return cudaSuccess;
+}
+
+template <int KIND>
+static LaunchResult launch(const LaunchEnv& env, TokenGemmParams& p) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attrs[2];
+    cudaError_t e = configure<KIND>(env, p.tok, p.splits, &cfg, attrs);
+    if (e != cudaSuccess) return {e, LAUNCH_OK, "cudaFuncSetAttribute(few-token kernel)"};
+    p.stage_bytes = kTokenWBytes + p.tok * kRowBytes;
+    p.stages = stages_for(p.tok);
+    p.tmem_cols = 32;
+    while (p.tmem_cols < p.tok) p.tmem_cols *= 2;
+    cfg.gridDim = dim3(p.splits * ((p.N + kBlockM - 1) / kBlockM), (p.M + p.tok - 1) / p.tok);
+    e = cudaLaunchKernelEx(&cfg, gemm_tokens_kernel<KIND>, p);
+    return {e != cudaSuccess ? e : cudaGetLastError(), LAUNCH_OK, "few-token kernel launch"};
+}
+
+LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmParams p) {
+    return kind == KIND_I8 ? launch<KIND_I8>(env, p) : launch<KIND_F8>(env, p);
+}
+
+template <int KIND>
+static int capacity(const LaunchEnv& env, uint32_t tok, uint32_t splits) {
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attrs[2];
+    if (configure<KIND>(env, tok, splits, &cfg, attrs) != cudaSuccess) return 0;
+    cfg.gridDim = dim3(splits * unsigned(env.sm_count));
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, gemm_tokens_kernel<KIND>, &cfg) != cudaSuccess) return 0;
+    return n * int(splits);
+}
+
+LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p) {
+    const uint64_t blocks = (uint64_t(p.M) * p.N + 255) / 256, most = uint64_t(env.sm_count) * 8;
+    gemm_empty_sum_kernel<<<unsigned(blocks < most ? blocks : most), 256, 0, env.stream>>>(p);
+    return {cudaGetLastError(), LAUNCH_OK, "empty-sum kernel launch"};
+}
+
+int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits) {
+    return kind == KIND_I8 ? capacity<KIND_I8>(env, tok, splits) : capacity<KIND_F8>(env, tok, splits);
+}
+
+}  // namespace mmeb200

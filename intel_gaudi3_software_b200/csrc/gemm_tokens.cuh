@@ -1,0 +1,202 @@
+// Scaled 8-bit product for few tokens (or few output tiles): out[m][n] = acc * row_scale[m] * col_scale[n] + bias[n].
+//
+// With few tokens the weights are what has to be read, once, and everything else is small, so the weights take the MMA's
+// 128-row side and the tokens its N side: a CTA accumulates (128 output channels) x (tok tokens), tok a multiple of 16 that
+// just holds the tokens, and the padding costs neither bandwidth nor shared memory. Tensor cores at this shape consume
+// 64 bytes of weights per clock and SM, above what HBM delivers, so the kernel is bound by the weights' stream; a ring of
+// 128-byte-wide stages that fills the SM's shared memory keeps it fed.
+//
+// One column of channel tiles rarely fills 148 SMs, so the k blocks are split over the CTAs of a cluster. Their partial
+// accumulators meet in distributed shared memory: every CTA owns a share of the tile's tokens, receives the others' partial
+// sums for them, adds them in rank order (integer sums are exact anyway; fp32 sums have a fixed order) and writes them
+// out. No workspace in global memory, no second launch, no atomics.
+//
+// CTA layout (192 threads): warp 0 feeds the ring by TMA, warp 1 allocates tensor memory and issues the MMAs, warps 2-5 are
+// the epilogue (lane = channel). Every mbarrier wait is bounded as in the other GEMM kernels.
+#pragma once
+#include "gemm_tokens.h"
+
+namespace mmeb200 {
+
+constexpr int kTokenThreads = 192;
+constexpr uint32_t kTokenBarrierBytes = 256;
+constexpr uint32_t kTokenWBytes = kBlockM * kRowBytes;
+constexpr uint32_t kTokenMaxStages = 12;
+
+// The outputs of one token: 32 lanes write 32 consecutive channels.
+__device__ __forceinline__ void token_store(const TokenGemmParams& p, uint32_t m, uint32_t n, float acc, float xs, float ws, float bias) {
+    float y = acc * xs * ws;
+    if (p.scaled.col_bias) y += bias;
+    if (p.out_bf16) {
+        uint32_t w;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(0.0f), "f"(y));
+        static_cast<uint16_t*>(p.out)[uint64_t(m) * p.out_ld + n] = uint16_t(w);
+    } else {
+        static_cast<float*>(p.out)[uint64_t(m) * p.out_ld + n] = y;
+    }
+}
+
+template <int KIND>
+__global__ void __launch_bounds__(kTokenThreads, 1) gemm_tokens_kernel(const __grid_constant__ TokenGemmParams p) {
+    griddep_launch_dependents();
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) & 1023u) {   // uniform over the cluster
+        if (threadIdx.x == 0) atomicCAS(p.status, 0u, SMEM_MISALIGNED);
+        return;
+    }
+    const uint32_t stages = p.stages, stage_bytes = p.stage_bytes;
+    uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + stages * stage_bytes);
+    uint64_t* empty_bar = full_bar + kTokenMaxStages;
+    uint64_t* done_bar = empty_bar + kTokenMaxStages;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done_bar + 1);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = blockIdx.x % p.splits, n0 = (blockIdx.x / p.splits) * kBlockM, m0 = blockIdx.y * p.tok;
+    const uint32_t per = (p.num_k_blocks + p.splits - 1) / p.splits;
+    const uint32_t kb0 = rank * per, kb1 = min(p.num_k_blocks, kb0 + per);   // the planner leaves no share empty
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < stages; ++s) {
+            mbar_init(&full_bar[s], 1);
+            mbar_init(&empty_bar[s], 1);
+        }
+        mbar_init(done_bar, 1);
+        fence_mbar_init();
+        tma_prefetch_desc(&p.tm_w);
+        tma_prefetch_desc(&p.tm_x);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_holder, p.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_holder;
+    griddep_wait();
+
+    const uint32_t sub = warp & 3, n = n0 + sub * 32 + lane;   // epilogue: this lane's channel
+    float ws = 0.0f, bias = 0.0f;
+    bool ready = true;
+    if (warp == 0) {
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_bounded(&empty_bar[stage], phase ^ 1, kWaitLimitNs)) {
+                    atomicCAS(p.status, 0u, WAIT_PRODUCER_EMPTY);
+                    break;
+                }
+                uint8_t* dst = smem + stage * stage_bytes;
+                mbar_arrive_expect_tx(&full_bar[stage], stage_bytes);
+                tma_load_5d(dst, &p.tm_w, &full_bar[stage], int(kb * kRowBytes), int(n0), 0, 0, 0);
+                tma_load_5d(dst + kTokenWBytes, &p.tm_x, &full_bar[stage], int(kb * kRowBytes), int(m0), 0, 0, 0);
+                if (++stage == stages) { stage = 0; phase ^= 1; }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (elect_one()) {
+            uint32_t stage = 0, phase = 0, accumulate = 0;
+            const uint64_t w_desc0 = make_smem_desc(smem_u32(smem), 16, 1024);
+            bool ok = true;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                if (!mbar_wait_bounded(&full_bar[stage], phase, kWaitLimitNs)) {
+                    atomicCAS(p.status, 0u, WAIT_MMA_FULL);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after_sync();
+                const uint64_t w_desc = w_desc0 + ((stage * stage_bytes) >> 4);
+                const uint64_t x_desc = w_desc + (kTokenWBytes >> 4);
+#pragma unroll
+                for (uint32_t k = 0; k < kRowBytes / kUmmaKBytes; ++k) {
+                    umma_ss<KIND>(tmem_base, w_desc + k * (kUmmaKBytes >> 4), x_desc + k * (kUmmaKBytes >> 4), p.idesc, accumulate);
+                    accumulate = 1;
+                }
+                umma_commit(&empty_bar[stage]);
+                if (++stage == stages) { stage = 0; phase ^= 1; }
+            }
+            if (ok) umma_commit(done_bar);
+        }
+        __syncwarp();
+    } else {
+        if (n < p.N) {
+            ws = p.scaled.col_scale[uint64_t(n) * p.scaled.col_stride];
+            if (p.scaled.col_bias) bias = scaled_bias(p.scaled, n);
+        }
+        ready = mbar_wait_bounded(done_bar, 0, kWaitLimitNs);
+        ready = __all_sync(0xffffffffu, ready);
+        if (!ready) atomicCAS(p.status, 0u, WAIT_EPILOGUE_TMEM_FULL);
+        tc_fence_after_sync();
+    }
+
+    const uint32_t tokens = min(p.tok, p.M - m0);
+    if (p.splits == 1) {
+        if (warp >= 2 && ready) {
+            for (uint32_t c0 = 0; c0 < tokens; c0 += 16) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem_base + c0 + ((sub * 32) << 16), v);
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    const uint32_t m = m0 + c0 + j;
+                    if (c0 + j < tokens && n < p.N)
+                        token_store(p, m, n, scaled_acc<KIND>(v[j]), p.scaled.row_scale[uint64_t(m) * p.scaled.row_stride] * p.scale, ws, bias);
+                }
+            }
+        }
+    } else {
+        // Every CTA's stages are idle (its MMAs have completed) before anyone writes into them.
+        cluster_sync_all();
+        const uint32_t share = (tokens + p.splits - 1) / p.splits;   // tokens a rank owns
+        uint32_t* inbox = reinterpret_cast<uint32_t*>(smem);         // [source rank][token of the share][channel]
+        if (warp >= 2 && ready) {
+            const uint32_t channel = sub * 32 + lane;
+            for (uint32_t c0 = 0; c0 < tokens; c0 += 16) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem_base + c0 + ((sub * 32) << 16), v);
+                tmem_ld_wait();
+#pragma unroll
+                for (uint32_t j = 0; j < 16; ++j) {
+                    if (c0 + j < tokens) {
+                        const uint32_t owner = (c0 + j) / share, t = (c0 + j) - owner * share;
+                        st_shared_cluster_u32(mapa_shared(smem_u32(inbox + (rank * share + t) * kBlockM + channel), owner), v[j]);
+                    }
+                }
+            }
+        }
+        cluster_sync_all();
+        if (warp >= 2) {
+            const uint32_t channel = sub * 32 + lane;
+            for (uint32_t t = 0; t < share; ++t) {
+                const uint32_t m = m0 + rank * share + t;
+                if (rank * share + t >= tokens) break;
+                uint32_t sum = inbox[t * kBlockM + channel];
+                for (uint32_t r = 1; r < p.splits; ++r) {
+                    const uint32_t v = inbox[(r * share + t) * kBlockM + channel];
+                    if constexpr (KIND == KIND_I8) sum += v;
+                    else sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
+                }
+                if (n < p.N) token_store(p, m, n, scaled_acc<KIND>(sum), p.scaled.row_scale[uint64_t(m) * p.scaled.row_stride] * p.scale, ws, bias);
+            }
+        }
+    }
+
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, p.tmem_cols);
+    }
+}
+
+// No common dimension: the sums are empty and the bias, or zero, is the result.
+static __global__ void __launch_bounds__(256) gemm_empty_sum_kernel(const __grid_constant__ TokenGemmParams p) {
+    griddep_wait();
+    const uint64_t total = uint64_t(p.M) * p.N;
+    for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
+        const uint32_t m = uint32_t(i / p.N), n = uint32_t(i % p.N);
+        token_store(p, m, n, 0.0f, 0.0f, 0.0f, p.scaled.col_bias ? scaled_bias(p.scaled, n) : 0.0f);
+    }
+}
+
+}  // namespace mmeb200

@@ -1,0 +1,36 @@
+// Host-side launcher of the few-token product kernel (gemm_tokens.cuh).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "gemm_launch.h"
+
+namespace mmeb200 {
+
+struct TokenGemmParams {
+    CUtensorMap tm_w, tm_x;     // (K, channels) and (K, tokens); boxes 128 B x 128 rows and 128 B x tok rows
+    uint32_t M, N;              // tokens, output channels
+    uint32_t num_k_blocks;      // 128-byte blocks of K
+    uint32_t tok;               // tokens of a tile (a multiple of 16, at most 256)
+    uint32_t splits;            // CTAs of a cluster, each with its share of the k blocks
+    uint32_t stages, stage_bytes;
+    uint32_t tmem_cols;
+    uint32_t idesc;
+    float scale;                // power of two of the operands' exponent biases
+    ScaledOut scaled;
+    void* out;
+    uint32_t out_bf16;
+    uint64_t out_ld;
+    uint32_t* status;
+};
+
+// Fills stages, stage_bytes and tmem_cols for p.tok and launches on a grid of splits x channel tiles x token tiles.
+LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmParams p);
+// out = bias (or zero) for operands without a common dimension.
+LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p);
+// Most CTAs the device runs at once in clusters of `splits` with tiles of `tok` tokens (0 on failure).
+int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits);
+
+}  // namespace mmeb200

@@ -1,0 +1,81 @@
+// Host-side launchers of the row kernels (norm_quant.cu): RMS norm with the residual's addition and an optional 8-bit
+// output, its gradient, and row-wise quantisation to 8 bits. This is what api.cu sees of them.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "numerics.cuh"
+
+namespace mmeb200 {
+
+enum : int { ROW_NONE = 0, ROW_BF16 = 1, ROW_F32 = 2, ROW_I8 = 3, ROW_F8 = 4 };   // element types of the row kernels
+
+// Rows of a tensor: row r is the index of dims 1..4 with dim 1 fastest; element c of it sits at base + off(r) + c.
+struct RowTensor {
+    void* ptr;
+    int type;              // ROW_*
+    uint32_t stride[4];    // elements, dims 1..4
+};
+
+struct NormParams {
+    RowTensor x, residual, sum, out;
+    const void* gamma;     // nullptr: ones
+    int gamma_type;
+    float* scale;          // 8-bit outputs: the step of every row (written)
+    const float* given;    // 8-bit outputs with a given scale: read instead; given_stride 0 = one for all rows
+    uint32_t given_stride;
+    uint32_t rows, cols;
+    uint32_t dims[4];      // sizes of dims 1..4
+    uint32_t flat;         // 1: rows are dims[0] alone (no division per row)
+    uint32_t norm;         // 0: quantise x as it is
+    float eps;
+    float top;             // largest code of the 8-bit output
+    Fp8HwCast hw;          // ROW_F8
+};
+
+struct NormGradParams {
+    RowTensor dx, dy, x, dsum;
+    const void* gamma;
+    int gamma_type;
+    float* partial;        // [blocks][cols]; nullptr: no gradient of gamma wanted
+    uint32_t rows, cols;
+    uint32_t dims[4];
+    uint32_t flat;
+    float eps;
+};
+
+// Quantisation of columns with a transposed result: x is rows x cols (cols fastest), out cols x rows (rows fastest).
+struct QuantTransParams {
+    const void* x;
+    int x_type;
+    uint64_t x_ld, out_ld;   // elements between rows of x / of out
+    void* out;
+    int out_type;
+    float* scale;            // [cols]
+    const float* given;
+    uint32_t given_stride;
+    uint32_t rows, cols;
+    float top;
+    Fp8HwCast hw;
+};
+
+struct RowLaunch {
+    int device, sm_count;
+    cudaStream_t stream;
+    bool dependent_launch;
+};
+
+// `vec`: every row of every tensor may be read and written eight elements at a time.
+cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec);
+// Blocks the gradient kernel runs with, i.e. rows of `partial`.
+uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols);
+cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks);
+cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols);
+// Number of kernels launched is returned in *launches.
+cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int* launches);
+
+// Rows of `cols` bytes, src_ld bytes apart at any alignment, copied to rows dst_ld bytes apart (dst and dst_ld multiples of 16).
+cudaError_t launch_pad_rows(const RowLaunch& env, const void* src, void* dst, uint64_t rows, uint64_t cols, uint64_t src_ld, uint64_t dst_ld);
+
+}  // namespace mmeb200
