@@ -161,6 +161,7 @@ RowTensor layer_rows(const mmeb200_tensor* t) {
     r.ptr = t->data;
     r.type = layer_row_type(t->dtype);
     for (int d = 0; d < 4; ++d) r.stride[d] = t->strides[d + 1];
+    r.bytes = span_elems(t) * unsigned(layer_elem_size(t));
     return r;
 }
 // Merges dims 1..4 into one where every tensor's strides allow it, so that a row's place needs no division.
@@ -294,9 +295,10 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     for (int d = 0; d < 4; ++d) p.dims[d] = x->sizes[d + 1];
     layer_flatten(p.dims, &p.flat, {&p.x, &p.residual, &p.sum, &p.out});
-    p.norm = norm; p.eps = eps; p.top = top; p.hw = hw;
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.residual, p.dims) && layer_vectors(p.sum, p.dims) &&
-                     layer_vectors(p.out, p.dims) && reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
+    p.norm = norm; p.eps = eps; p.per_col = 1.0f / float(cols); p.top = top; p.hw = hw;
+    p.mode = out->dtype == DT_BF16 ? NORM_BF16 : out->dtype == DT_FP32 ? NORM_F32 : out->dtype == MMEB200_INT8 ? (given ? NORM_I8_GIVEN : NORM_I8) : given ? NORM_F8_GIVEN : NORM_F8;
+    p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
+    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.residual, p.dims) && layer_vectors(p.sum, p.dims) && layer_vectors(p.out, p.dims);
     CUDA_OK(c, launch_norm(layer_launch(c), p, vec));
     c->launches++;
     return st.finish();
@@ -368,7 +370,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     for (int d = 0; d < 4; ++d) p.dims[d] = x->sizes[d + 1];
     layer_flatten(p.dims, &p.flat, {&p.x, &p.dy, &p.dsum, &p.dx});
-    p.eps = eps;
+    p.eps = eps; p.per_col = 1.0f / float(cols);
     void* scratch = nullptr;
     if (dgamma) {
         if (workspace) p.partial = static_cast<float*>(workspace->data);
@@ -377,8 +379,9 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
             p.partial = static_cast<float*>(scratch);
         }
     }
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.dy, p.dims) && layer_vectors(p.dsum, p.dims) &&
-                     layer_vectors(p.dx, p.dims) && reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
+    p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
+    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.dy, p.dims) && layer_vectors(p.dsum, p.dims) && layer_vectors(p.dx, p.dims) &&
+                     reinterpret_cast<uintptr_t>(p.partial) % 16 == 0;
     CUDA_OK(c, launch_norm_grad(layer_launch(c), p, vec, blocks));
     c->launches++;
     if (dgamma) {
@@ -418,13 +421,14 @@ int run_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, con
     TRY(st.add(&tx, true, false));
     TRY(st.add(&to, false, true));
     TRY(st.add(&ts, given, !given));
-    p.x = tx->data; p.x_type = layer_row_type(tx->dtype); p.x_ld = tx->strides[1];
+    p.x = layer_rows(tx); p.x_ld = tx->strides[1];
     p.out = to->data; p.out_type = layer_row_type(to->dtype); p.out_ld = to->strides[1];
     if (given) { p.given = static_cast<const float*>(ts->data); p.given_stride = num_elems(ts) == 1 ? 0 : 1; }
     else p.scale = static_cast<float*>(ts->data);
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     int launches = 0;
-    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, &launches));
+    const uint32_t dims[4] = {p.rows, 1, 1, 1};
+    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, cols % 8 == 0 && layer_vectors(p.x, dims), &launches));
     c->launches += uint64_t(launches);
     return st.finish();
 }

@@ -1,52 +1,15 @@
-// Launchers of the row kernels (norm_quant.cuh): the instantiation for a row's length, types and alignment.
-#include "norm_quant.cuh"
-
+// Launchers of the row kernels: the instantiation for a call's element types and alignment, and the small kernels beside them.
 #include <algorithm>
-#include <cstring>
+
+#include "norm_quant.cuh"
+#include "norm_quant_launch.h"
 
 namespace mmeb200 {
 
-template <typename P>
-static cudaError_t launch_rows(const RowLaunch& env, void (*kern)(P), const P& p, dim3 grid, unsigned threads, size_t smem) {
-    cudaLaunchConfig_t cfg;
-    memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = env.stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = env.dependent_launch ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    return e != cudaSuccess ? e : cudaGetLastError();
-}
-
-// A row's elements are spread over T threads with at most 32 of them per thread: few enough for registers, enough for
-// the loads in flight to cover the latency of HBM. Short rows take one warp each.
 template <int XT, int RT>
 static cudaError_t norm_of(const RowLaunch& env, const NormParams& p, bool vec) {
-    const dim3 warps((p.rows + 3) / 4), blocks(p.rows);
-    if (vec) {
-        if (p.cols <= 256) return launch_rows(env, norm_kernel<XT, RT, 8, 1, 32>, p, warps, 128, 0);
-        if (p.cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, 8, 4, 32>, p, warps, 128, 0);
-        if (p.cols <= 2048) return launch_rows(env, norm_kernel<XT, RT, 8, 2, 128>, p, blocks, 128, 0);
-        if (p.cols <= 4096) return launch_rows(env, norm_kernel<XT, RT, 8, 2, 256>, p, blocks, 256, 0);
-        if (p.cols <= 8192) return launch_rows(env, norm_kernel<XT, RT, 8, 2, 512>, p, blocks, 512, 0);
-        if (p.cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, 8, 4, 512>, p, blocks, 512, 0);
-        if (p.cols <= 32768) return launch_rows(env, norm_kernel<XT, RT, 8, 4, 1024>, p, blocks, 1024, 0);
-        return launch_rows(env, norm_long_kernel<XT, RT, 8>, p, blocks, 1024, 0);
-    }
-    if (p.cols <= 256) return launch_rows(env, norm_kernel<XT, RT, 1, 8, 32>, p, warps, 128, 0);
-    if (p.cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, 1, 32, 32>, p, warps, 128, 0);
-    if (p.cols <= 2048) return launch_rows(env, norm_kernel<XT, RT, 1, 16, 128>, p, blocks, 128, 0);
-    if (p.cols <= 4096) return launch_rows(env, norm_kernel<XT, RT, 1, 16, 256>, p, blocks, 256, 0);
-    if (p.cols <= 8192) return launch_rows(env, norm_kernel<XT, RT, 1, 16, 512>, p, blocks, 512, 0);
-    if (p.cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, 1, 32, 512>, p, blocks, 512, 0);
-    return launch_rows(env, norm_long_kernel<XT, RT, 1>, p, blocks, 1024, 0);
+    return vec ? norm_of<XT, RT, false>(env, p) : norm_of<XT, RT, true>(env, p);
 }
-
 cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec) {
     const int rt = p.residual.ptr ? p.residual.type : ROW_NONE;
     if (p.x.type == ROW_BF16)
@@ -56,33 +19,18 @@ cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec) {
 
 uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols) {
     const uint32_t per_block = cols <= 1024 ? 4 : 1;
-    const uint32_t resident = cols <= 1024 ? 4 : cols <= 2048 ? 6 : cols <= 4096 ? 4 : cols <= 8192 ? 2 : 1;   // blocks an SM holds
+    // no more blocks than the SMs hold at once: a block walks its rows to the end
+    const uint32_t resident = std::max(1u, (cols <= 1024 ? 512u : 640u) / grad_threads(cols));
     return std::min<uint32_t>((rows + per_block - 1) / per_block, uint32_t(sm_count) * resident);
 }
 
-template <int XT, int DT_>
+template <int XT>
 static cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks) {
-    const dim3 g(blocks);
-    const size_t sums = p.cols <= 1024 ? p.cols * sizeof(float) : 0;
-    if (vec) {
-        if (p.cols <= 256) return launch_rows(env, norm_grad_kernel<XT, DT_, 8, 1, 32>, p, g, 128, sums);
-        if (p.cols <= 1024) return launch_rows(env, norm_grad_kernel<XT, DT_, 8, 4, 32>, p, g, 128, sums);
-        if (p.cols <= 2048) return launch_rows(env, norm_grad_kernel<XT, DT_, 8, 2, 128>, p, g, 128, 0);
-        if (p.cols <= 4096) return launch_rows(env, norm_grad_kernel<XT, DT_, 8, 2, 256>, p, g, 256, 0);
-        if (p.cols <= 8192) return launch_rows(env, norm_grad_kernel<XT, DT_, 8, 2, 512>, p, g, 512, 0);
-        return launch_rows(env, norm_grad_long_kernel<XT, DT_, 8>, p, g, 1024, 0);
-    }
-    if (p.cols <= 256) return launch_rows(env, norm_grad_kernel<XT, DT_, 1, 8, 32>, p, g, 128, sums);
-    if (p.cols <= 1024) return launch_rows(env, norm_grad_kernel<XT, DT_, 1, 32, 32>, p, g, 128, sums);
-    if (p.cols <= 2048) return launch_rows(env, norm_grad_kernel<XT, DT_, 1, 16, 128>, p, g, 128, 0);
-    if (p.cols <= 4096) return launch_rows(env, norm_grad_kernel<XT, DT_, 1, 16, 256>, p, g, 256, 0);
-    if (p.cols <= 8192) return launch_rows(env, norm_grad_kernel<XT, DT_, 1, 16, 512>, p, g, 512, 0);
-    return launch_rows(env, norm_grad_long_kernel<XT, DT_, 1>, p, g, 1024, 0);
+    if (p.dsum.ptr) return vec ? norm_grad_of<XT, true, false>(env, p, blocks) : norm_grad_of<XT, true, true>(env, p, blocks);
+    return vec ? norm_grad_of<XT, false, false>(env, p, blocks) : norm_grad_of<XT, false, true>(env, p, blocks);
 }
-
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks) {
-    if (p.x.type == ROW_BF16) return p.dsum.ptr ? norm_grad_of<ROW_BF16, ROW_BF16>(env, p, vec, blocks) : norm_grad_of<ROW_BF16, ROW_NONE>(env, p, vec, blocks);
-    return p.dsum.ptr ? norm_grad_of<ROW_F32, ROW_F32>(env, p, vec, blocks) : norm_grad_of<ROW_F32, ROW_NONE>(env, p, vec, blocks);
+    return p.x.type == ROW_BF16 ? norm_grad_of<ROW_BF16>(env, p, vec, blocks) : norm_grad_of<ROW_F32>(env, p, vec, blocks);
 }
 
 struct ColumnSums { const float* partial; float* out; uint32_t blocks, cols; };
@@ -92,32 +40,10 @@ cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float
     return launch_rows(env, column_sums_kernel, p, dim3((cols + 31) / 32), 256, 0);
 }
 
-struct ColumnSteps { float* scale; uint32_t cols; float top; };
-static __global__ void __launch_bounds__(256) column_steps_kernel(const __grid_constant__ ColumnSteps p) { column_steps(p.scale, p.cols, p.top); }
-
-cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int* launches) {
+cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, bool vec, int* launches) {
     *launches = 0;
-    const bool bf16 = p.x_type == ROW_BF16;
-    cudaError_t e = cudaSuccess;
-    if (!p.given) {
-        e = cudaMemsetAsync(p.scale, 0, size_t(p.cols) * sizeof(float), env.stream);
-        if (e != cudaSuccess) return e;
-        const uint32_t strips = (p.cols + 31) / 32;
-        const uint32_t cuts = std::max(1u, std::min((p.rows + 63) / 64, uint32_t(env.sm_count) * 8 / std::max(1u, std::min(strips, uint32_t(env.sm_count) * 8))));
-        e = launch_rows(env, bf16 ? column_max_kernel<ROW_BF16> : column_max_kernel<ROW_F32>, p, dim3(strips, cuts), 256, 0);
-        if (e != cudaSuccess) return e;
-        ++*launches;
-    }
-    e = launch_rows(env, bf16 ? quant_trans_kernel<ROW_BF16> : quant_trans_kernel<ROW_F32>, p, dim3((p.cols + 63) / 64, (p.rows + 63) / 64), 256, 0);
-    if (e != cudaSuccess) return e;
-    ++*launches;
-    if (!p.given) {
-        const ColumnSteps s{p.scale, p.cols, p.top};
-        e = launch_rows(env, column_steps_kernel, s, dim3((p.cols + 255) / 256), 256, 0);
-        if (e != cudaSuccess) return e;
-        ++*launches;
-    }
-    return cudaSuccess;
+    if (p.x.type == ROW_BF16) return vec ? quant_trans_of<ROW_BF16, false>(env, p, launches) : quant_trans_of<ROW_BF16, true>(env, p, launches);
+    return vec ? quant_trans_of<ROW_F32, false>(env, p, launches) : quant_trans_of<ROW_F32, true>(env, p, launches);
 }
 
 // A product's operand whose rows do not start on 16 bytes, copied to rows that do. A thread makes 16 bytes of the copy from

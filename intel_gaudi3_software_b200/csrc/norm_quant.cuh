@@ -14,58 +14,197 @@
 namespace mmeb200 {
 
 // ------------------------------------------------------------------------------------------ elements
+// A lane works on pieces of eight consecutive elements, a warp on a run of consecutive pieces. Where every row of every tensor
+// starts on a multiple of eight elements (SHIFT = false) a piece is one or two 16-byte accesses. Rows of any other length,
+// pitch or start (SHIFT = true) are read as the aligned 16-byte words that contain the piece and shifted into place in
+// registers, and written as aligned words put together from the lane's piece and its left neighbour's: odd rows move as many
+// bytes per instruction as even ones do. How far a row is off is the same for all its pieces, so the shifts are branches that
+// a whole warp takes. Reads stay inside the tensor (first byte to last), writes inside the row; the ends of a warp's run go
+// element by element.
 template <int TYPE>
 struct RowElem;
-template <> struct RowElem<ROW_BF16> { using T = uint16_t; static constexpr int kBytes = 2; };
-template <> struct RowElem<ROW_F32> { using T = float; static constexpr int kBytes = 4; };
+template <> struct RowElem<ROW_BF16> { static constexpr int kBytes = 2; };
+template <> struct RowElem<ROW_F32> { static constexpr int kBytes = 4; };
+template <> struct RowElem<ROW_I8> { static constexpr int kBytes = 1; };   // codes of either kind
 
-// VEC elements as they lie in memory. Loading and decoding are separate so that all loads of a row are in flight before
-// the first value is needed.
-template <int TYPE, int VEC>
-struct RowPiece {
-    static constexpr int kWords = VEC == 8 ? RowElem<TYPE>::kBytes * 2 : 1;
-    uint32_t w[kWords];
-    __device__ __forceinline__ void load(const void* base, uint64_t at) {
-        if constexpr (VEC == 8) {
-            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const typename RowElem<TYPE>::T*>(base) + at);
+// out[i] = the four bytes from byte `off` + 4 i of `in`. off < 4 * (N - W) is the same in all lanes.
+template <int N, int W>
+__device__ __forceinline__ void shift_words(const uint32_t (&in)[N], uint32_t off, uint32_t (&out)[W]) {
+    const uint32_t bits = (off & 3) * 8;
 #pragma unroll
-            for (int i = 0; i < kWords / 4; ++i) {
-                const uint4 q = p[i];
-                w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-            }
-        } else if constexpr (TYPE == ROW_BF16) {
-            w[0] = static_cast<const uint16_t*>(base)[at];
-        } else {
-            w[0] = static_cast<const uint32_t*>(base)[at];
+    for (int q = 0; q < N - W; ++q)
+        if ((off >> 2) == uint32_t(q)) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) out[i] = __funnelshift_r(in[q + i], in[q + i + 1], bits);
+        }
+}
+
+__device__ __forceinline__ int piece_size(uint32_t c, uint32_t cols) { return c >= cols ? 0 : int(min(8u, cols - c)); }
+
+// A row that is read: `raw` pieces are loaded first, all of them in flight, and turned into packed elements when needed.
+template <int TYPE, bool SHIFT>
+struct RowIn {
+    static constexpr int kBytes = RowElem<TYPE>::kBytes, kWords = 2 * kBytes, kRaw = kWords + (SHIFT ? 4 : 0);
+    struct Raw { uint32_t w[kRaw]; };
+    const uint8_t* row;      // SHIFT: rounded down to 16 bytes
+    const uint8_t* lo;       // SHIFT: the tensor's bytes, [lo, hi)
+    const uint8_t* hi;
+    uint32_t off;
+    __device__ __forceinline__ RowIn(const RowTensor& t, uint64_t at) {
+        lo = static_cast<const uint8_t*>(t.ptr);
+        row = lo + at * kBytes;
+        if constexpr (SHIFT) {
+            hi = lo + t.bytes;
+            off = uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
+            row -= off;
         }
     }
-    __device__ __forceinline__ float value(int e) const {
-        if constexpr (TYPE == ROW_F32) return __uint_as_float(w[e]);
-        else return __uint_as_float(VEC == 8 ? ((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16)) : (w[0] << 16));
+    __device__ __forceinline__ void load(Raw& r, uint32_t c) const {
+        const uint8_t* a = row + uint64_t(c) * kBytes;
+        if (!SHIFT || (a >= lo && a + 4 * kRaw <= hi)) {
+#pragma unroll
+            for (int i = 0; i < kRaw / 4; ++i) {
+                const uint4 q = reinterpret_cast<const uint4*>(a)[i];
+                r.w[4 * i] = q.x; r.w[4 * i + 1] = q.y; r.w[4 * i + 2] = q.z; r.w[4 * i + 3] = q.w;
+            }
+        } else {   // the tensor's first and last pieces
+            load_guarded(r, a);
+        }
+    }
+    __device__ __forceinline__ void words(const Raw& r, uint32_t (&w)[kWords]) const {
+        if constexpr (SHIFT) shift_words(r.w, off, w);
+        else {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = r.w[i];
+        }
+    }
+
+private:
+    __device__ __noinline__ void load_guarded(Raw& r, const uint8_t* a) const {
+#pragma unroll 1
+        for (int i = 0; i < kRaw; ++i) {
+            uint32_t v = 0;
+#pragma unroll 1
+            for (int k = 0; k < 4; k += kBytes) {   // elements, which do not straddle the tensor's ends
+                const uint8_t* e = a + 4 * i + k;
+                if (e >= lo && e + kBytes <= hi) v |= (kBytes == 2 ? uint32_t(*reinterpret_cast<const uint16_t*>(e)) : *reinterpret_cast<const uint32_t*>(e)) << (8 * k);
+            }
+            r.w[i] = v;
+        }
     }
 };
-template <int VEC>
-struct RowPiece<ROW_NONE, VEC> {
-    __device__ __forceinline__ void load(const void*, uint64_t) {}
-    __device__ __forceinline__ float value(int) const { return 0.0f; }
+template <bool SHIFT>
+struct RowIn<ROW_NONE, SHIFT> {
+    struct Raw {};
+    __device__ __forceinline__ RowIn(const RowTensor&, uint64_t) {}
+    __device__ __forceinline__ void load(Raw&, uint32_t) const {}
+};
+template <int TYPE, int W>
+__device__ __forceinline__ void unpack(const uint32_t (&w)[W], float (&f)[8]) {
+    static_assert(W == 2 * RowElem<TYPE>::kBytes, "packed words");
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (TYPE == ROW_F32) f[e] = __uint_as_float(w[e]);
+        else f[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16));
+    }
+}
+
+// A row that is written. A warp writes its run step by step (32 pieces each), in order, all lanes together (SHIFT).
+// `start`: its first step; `last`: no step follows whose first piece is full.
+template <int TYPE, bool SHIFT>
+struct RowOut {
+    static constexpr int kBytes = RowElem<TYPE>::kBytes, kWords = 2 * kBytes;
+    static constexpr uint32_t kUnit = kWords == 2 ? 8 : 16;   // bytes of an aligned store
+    static constexpr int kTail = kUnit / 4;
+    uint8_t* row;
+    uint32_t off;
+    uint32_t carry[SHIFT ? kTail : 1];   // the end of this lane's piece before
+    __device__ __forceinline__ RowOut(const RowTensor& t, uint64_t at) {
+        row = static_cast<uint8_t*>(t.ptr) + at * kBytes;
+        if constexpr (SHIFT) {
+            off = uint32_t(reinterpret_cast<uintptr_t>(row)) & (kUnit - 1);
+#pragma unroll
+            for (int i = 0; i < kTail; ++i) carry[i] = 0;
+        }
+    }
+    __device__ __forceinline__ static void put(uint8_t* a, const uint32_t (&v)[kWords]) {
+        if constexpr (kWords == 2) *reinterpret_cast<uint2*>(a) = make_uint2(v[0], v[1]);
+        else {
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(a)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+    }
+    __device__ __forceinline__ static void put_elements(uint8_t* a, const uint32_t (&v)[kWords], int from, int to) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e >= from && e < to) {
+                if constexpr (kBytes == 4) reinterpret_cast<uint32_t*>(a)[e] = v[e];
+                else if constexpr (kBytes == 2) reinterpret_cast<uint16_t*>(a)[e] = uint16_t(v[e >> 1] >> (16 * (e & 1)));
+                else a[e] = uint8_t(v[e >> 2] >> (8 * (e & 3)));
+            }
+    }
+    // n: elements of this lane's piece that exist; whole: the warp's 32 pieces are full
+    __device__ __forceinline__ void store(uint32_t c, int n, const uint32_t (&v)[kWords], bool whole, bool start, bool last) {
+        uint8_t* a = row + uint64_t(c) * kBytes;
+        if constexpr (!SHIFT) {
+            if (n) put(a, v);
+        } else if (off == 0) {
+            if (n == 8) put(a, v);
+            else put_elements(a, v, 0, n);
+        } else {
+            const uint32_t lane = threadIdx.x & 31;
+            uint32_t both[kTail + kWords], out[kWords];
+#pragma unroll
+            for (int i = 0; i < kTail; ++i) {
+                // lane L takes lane L - 1's end, lane 0 what lane 31 had before
+                const uint32_t mine = v[kWords - kTail + i], give = lane == 31 ? carry[i] : mine;
+                both[i] = __shfl_sync(0xffffffffu, give, (lane + 31) & 31);
+                carry[i] = mine;
+            }
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) both[kTail + i] = v[i];
+            shift_words(both, kUnit - off, out);
+            const bool head = start && lane == 0;   // nobody gave it the bytes before its piece
+            if (n == 8 && !head) put(a - off, out);
+            if (start || last || !whole) {
+                // by elements: a head, and a piece that is not full; the last `off` bytes of a full piece without a successor,
+                // and those of a left neighbour of a piece that is not full
+                const int left = int(off) / kBytes;
+                const bool next_full = __shfl_down_sync(0xffffffffu, n, 1) == 8 && lane != 31;
+                const bool tail_mine = !(next_full || (lane == 31 && !last));
+                int from = 8, to = n;
+                if (head || n < 8) from = 0;
+                else if (tail_mine) from = 8 - left;
+                if (n == 8 && !tail_mine && from == 0) to = 8 - left;
+                if (from < to) put_elements(a, v, from, to);
+            }
+        }
+    }
 };
 
 // gamma is read by every row and sits in the caches; its type is a runtime value.
-template <int VEC>
-__device__ __forceinline__ void load_gamma(float (&g)[VEC], const void* base, int type, uint32_t at) {
-    if (type == ROW_BF16) {
-        RowPiece<ROW_BF16, VEC> p;
-        p.load(base, at);
+__device__ __forceinline__ void load_gamma(float (&g)[8], const void* base, int type, bool whole, uint32_t at, int n) {
+    if (type == ROW_NONE) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = p.value(e);
-    } else if (type == ROW_F32) {
-        RowPiece<ROW_F32, VEC> p;
-        p.load(base, at);
+        for (int e = 0; e < 8; ++e) g[e] = 1.0f;
+    } else if (whole && n == 8) {
+        if (type == ROW_BF16) {
+            const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = p.value(e);
+            for (int e = 0; e < 8; ++e) g[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16));
+        } else {
+            const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
+            const float4 a = __ldg(q), b = __ldg(q + 1);
+            g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+            g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+        }
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) g[e] = 1.0f;
+        for (int e = 0; e < 8; ++e) {
+            g[e] = 1.0f;
+            if (e < n) g[e] = type == ROW_BF16 ? __uint_as_float(uint32_t(static_cast<const uint16_t*>(base)[at + e]) << 16) : static_cast<const float*>(base)[at + e];
+        }
     }
 }
 
@@ -74,23 +213,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
     return w;
 }
-template <int VEC>
-__device__ __forceinline__ void store_bf16(void* base, uint64_t at, const float (&f)[VEC]) {
-    uint16_t* p = static_cast<uint16_t*>(base) + at;
-    if constexpr (VEC == 8) *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-    else *p = uint16_t(pack_bf16(f[0], 0.0f));
+__device__ __forceinline__ void pack_bf16x8(const float (&f)[8], uint32_t (&w)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
 }
-template <int VEC>
-__device__ __forceinline__ void store_f32(void* base, uint64_t at, const float (&f)[VEC]) {
-    float* p = static_cast<float*>(base) + at;
-    if constexpr (VEC == 8) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
-        *p = f[0];
-    }
-}
-
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -109,285 +235,360 @@ __device__ __forceinline__ uint64_t row_offset(const RowTensor& t, uint32_t row,
 }
 
 // ------------------------------------------------------------------------------------------ 8-bit codes
-// How a row's values become codes. `ok` is false for rows whose step is zero or no number: their codes are zero.
-struct RowStep {
+// How values become codes: `step`, and its reciprocal where that decides them. recip = 0: no codes (a step that is zero,
+// negative or no finite number), NaN: the reciprocal is no normal number, every code is divided for.
+struct CodeStep {
     float step, recip;
-    bool ok, fast;
 };
-__device__ __forceinline__ RowStep make_row_step(float step) {
-    RowStep s;
+__device__ __forceinline__ CodeStep make_code_step(float step) {
+    CodeStep s;
     s.step = step;
-    s.recip = __frcp_rn(step);
-    s.ok = step > 0.0f && step < __uint_as_float(0x7F800000u);
-    s.fast = step >= 0x1p-126f && step <= 0x1p126f;   // the reciprocal is a normal number
+    if (!(step > 0.0f && step < __uint_as_float(0x7F800000u))) s.recip = 0.0f;
+    else s.recip = (step >= 0x1p-126f && step <= 0x1p126f) ? __frcp_rn(step) : __uint_as_float(0x7FC00000u);
     return s;
 }
 constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to the nearest whole number, ties to even
 
-// The int8 code of v / step in the low byte. v * recip is within 2^-23 of the quotient, relatively, i.e. within 2^-16 for
-// |quotient| <= 127: unless it lies closer than 2^-15 to the middle between two whole numbers, it rounds as the correctly
-// rounded quotient does. The few that do lie there are divided.
-__device__ __forceinline__ uint32_t int8_code(float v, const RowStep& s) {
-    float t = v * s.recip;
-    t = fminf(fmaxf(t, -127.0f), 127.0f);
-    float m = t + kRoundMagic;
-    const float f = fabsf(t - (m - kRoundMagic));
-    if (f > 0.5f - 0x1p-15f || !s.fast) {
-        t = fminf(fmaxf(__fdiv_rn(v, s.step), -127.0f), 127.0f);
-        m = t + kRoundMagic;
-    }
-    return __float_as_uint(m);
+__device__ __forceinline__ uint32_t pack_low_bytes(float a, float b, float c, float d) {
+    return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
 }
-
-// VEC codes of the values v: stored at element `at` of a row of codes.
-template <int VEC>
-__device__ __forceinline__ void store_codes(void* base, uint64_t at, const float (&v)[VEC], int type, const RowStep& s, const Fp8HwCast& hw) {
-    uint8_t* p = static_cast<uint8_t*>(base) + at;
-    uint32_t w[VEC == 8 ? 2 : 1];
-    if (!s.ok) {
+// Four codes by the definition: the correctly rounded quotient, then the code. Out of line: few values come here.
+template <bool I8>
+static __device__ __noinline__ uint32_t codes_by_division(float v0, float v1, float v2, float v3, float step, const Fp8HwCast& hw) {
+    float t[4] = {__fdiv_rn(v0, step), __fdiv_rn(v1, step), __fdiv_rn(v2, step), __fdiv_rn(v3, step)};
+    if constexpr (I8) {
 #pragma unroll
-        for (int i = 0; i < (VEC == 8 ? 2 : 1); ++i) w[i] = 0;
-    } else if (type == ROW_I8) {
-        uint32_t q[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) q[e] = int8_code(v[e] == v[e] ? v[e] : 0.0f, s);   // a NaN (given scales only) has no code
-        if constexpr (VEC == 8) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t lo = __byte_perm(q[4 * i], q[4 * i + 1], 0x0040), hi = __byte_perm(q[4 * i + 2], q[4 * i + 3], 0x0040);
-                w[i] = __byte_perm(lo, hi, 0x5410);
-            }
-        } else {
-            w[0] = q[0];
-        }
+        for (int e = 0; e < 4; ++e) t[e] = fminf(fmaxf(t[e], -127.0f), 127.0f) + kRoundMagic;
+        return pack_low_bytes(t[0], t[1], t[2], t[3]);
     } else {
-#pragma unroll
-        for (int i = 0; i < (VEC == 8 ? 2 : 1); ++i) {
-            float t[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) t[e] = (VEC == 8 || e == 0) ? __fdiv_rn(v[VEC == 8 ? 4 * i + e : 0], s.step) : 0.0f;
-            w[i] = f32x4_to_fp8_hw(t, hw);
-        }
+        return f32x4_to_fp8_hw(t, hw);
     }
-    if constexpr (VEC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *p = uint8_t(w[0]);
+}
+// The four codes of v / step, packed. v * recip is within 2^-23 of the quotient, relatively, and the 32-bit quotient within
+// 2^-24 of the exact one, so
+//   int8: for |quotient| <= 127 the product is off by at most 2^-15.4; unless it lies closer than 2^-15 to the middle between two
+//         whole numbers it rounds as the quotient does (one multiplication and three additions per element);
+//   fp8:  where product * (1 - 2^-22) and product * (1 + 2^-22) have the same code, it is the quotient's (the cast is monotone).
+// The few quads with an element that fails its test are divided. GIVEN: the step is the caller's, quotients may be anything.
+template <bool I8, bool GIVEN>
+__device__ __forceinline__ uint32_t make_codes(float v0, float v1, float v2, float v3, const CodeStep& s, const Fp8HwCast& hw) {
+    if (s.recip == 0.0f) return 0u;
+    float x[4] = {v0, v1, v2, v3};
+    uint32_t w;
+    bool sure;
+    if constexpr (I8) {
+        float m[4], worst = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (GIVEN) x[e] = x[e] == x[e] ? x[e] : 0.0f;   // a NaN has no code (rows with one have no step of their own)
+            float t = x[e] * s.recip;
+            if constexpr (GIVEN) t = fminf(fmaxf(t, -127.0f), 127.0f);
+            m[e] = t + kRoundMagic;
+            worst = fmaxf(worst, fabsf(t - (m[e] - kRoundMagic)));
+        }
+        sure = worst <= 0.5f - 0x1p-15f && s.recip == s.recip;
+        w = pack_low_bytes(m[0], m[1], m[2], m[3]);
+    } else {
+        float lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float t = x[e] * s.recip;
+            lo[e] = t * (1.0f - 0x1p-22f);
+            hi[e] = t * (1.0f + 0x1p-22f);
+        }
+        w = f32x4_to_fp8_hw(lo, hw);
+        sure = w == f32x4_to_fp8_hw(hi, hw) && s.recip == s.recip;
+    }
+    if (!sure) w = codes_by_division<I8>(x[0], x[1], x[2], x[3], s.step, hw);
+    return w;
 }
 
 // ------------------------------------------------------------------------------------------ reductions
-// Sum of `a` and NaN-keeping maximum of `b` over the T threads of a row (a warp, or the whole block). The order is fixed.
-struct RowSums { float sum, top; };
-template <int T>
-__device__ __forceinline__ RowSums reduce_row(float a, float b, float2* scratch) {
+// Sums over the threads of a row: a warp, or the `warps` warps of the block (BLOCK). The order is fixed. MAX: the second is a
+// maximum that keeps NaN.
+template <bool BLOCK, bool MAX>
+__device__ __forceinline__ float2 reduce_row(float a, float b, uint32_t warps, float2* scratch) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, o);
-        b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+        const float t = __shfl_xor_sync(0xffffffffu, b, o);
+        b = MAX ? max_nan(b, t) : b + t;
     }
-    if constexpr (T > 32) {
-        constexpr int W = T / 32;
+    if constexpr (BLOCK) {
         if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
         __syncthreads();
-        const float2 v = (threadIdx.x & 31) < W ? scratch[threadIdx.x & 31] : make_float2(0.0f, 0.0f);
-        a = v.x;
-        b = v.y;
-#pragma unroll
-        for (int o = W / 2; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+        a = scratch[0].x;
+        b = scratch[0].y;
+#pragma unroll 4
+        for (uint32_t w = 1; w < warps; ++w) {
+            const float2 t = scratch[w];
+            a += t.x;
+            b = MAX ? max_nan(b, t.y) : b + t.y;
         }
-        a = __shfl_sync(0xffffffffu, a, 0);
-        b = __shfl_sync(0xffffffffu, b, 0);
-    }
-    return {a, b};
-}
-template <int T>
-__device__ __forceinline__ float2 reduce_row2(float a, float b, float2* scratch) {   // two sums
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, o);
-        b += __shfl_xor_sync(0xffffffffu, b, o);
-    }
-    if constexpr (T > 32) {
-        constexpr int W = T / 32;
-        if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
-        __syncthreads();
-        const float2 v = (threadIdx.x & 31) < W ? scratch[threadIdx.x & 31] : make_float2(0.0f, 0.0f);
-        a = v.x;
-        b = v.y;
-#pragma unroll
-        for (int o = W / 2; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-        }
-        a = __shfl_sync(0xffffffffu, a, 0);
-        b = __shfl_sync(0xffffffffu, b, 0);
     }
     return make_float2(a, b);
 }
-__device__ __forceinline__ float inverse_rms(float sum_of_squares, uint32_t cols, float eps) {
-    return __frcp_rn(__fsqrt_rn(__fdiv_rn(sum_of_squares, float(cols)) + eps));
+__device__ __forceinline__ float inverse_rms(float sum_of_squares, float per_col, float eps) {
+    return __frsqrt_rn(fmaf(sum_of_squares, per_col, eps));   // per_col: 1 / cols
 }
 
 // What a row's sums decide: the factor of float outputs, the step of codes, the scale that is written.
-struct RowFactors { float inv; RowStep step; float scale; };
-__device__ __forceinline__ RowFactors row_factors(const NormParams& p, const RowSums& s, uint32_t row) {
+struct RowFactors { float inv; CodeStep step; float scale; };
+__device__ __forceinline__ RowFactors row_factors(const NormParams& p, float sum, float top, uint32_t row) {
     RowFactors f;
-    f.inv = p.norm ? inverse_rms(s.sum, p.cols, p.eps) : 1.0f;
+    f.inv = p.norm ? inverse_rms(sum, p.per_col, p.eps) : 1.0f;
     f.scale = 0.0f;
-    if (p.given) {
-        f.step = make_row_step(p.given[uint64_t(row) * p.given_stride]);
-    } else {
-        f.step = make_row_step(__fdiv_rn(s.top, p.top));
+    if (p.mode == NORM_I8_GIVEN || p.mode == NORM_F8_GIVEN) {
+        f.step = make_code_step(p.given[uint64_t(row) * p.given_stride]);
+    } else if (p.mode == NORM_I8 || p.mode == NORM_F8) {
+        f.step = make_code_step(__fdiv_rn(top, p.top));
         const bool finite = f.step.step < __uint_as_float(0x7F800000u);   // false for NaN
-        f.scale = !finite ? __uint_as_float(0x7FC00000u) : f.step.ok ? f.step.step * f.inv : 0.0f;
+        f.scale = !finite ? __uint_as_float(0x7FC00000u) : f.step.step > 0.0f ? f.step.step * f.inv : 0.0f;
     }
     return f;
 }
-template <int VEC>
-__device__ __forceinline__ void store_row_piece(const NormParams& p, uint64_t at, float (&v)[VEC], const RowFactors& f) {
-    if (p.out.type >= ROW_I8) {
-        if (p.given) {
+// The type a row is kept in while its sums are taken: the stream's, or x's where nothing is added. bf16 rows take four
+// registers per piece, and their values are exact.
+template <int XT, int RT>
+struct RowKept {
+    static constexpr int kType = RT != ROW_NONE ? RT : XT, kWords = 2 * RowElem<kType>::kBytes;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void values(float (&h)[8]) const { unpack<kType>(w, h); }
+};
+// x + residual, rounded to the stream's type, which is what the norm sees.
+template <int XT, int RT, bool SHIFT>
+__device__ __forceinline__ void stream_piece(const RowIn<XT, SHIFT>& xin, const typename RowIn<XT, SHIFT>::Raw& x, const RowIn<RT, SHIFT>& rin,
+                                             const typename RowIn<RT, SHIFT>::Raw& r, RowKept<XT, RT>& h) {
+    uint32_t xw[RowIn<XT, SHIFT>::kWords];
+    xin.words(x, xw);
+    if constexpr (RT == ROW_NONE) {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] *= f.inv;
-        }
-        store_codes<VEC>(p.out.ptr, at, v, p.out.type, f.step, p.hw);
+        for (int i = 0; i < RowIn<XT, SHIFT>::kWords; ++i) h.w[i] = xw[i];
     } else {
+        uint32_t rw[RowIn<RT, SHIFT>::kWords];
+        rin.words(r, rw);
+        float f[8], g[8];
+        unpack<XT>(xw, f);
+        unpack<RT>(rw, g);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] *= f.inv;
-        if (p.out.type == ROW_BF16) store_bf16<VEC>(p.out.ptr, at, v);
-        else store_f32<VEC>(p.out.ptr, at, v);
+        for (int e = 0; e < 8; ++e) f[e] += g[e];
+        if constexpr (RT == ROW_BF16) pack_bf16x8(f, h.w);
+        else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h.w[e] = __float_as_uint(f[e]);
+        }
     }
 }
-// h of one piece: the residual's addition, rounded to the stream's type, which is what the norm sees.
-template <int XT, int RT, int VEC>
-__device__ __forceinline__ void stream_values(const RowPiece<XT, VEC>& x, const RowPiece<RT, VEC>& r, float (&h)[VEC]) {
+// A row's last piece may be partial: its missing elements count as zeros.
+template <int XT, int RT>
+__device__ __forceinline__ void clear_missing(RowKept<XT, RT>& h, int n) {
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-        h[e] = x.value(e);
-        if constexpr (RT != ROW_NONE) h[e] += r.value(e);
-        if constexpr (RT == ROW_BF16) h[e] = __uint_as_float(pack_bf16(h[e], 0.0f) << 16);
+    for (int e = 0; e < 8; ++e)
+        if (e >= n) {
+            if constexpr (RowKept<XT, RT>::kType == ROW_F32) h.w[e] = 0;
+            else h.w[e >> 1] &= (e & 1) ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+}
+// Adds a piece to its row's sums.
+template <bool TOPS, int XT, int RT>
+__device__ __forceinline__ void sum_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float& sum, float& top) {
+    float h[8];
+    kept.values(h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum = fmaf(h[e], h[e], sum);
+    if constexpr (TOPS) {
+        if (p.gamma_type != ROW_NONE) {
+            float g[8];
+            load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] *= g[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(h[e]));
+    }
+}
+// v = h * gamma of a piece.
+template <int XT, int RT>
+__device__ __forceinline__ void scaled_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float (&v)[8]) {
+    kept.values(v);
+    if (p.gamma_type != ROW_NONE && n) {
+        float g[8];
+        load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= g[e];
     }
 }
 
-// One row per T threads (a warp: several rows per block; else the block), NV pieces of VEC elements per thread, all in
-// registers between the row's one read and its one write.
-template <int XT, int RT, int VEC, int NV, int T>
-__global__ void __launch_bounds__(T < 128 ? 128 : T) norm_kernel(const __grid_constant__ NormParams p) {
+// The warp's run of pieces: piece i of a lane starts at column c0 + 256 i.
+struct WarpRun {
+    uint32_t c0, cols;
+    __device__ __forceinline__ uint32_t col(uint32_t i) const { return c0 + 256 * i + (threadIdx.x & 31) * 8; }
+    __device__ __forceinline__ bool any(uint32_t i) const { return c0 + 256 * i < cols; }
+    __device__ __forceinline__ bool whole(uint32_t i) const { return c0 + 256 * i + 256 <= cols; }
+    __device__ __forceinline__ int size(uint32_t i) const { return piece_size(col(i), cols); }
+    // step i is the last of `steps` that hands nothing on to a full piece
+    __device__ __forceinline__ bool last(uint32_t i, uint32_t steps) const { return i + 1 == steps || c0 + 256 * (i + 1) + 8 > cols; }
+};
+
+// The second pass over a row: `piece(i, n, v)` gives the values h * gamma of piece i.
+template <int MODE, bool SHIFT, int UNROLL, typename F>
+__device__ __forceinline__ void write_row(const NormParams& p, uint64_t at, const WarpRun& run, uint32_t pieces, const RowFactors& f, F&& piece) {
+    constexpr int kType = MODE == NORM_BF16 ? ROW_BF16 : MODE == NORM_F32 ? ROW_F32 : ROW_I8;
+    RowOut<kType, SHIFT> out(p.out, at);
+#pragma unroll UNROLL
+    for (uint32_t i = 0; i < pieces; ++i) {
+        const int n = run.size(i);
+        if (SHIFT ? run.any(i) : n != 0) {
+            float v[8];
+            uint32_t w[RowOut<kType, SHIFT>::kWords];
+            piece(i, n, v);
+            if constexpr (MODE == NORM_I8 || MODE == NORM_F8) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8, false>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], f.step, p.hw);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] *= f.inv;
+                if constexpr (MODE == NORM_BF16) pack_bf16x8(v, w);
+                else if constexpr (MODE == NORM_F32) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[e]);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8_GIVEN, true>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], f.step, p.hw);
+                }
+            }
+            out.store(run.col(i), n, w, run.whole(i), i == 0, run.last(i, pieces));
+        }
+    }
+}
+// What differs between the kinds of output is decided once per row, not once per piece.
+template <bool SHIFT, int UNROLL, typename F>
+__device__ __forceinline__ void write_row_any(const NormParams& p, uint64_t at, const WarpRun& run, uint32_t pieces, const RowFactors& f, F&& piece) {
+    switch (p.mode) {
+        case NORM_BF16: write_row<NORM_BF16, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+        case NORM_F32: write_row<NORM_F32, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+        case NORM_I8: write_row<NORM_I8, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+        case NORM_F8: write_row<NORM_F8, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+        case NORM_I8_GIVEN: write_row<NORM_I8_GIVEN, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+        default: write_row<NORM_F8_GIVEN, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
+    }
+}
+
+// The first pass: reads x and the residual, writes the stream, takes the sums. NV pieces per lane, loads G pieces at a time.
+template <bool TOPS, int XT, int RT, bool SHIFT, int NV>
+__device__ __forceinline__ float2 read_row(const NormParams& p, uint32_t row, const WarpRun& run, RowKept<XT, RT> (&kept)[NV]) {
+    constexpr int G = NV < 2 ? 1 : 2, KT = RowKept<XT, RT>::kType;
+    const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat));
+    const RowIn<RT, SHIFT> rin(p.residual, RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0);
+    RowOut<KT, SHIFT> sout(p.sum, RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0);
+    float sum = 0.0f, top = 0.0f;
+#pragma unroll
+    for (int i0 = 0; i0 < NV; i0 += G) {
+        typename RowIn<XT, SHIFT>::Raw x[G];
+        typename RowIn<RT, SHIFT>::Raw r[G];
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+            if (run.size(i0 + j)) {
+                xin.load(x[j], run.col(i0 + j));
+                rin.load(r[j], run.col(i0 + j));
+            }
+#pragma unroll
+        for (int j = 0; j < G; ++j) {
+            const int i = i0 + j;
+            const int n = run.size(i);
+            if (n) {
+                stream_piece<XT, RT, SHIFT>(xin, x[j], rin, r[j], kept[i]);
+                if (SHIFT && n < 8) clear_missing(kept[i], n);
+                sum_piece<TOPS>(p, kept[i], run.col(i), n, sum, top);
+            }
+            if constexpr (RT != ROW_NONE) {
+                if (p.sum.ptr && (SHIFT ? run.any(i) : n != 0)) sout.store(run.col(i), n, kept[i].w, run.whole(i), i == 0, run.last(i, NV));
+            }
+        }
+    }
+    return make_float2(sum, top);
+}
+
+// A row per warp (BLOCK = false: four rows per block) or per block, NV pieces per lane, kept in registers between the row's
+// one read and its one write.
+template <int XT, int RT, bool SHIFT, int NV, bool BLOCK, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 scratch[32];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t tid = T == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const uint32_t row = T == 32 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= p.rows) return;   // whole warps (T == 32), never part of a block that synchronises
-    const uint64_t xo = row_offset(p.x, row, p.dims, p.flat), ro = RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0;
-    RowPiece<XT, VEC> xs[NV];
-    RowPiece<RT, VEC> rs[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = (i * T + tid) * VEC;
-        if (c < p.cols) {
-            xs[i].load(p.x.ptr, xo + c);
-            rs[i].load(p.residual.ptr, ro + c);
-        }
-    }
-    const bool eight = p.out.type >= ROW_I8;
-    const uint64_t so = RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0;
-    float v[NV][VEC];
-    float sum = 0.0f, top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = (i * T + tid) * VEC;
-        if (c < p.cols) {
-            float g[VEC];
-            load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
-            stream_values<XT, RT, VEC>(xs[i], rs[i], v[i]);
-            if constexpr (RT != ROW_NONE) {
-                if (p.sum.ptr) {
-                    if constexpr (RT == ROW_BF16) store_bf16<VEC>(p.sum.ptr, so + c, v[i]);
-                    else store_f32<VEC>(p.sum.ptr, so + c, v[i]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                sum = fmaf(v[i][e], v[i][e], sum);
-                v[i][e] *= g[e];
-                if (eight) top = max_nan(top, fabsf(v[i][e]));
-            }
-        }
-    }
-    const RowSums s = reduce_row<T>(sum, top, scratch);
-    const RowFactors f = row_factors(p, s, row);
-    if (p.scale && tid == 0) p.scale[row] = f.scale;
-    const uint64_t oo = row_offset(p.out, row, p.dims, p.flat);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t c = (i * T + tid) * VEC;
-        if (c < p.cols) store_row_piece<VEC>(p, oo + c, v[i], f);
-    }
+    const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (row >= p.rows) return;   // whole warps, never part of a block that synchronises
+    const WarpRun run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
+    RowKept<XT, RT> kept[NV];
+    float2 s = (p.mode == NORM_I8 || p.mode == NORM_F8) ? read_row<true, XT, RT, SHIFT, NV>(p, row, run, kept) : read_row<false, XT, RT, SHIFT, NV>(p, row, run, kept);
+    s = reduce_row<BLOCK, true>(s.x, s.y, blockDim.x >> 5, scratch);
+    const RowFactors f = row_factors(p, s.x, s.y, row);
+    if (p.scale && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) p.scale[row] = f.scale;
+    write_row_any<SHIFT, NV>(p, row_offset(p.out, row, p.dims, p.flat), run, NV, f,
+                         [&](uint32_t i, int n, float (&v)[8]) { scaled_piece(p, kept[i], run.col(i), n, v); });
 }
 
 // Rows too long for registers: the row is read a second time (from L2, mostly) once its sums are known. The second read
-// takes the stream from `sum` where it was written (in place, x and the residual may be gone by then). A thread reads and
+// takes the stream from `sum` where it was written (in place, x and the residual may be gone by then). A warp reads and
 // writes the same elements in both passes.
-template <int XT, int RT, int VEC>
+template <int XT, int RT, bool SHIFT>
 __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__ NormParams p) {
+    constexpr int KT = RowKept<XT, RT>::kType;
     __shared__ float2 scratch[32];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t row = blockIdx.x;
-    const uint64_t xo = row_offset(p.x, row, p.dims, p.flat), ro = RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0;
-    const uint64_t so = RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0, oo = row_offset(p.out, row, p.dims, p.flat);
-    const bool eight = p.out.type >= ROW_I8;
+    const uint32_t row = blockIdx.x, pieces = (p.cols + 32 * 256 - 1) / (32 * 256);   // per lane
+    const WarpRun run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
+    const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat));
+    const RowIn<RT, SHIFT> rin(p.residual, RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0);
+    const uint64_t so = RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0;
+    const bool tops = p.mode == NORM_I8 || p.mode == NORM_F8, has_sum = RT != ROW_NONE && p.sum.ptr != nullptr;
     float sum = 0.0f, top = 0.0f;
+    {
+        RowOut<KT, SHIFT> sout(p.sum, so);
 #pragma unroll 1
-    for (uint32_t c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-        RowPiece<XT, VEC> x;
-        RowPiece<RT, VEC> r;
-        float g[VEC], h[VEC];
-        x.load(p.x.ptr, xo + c);
-        r.load(p.residual.ptr, ro + c);
-        load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
-        stream_values<XT, RT, VEC>(x, r, h);
-        if constexpr (RT != ROW_NONE) {
-            if (p.sum.ptr) {
-                if constexpr (RT == ROW_BF16) store_bf16<VEC>(p.sum.ptr, so + c, h);
-                else store_f32<VEC>(p.sum.ptr, so + c, h);
+        for (uint32_t i = 0; i < pieces && run.any(i); ++i) {
+            const int n = run.size(i);
+            RowKept<XT, RT> kept;
+            if (n) {
+                typename RowIn<XT, SHIFT>::Raw x;
+                typename RowIn<RT, SHIFT>::Raw r;
+                xin.load(x, run.col(i));
+                rin.load(r, run.col(i));
+                stream_piece<XT, RT, SHIFT>(xin, x, rin, r, kept);
+                if (SHIFT && n < 8) clear_missing(kept, n);
+                if (tops) sum_piece<true>(p, kept, run.col(i), n, sum, top);
+                else sum_piece<false>(p, kept, run.col(i), n, sum, top);
+            }
+            if constexpr (RT != ROW_NONE) {
+                if (has_sum && (SHIFT || n)) sout.store(run.col(i), n, kept.w, run.whole(i), i == 0, run.last(i, pieces));
             }
         }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-            sum = fmaf(h[e], h[e], sum);
-            if (eight) top = max_nan(top, fabsf(h[e] * g[e]));
-        }
     }
-    const RowSums s = reduce_row<1024>(sum, top, scratch);
-    const RowFactors f = row_factors(p, s, row);
+    const float2 s = reduce_row<true, true>(sum, top, 32, scratch);   // its barrier also orders the stores of `sum` and the reads below
+    const RowFactors f = row_factors(p, s.x, s.y, row);
     if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
-#pragma unroll 1
-    for (uint32_t c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-        float g[VEC], h[VEC];
-        load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
-        bool kept = false;
-        if constexpr (RT != ROW_NONE) {
-            if (p.sum.ptr) {
-                RowPiece<RT, VEC> r;
-                r.load(p.sum.ptr, so + c);
+    const RowIn<KT, SHIFT> again(p.sum, so);
+    const uint64_t oo = row_offset(p.out, row, p.dims, p.flat);
+    write_row_any<SHIFT, 1>(p, oo, run, pieces, f, [&](uint32_t i, int n, float (&v)[8]) {
+        RowKept<XT, RT> kept;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) h[e] = r.value(e);
-                kept = true;
+        for (int k = 0; k < RowKept<XT, RT>::kWords; ++k) kept.w[k] = 0;
+        if (n) {
+            if (has_sum) {
+                typename RowIn<KT, SHIFT>::Raw h;
+                again.load(h, run.col(i));
+                again.words(h, kept.w);
+            } else {
+                typename RowIn<XT, SHIFT>::Raw x;
+                typename RowIn<RT, SHIFT>::Raw r;
+                xin.load(x, run.col(i));
+                rin.load(r, run.col(i));
+                stream_piece<XT, RT, SHIFT>(xin, x, rin, r, kept);
             }
         }
-        if (!kept) {
-            RowPiece<XT, VEC> x;
-            RowPiece<RT, VEC> r;
-            x.load(p.x.ptr, xo + c);
-            r.load(p.residual.ptr, ro + c);
-            stream_values<XT, RT, VEC>(x, r, h);
-        }
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) h[e] *= g[e];
-        store_row_piece<VEC>(p, oo + c, h, f);
-    }
+        scaled_piece(p, kept, run.col(i), n, v);
+    });
 }
 
 // ------------------------------------------------------------------------------------------ gradient
@@ -395,85 +596,109 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
 // mean(a * u) = inv * mean(a * x), so both sums of a row (x^2 and a * x) are taken in one pass. A block walks rows b, b +
 // blocks, ...; every thread keeps the sums of its own columns of dgamma, and the block's partial sums (one row of `partial`)
 // are added in a fixed order by column_sums: results do not depend on timing.
-template <int XT, int DT_, int VEC, int NV, int T>
-__global__ void __launch_bounds__(T < 128 ? 128 : T) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
-    constexpr int kRowsPerBlock = T == 32 ? 4 : 1;
+// XT: type of x, dy, dsum and dx; DSUM: whether there is a gradient of the sum. A row per warp or per block, as in norm_kernel.
+template <int XT, bool DSUM, bool SHIFT, int NV, bool BLOCK, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr int kRowsPerBlock = BLOCK ? 1 : 4, ST = DSUM ? XT : ROW_NONE, W = 2 * RowElem<XT>::kBytes;
     __shared__ float2 scratch[2][32];
-    extern __shared__ float block_sums[];   // T == 32: [cols], the four warps' sums of dgamma
+    extern __shared__ float block_sums[];   // a row per warp: [cols], the four warps' sums of dgamma
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t tid = T == 32 ? (threadIdx.x & 31) : threadIdx.x;
-    const uint32_t sub = T == 32 ? (threadIdx.x >> 5) : 0;
-    float acc[NV][VEC];
+    const uint32_t sub = BLOCK ? 0 : (threadIdx.x >> 5);
+    const WarpRun run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
+    float acc[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) acc[i][e] = 0.0f;
+        for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x * kRowsPerBlock + sub; row < p.rows; row += gridDim.x * kRowsPerBlock, turn ^= 1) {
-        const uint64_t xo = row_offset(p.x, row, p.dims, p.flat), yo = row_offset(p.dy, row, p.dims, p.flat);
-        const uint64_t so = DT_ != ROW_NONE ? row_offset(p.dsum, row, p.dims, p.flat) : 0;
-        RowPiece<XT, VEC> xs[NV], ys[NV];
-        RowPiece<DT_, VEC> ds[NV];
+        const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat)), yin(p.dy, row_offset(p.dy, row, p.dims, p.flat));
+        const RowIn<ST, SHIFT> sin(p.dsum, DSUM ? row_offset(p.dsum, row, p.dims, p.flat) : 0);
+        uint32_t xs[NV][W], ys[NV][W];
+        typename RowIn<ST, SHIFT>::Raw ds[NV];
+        {
+            typename RowIn<XT, SHIFT>::Raw xr[NV], yr[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = (i * T + tid) * VEC;
-            if (c < p.cols) {
-                xs[i].load(p.x.ptr, xo + c);
-                ys[i].load(p.dy.ptr, yo + c);
-                ds[i].load(p.dsum.ptr, so + c);
-            }
+            for (int i = 0; i < NV; ++i)
+                if (run.size(i)) {
+                    xin.load(xr[i], run.col(i));
+                    yin.load(yr[i], run.col(i));
+                    sin.load(ds[i], run.col(i));
+                }
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (run.any(i)) {
+                    xin.words(xr[i], xs[i]);
+                    yin.words(yr[i], ys[i]);
+                }
         }
         float squares = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t c = (i * T + tid) * VEC;
-            if (c < p.cols) {
-                float g[VEC];
-                load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
+            const int n = run.size(i);
+            if (n) {
+                float g[8], x[8], y[8];
+                load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+                unpack<XT>(xs[i], x);
+                unpack<XT>(ys[i], y);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float x = xs[i].value(e);
-                    squares = fmaf(x, x, squares);
-                    dot = fmaf(ys[i].value(e) * g[e], x, dot);
+                for (int e = 0; e < 8; ++e) {
+                    if (SHIFT && e >= n) x[e] = y[e] = 0.0f;
+                    squares = fmaf(x[e], x[e], squares);
+                    dot = fmaf(y[e] * g[e], x[e], dot);
                 }
             }
         }
-        const float2 s = reduce_row2<T>(squares, dot, scratch[turn]);   // two buffers: the next row's sums may start before all have read
-        const float inv = inverse_rms(s.x, p.cols, p.eps);
-        const float mean_au = __fdiv_rn(s.y, float(p.cols)) * inv;
-        const uint64_t oo = row_offset(p.dx, row, p.dims, p.flat);
+        const float2 s = reduce_row<BLOCK, false>(squares, dot, blockDim.x >> 5, scratch[turn]);   // two buffers: the next row's sums may start before all have read
+        const float inv = inverse_rms(s.x, p.per_col, p.eps);
+        const float mean_au = s.y * p.per_col * inv;
+        auto write = [&](auto& out) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t c = (i * T + tid) * VEC;
-            if (c < p.cols) {
-                float g[VEC], d[VEC];
-                load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
+            for (int i = 0; i < NV; ++i) {
+                const int n = run.size(i);
+                if (SHIFT ? run.any(i) : n != 0) {
+                    float d[8], x[8], y[8], g[8];
+                    unpack<XT>(xs[i], x);
+                    unpack<XT>(ys[i], y);
+                    load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+                    float sv[8];
+                    if constexpr (DSUM) {
+                        uint32_t sw[W];
+                        sin.words(ds[i], sw);
+                        unpack<XT>(sw, sv);
+                    }
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float u = xs[i].value(e) * inv, y = ys[i].value(e);
-                    d[e] = (y * g[e] - u * mean_au) * inv;
-                    if constexpr (DT_ != ROW_NONE) d[e] += ds[i].value(e);
-                    acc[i][e] = fmaf(y, u, acc[i][e]);
+                    for (int e = 0; e < 8; ++e) {
+                        const float u = x[e] * inv, t = fmaf(-u, mean_au, y[e] * g[e]);
+                        d[e] = DSUM ? fmaf(t, inv, sv[e]) : t * inv;
+                        acc[i][e] = fmaf(y[e], u, acc[i][e]);   // of missing elements: never read
+                    }
+                    uint32_t w[W];
+                    if constexpr (XT == ROW_BF16) pack_bf16x8(d, w);
+                    else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(d[e]);
+                    }
+                    out.store(run.col(i), n, w, run.whole(i), i == 0, run.last(i, NV));
                 }
-                if (p.dx.type == ROW_BF16) store_bf16<VEC>(p.dx.ptr, oo + c, d);
-                else store_f32<VEC>(p.dx.ptr, oo + c, d);
             }
-        }
+        };
+        RowOut<XT, SHIFT> out(p.dx, row_offset(p.dx, row, p.dims, p.flat));
+        write(out);
     }
     if (!p.partial) return;
     float* mine = p.partial + uint64_t(blockIdx.x) * p.cols;
-    if constexpr (T == 32) {
+    if constexpr (!BLOCK) {
         for (uint32_t w = 0; w < 4; ++w) {   // the warps add their sums in turn: the order is fixed
             if (sub == w) {
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const uint32_t c = (i * T + tid) * VEC;
-                    if (c < p.cols) {
+                for (int i = 0; i < NV; ++i)
 #pragma unroll
-                        for (int e = 0; e < VEC; ++e) block_sums[c + e] = w ? block_sums[c + e] + acc[i][e] : acc[i][e];
+                    for (int e = 0; e < 8; ++e) {
+                        const uint32_t c = run.col(i) + e;
+                        if (c < p.cols) block_sums[c] = w ? block_sums[c] + acc[i][e] : acc[i][e];
                     }
-                }
             }
             __syncthreads();
         }
@@ -481,63 +706,96 @@ __global__ void __launch_bounds__(T < 128 ? 128 : T) norm_grad_kernel(const __gr
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const uint32_t c = (i * T + tid) * VEC;
-            if (c < p.cols) {
+            const uint32_t c = run.col(i);
+            if (!SHIFT && c < p.cols) {   // cols is a multiple of eight, and a block's row of `partial` starts on 16 bytes
+                reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+                reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+            } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) mine[c + e] = acc[i][e];
+                for (int e = 0; e < 8; ++e)
+                    if (c + e < p.cols) mine[c + e] = acc[i][e];
             }
         }
     }
 }
 // Rows too long for registers: both passes read from memory, the sums of dgamma are kept in the block's row of `partial`
-// (every thread its own columns, so no two threads touch a word).
-template <int XT, int DT_, int VEC>
+// (every lane its own columns, so no two threads touch a word).
+template <int XT, bool DSUM, bool SHIFT>
 __global__ void __launch_bounds__(1024) norm_grad_long_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr int ST = DSUM ? XT : ROW_NONE, W = 2 * RowElem<XT>::kBytes;
     __shared__ float2 scratch[2][32];
     griddep_wait();
     griddep_launch_dependents();
+    const uint32_t pieces = (p.cols + 32 * 256 - 1) / (32 * 256);
+    const WarpRun run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
     float* mine = p.partial ? p.partial + uint64_t(blockIdx.x) * p.cols : nullptr;
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        const uint64_t xo = row_offset(p.x, row, p.dims, p.flat), yo = row_offset(p.dy, row, p.dims, p.flat);
-        const uint64_t so = DT_ != ROW_NONE ? row_offset(p.dsum, row, p.dims, p.flat) : 0, oo = row_offset(p.dx, row, p.dims, p.flat);
+        const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat)), yin(p.dy, row_offset(p.dy, row, p.dims, p.flat));
+        const RowIn<ST, SHIFT> sin(p.dsum, DSUM ? row_offset(p.dsum, row, p.dims, p.flat) : 0);
+        auto read = [&](uint32_t i, int n, float (&x)[8], float (&y)[8], float (&g)[8]) {
+            typename RowIn<XT, SHIFT>::Raw xr, yr;
+            uint32_t xw[W], yw[W];
+            xin.load(xr, run.col(i));
+            yin.load(yr, run.col(i));
+            load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+            xin.words(xr, xw);
+            yin.words(yr, yw);
+            unpack<XT>(xw, x);
+            unpack<XT>(yw, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (SHIFT && e >= n) x[e] = y[e] = 0.0f;
+        };
         float squares = 0.0f, dot = 0.0f;
 #pragma unroll 1
-        for (uint32_t c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-            RowPiece<XT, VEC> xs, ys;
-            float g[VEC];
-            xs.load(p.x.ptr, xo + c);
-            ys.load(p.dy.ptr, yo + c);
-            load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
+        for (uint32_t i = 0; i < pieces && run.any(i); ++i) {
+            const int n = run.size(i);
+            if (n) {
+                float x[8], y[8], g[8];
+                read(i, n, x, y, g);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float x = xs.value(e);
-                squares = fmaf(x, x, squares);
-                dot = fmaf(ys.value(e) * g[e], x, dot);
+                for (int e = 0; e < 8; ++e) {
+                    squares = fmaf(x[e], x[e], squares);
+                    dot = fmaf(y[e] * g[e], x[e], dot);
+                }
             }
         }
-        const float2 s = reduce_row2<1024>(squares, dot, scratch[turn]);
-        const float inv = inverse_rms(s.x, p.cols, p.eps);
-        const float mean_au = __fdiv_rn(s.y, float(p.cols)) * inv;
+        const float2 s = reduce_row<true, false>(squares, dot, 32, scratch[turn]);
+        const float inv = inverse_rms(s.x, p.per_col, p.eps);
+        const float mean_au = s.y * p.per_col * inv;
         const bool first = row == blockIdx.x;
+        RowOut<XT, SHIFT> out(p.dx, row_offset(p.dx, row, p.dims, p.flat));
 #pragma unroll 1
-        for (uint32_t c = threadIdx.x * VEC; c < p.cols; c += 1024 * VEC) {
-            RowPiece<XT, VEC> xs, ys;
-            RowPiece<DT_, VEC> ds;
-            float g[VEC], d[VEC];
-            xs.load(p.x.ptr, xo + c);
-            ys.load(p.dy.ptr, yo + c);
-            ds.load(p.dsum.ptr, so + c);
-            load_gamma<VEC>(g, p.gamma, p.gamma_type, c);
+        for (uint32_t i = 0; i < pieces && run.any(i); ++i) {
+            const uint32_t c = run.col(i);
+            const int n = run.size(i);
+            uint32_t w[W];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const float u = xs.value(e) * inv, y = ys.value(e);
-                d[e] = (y * g[e] - u * mean_au) * inv;
-                if constexpr (DT_ != ROW_NONE) d[e] += ds.value(e);
-                if (mine) mine[c + e] = first ? y * u : fmaf(y, u, mine[c + e]);
+            for (int k = 0; k < W; ++k) w[k] = 0;
+            if (n) {
+                float x[8], y[8], g[8], d[8], sv[8];
+                read(i, n, x, y, g);
+                if constexpr (DSUM) {
+                    typename RowIn<ST, SHIFT>::Raw sr;
+                    uint32_t sw[W];
+                    sin.load(sr, c);
+                    sin.words(sr, sw);
+                    unpack<XT>(sw, sv);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float u = x[e] * inv, t = fmaf(-u, mean_au, y[e] * g[e]);
+                    d[e] = DSUM ? fmaf(t, inv, sv[e]) : t * inv;
+                    if (mine && e < n) mine[c + e] = first ? y[e] * u : fmaf(y[e], u, mine[c + e]);
+                }
+                if constexpr (XT == ROW_BF16) pack_bf16x8(d, w);
+                else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(d[e]);
+                }
             }
-            if (p.dx.type == ROW_BF16) store_bf16<VEC>(p.dx.ptr, oo + c, d);
-            else store_f32<VEC>(p.dx.ptr, oo + c, d);
+            if (SHIFT || n) out.store(c, n, w, run.whole(i), i == 0, run.last(i, pieces));
         }
     }
 }
@@ -564,54 +822,113 @@ __device__ __forceinline__ void column_sums(const float* partial, float* out, ui
 // ------------------------------------------------------------------------------------------ columns, transposed
 // One step per column of x, result transposed. First the columns' maxima (as bit patterns, whose order is the values'; a NaN's
 // is above infinity's, so it stays), then the codes through a tile in shared memory, then the steps in place of the maxima.
-template <int XT>
+// x is read twice; the second pass walks the rows from the end, so that it begins with what the first left in L2.
+template <int XT, bool SHIFT>
+__device__ __forceinline__ void column_values(const QuantTransParams& p, uint32_t row, const typename RowIn<XT, SHIFT>::Raw& x, float (&v)[8]) {
+    const RowIn<XT, SHIFT> in(p.x, uint64_t(row) * p.x_ld);
+    uint32_t w[RowIn<XT, SHIFT>::kWords];
+    in.words(x, w);
+    unpack<XT>(w, v);
+}
+template <int XT, bool SHIFT>
 __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__ QuantTransParams p) {
+    __shared__ float part[8][257];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t c = blockIdx.x * 32 + (threadIdx.x & 31);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
+    const int n = piece_size(c, p.cols);
     const uint32_t rows_per = (p.rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * rows_per, r1 = min(p.rows, r0 + rows_per);
-    __shared__ float part[8][33];
-    float top = 0.0f;
-    if (c < p.cols) {
-#pragma unroll 4
-        for (uint32_t r = r0 + (threadIdx.x >> 5); r < r1; r += 8) {
-            RowPiece<XT, 1> x;
-            x.load(p.x, uint64_t(r) * p.x_ld + c);
-            top = max_nan(top, fabsf(x.value(0)));
+    float top[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top[e] = 0.0f;
+    if (n) {
+#pragma unroll 1
+        for (uint32_t r = r0 + warp; r < r1; r += 32) {
+            typename RowIn<XT, SHIFT>::Raw x[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r + 8 * j < r1) RowIn<XT, SHIFT>(p.x, uint64_t(r + 8 * j) * p.x_ld).load(x[j], c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r + 8 * j < r1) {
+                    float v[8];
+                    column_values<XT, SHIFT>(p, r + 8 * j, x[j], v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) top[e] = max_nan(top[e], fabsf(v[e]));   // of missing columns: never read
+                }
         }
     }
-    part[threadIdx.x >> 5][threadIdx.x & 31] = top;
-    __syncthreads();
-    if (threadIdx.x < 32 && c < p.cols) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = max_nan(top, part[i][threadIdx.x]);
-        atomicMax(reinterpret_cast<uint32_t*>(p.scale) + c, __float_as_uint(top) & 0x7FFFFFFFu);
-    }
+    for (int e = 0; e < 8; ++e) part[warp][e * 32 + lane] = top[e];
+    __syncthreads();
+    const uint32_t mine = blockIdx.x * 256 + (threadIdx.x & 31) * 8 + (threadIdx.x >> 5);
+    float t = part[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t = max_nan(t, part[i][threadIdx.x]);
+    if (mine < p.cols) atomicMax(reinterpret_cast<uint32_t*>(p.scale) + mine, __float_as_uint(t) & 0x7FFFFFFFu);
 }
-template <int XT>
+// Tiles of 128 rows x 64 columns, kTransTiles of them one below the other per block: a thread takes four rows of eight
+// columns, whose codes make one word per column. A tile's columns leave as aligned 16-byte words (byte by byte at their ends).
+constexpr uint32_t kTransTiles = 4;
+template <int XT, bool SHIFT, bool I8, bool GIVEN>
 __global__ void __launch_bounds__(256) quant_trans_kernel(const __grid_constant__ QuantTransParams p) {
-    __shared__ uint8_t tile[64][68];   // [column][row]
+    constexpr uint32_t kPitch = 33;   // words: 128 rows and one word that keeps the banks apart
+    __shared__ uint32_t tile[64 * kPitch + 4];
+    __shared__ CodeStep steps[64];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-    const uint32_t cl = threadIdx.x & 63, c = c0 + cl;
-    if (c < p.cols) {
-        const RowStep s = make_row_step(p.given ? p.given[uint64_t(c) * p.given_stride] : __fdiv_rn(p.scale[c], p.top));
-#pragma unroll 4
-        for (uint32_t i = threadIdx.x >> 6; i < 64; i += 4) {
-            if (r0 + i < p.rows) {
-                RowPiece<XT, 1> x;
-                x.load(p.x, uint64_t(r0 + i) * p.x_ld + c);
-                const float v[1] = {x.value(0)};
-                store_codes<1>(&tile[0][0], cl * 68 + i, v, p.out_type, s, p.hw);
+    const uint32_t c0 = blockIdx.x * 64;
+    if (threadIdx.x < 64) {
+        const uint32_t c = c0 + threadIdx.x;
+        float s = 0.0f;
+        if (c < p.cols) s = GIVEN ? p.given[uint64_t(c) * p.given_stride] : __fdiv_rn(p.scale[c], p.top);
+        steps[threadIdx.x] = make_code_step(s);
+    }
+    const uint32_t cg = threadIdx.x & 7, rq = threadIdx.x >> 3, cc = c0 + cg * 8;
+    const bool exists = cc < p.cols;
+#pragma unroll 1
+    for (uint32_t t = 0; t < kTransTiles; ++t) {
+        const uint32_t block = gridDim.y - 1 - blockIdx.y, r0 = (block * kTransTiles + (kTransTiles - 1 - t)) * 128;
+        if (r0 >= p.rows) continue;   // uniform over the block
+        const uint32_t r = r0 + rq * 4;
+        typename RowIn<XT, SHIFT>::Raw x[4];
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (exists && r + j < p.rows) RowIn<XT, SHIFT>(p.x, uint64_t(p.row0 + r + j) * p.x_ld).load(x[j], cc);
+        __syncthreads();   // the steps are there, and the tile before has left
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (exists && r + j < p.rows) column_values<XT, SHIFT>(p, p.row0 + r + j, x[j], v[j]);
+            else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
             }
         }
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x >> 6; i < 64; i += 4) {
-        const uint32_t r = threadIdx.x & 63;
-        if (c0 + i < p.cols && r0 + r < p.rows) static_cast<uint8_t*>(p.out)[uint64_t(c0 + i) * p.out_ld + r0 + r] = tile[i][r];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) tile[(cg * 8 + e) * kPitch + rq] = make_codes<I8, GIVEN>(v[0][e], v[1][e], v[2][e], v[3][e], steps[cg * 8 + e], p.hw);
+        __syncthreads();
+        const uint32_t rows = min(128u, p.rows - r0), cols = min(64u, p.cols - c0);
+        // nine 16-byte words cover a column's 128 bytes at any alignment
+        for (uint32_t i = threadIdx.x; i < cols * 9; i += 256) {
+            const uint32_t col = i / 9, k = i % 9;
+            uint8_t* a = static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0;
+            const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u;
+            const int begin = int(16 * k) - int(off);   // first row of the word
+            if (begin >= int(rows)) continue;
+            const uint32_t* column = tile + col * kPitch;
+            if (begin >= 0 && begin + 16 <= int(rows)) {
+                const uint32_t q = uint32_t(begin) >> 2, sh = (uint32_t(begin) & 3u) * 8;
+                uint32_t w[5], o[4];
+    #pragma unroll
+                for (int j = 0; j < 5; ++j) w[j] = column[q + j];   // the fifth word (the padding, at the end) counts only when sh != 0
+    #pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], sh);
+                *reinterpret_cast<uint4*>(a + begin) = make_uint4(o[0], o[1], o[2], o[3]);
+            } else {
+                for (int r = max(begin, 0); r < min(begin + 16, int(rows)); ++r) a[r] = uint8_t(column[r >> 2] >> (8 * (r & 3)));
+            }
+        }
     }
 }
 __device__ __forceinline__ void column_steps(float* scale, uint32_t cols, float top) {

@@ -11,17 +11,22 @@ namespace mmeb200 {
 
 enum : int { ROW_NONE = 0, ROW_BF16 = 1, ROW_F32 = 2, ROW_I8 = 3, ROW_F8 = 4 };   // element types of the row kernels
 
+// What a norm writes: floats, codes whose step the row decides, codes under a given scale.
+enum : int { NORM_BF16 = 0, NORM_F32 = 1, NORM_I8 = 2, NORM_F8 = 3, NORM_I8_GIVEN = 4, NORM_F8_GIVEN = 5 };
+
 // Rows of a tensor: row r is the index of dims 1..4 with dim 1 fastest; element c of it sits at base + off(r) + c.
 struct RowTensor {
     void* ptr;
     int type;              // ROW_*
     uint32_t stride[4];    // elements, dims 1..4
+    uint64_t bytes;        // from the first element to the last
 };
 
 struct NormParams {
     RowTensor x, residual, sum, out;
     const void* gamma;     // nullptr: ones
     int gamma_type;
+    uint32_t gamma_whole;  // gamma starts on 16 bytes
     float* scale;          // 8-bit outputs: the step of every row (written)
     const float* given;    // 8-bit outputs with a given scale: read instead; given_stride 0 = one for all rows
     uint32_t given_stride;
@@ -29,7 +34,8 @@ struct NormParams {
     uint32_t dims[4];      // sizes of dims 1..4
     uint32_t flat;         // 1: rows are dims[0] alone (no division per row)
     uint32_t norm;         // 0: quantise x as it is
-    float eps;
+    int mode;              // NORM_*
+    float eps, per_col;    // per_col: 1 / cols
     float top;             // largest code of the 8-bit output
     Fp8HwCast hw;          // ROW_F8
 };
@@ -38,17 +44,17 @@ struct NormGradParams {
     RowTensor dx, dy, x, dsum;
     const void* gamma;
     int gamma_type;
+    uint32_t gamma_whole;
     float* partial;        // [blocks][cols]; nullptr: no gradient of gamma wanted
     uint32_t rows, cols;
     uint32_t dims[4];
     uint32_t flat;
-    float eps;
+    float eps, per_col;
 };
 
 // Quantisation of columns with a transposed result: x is rows x cols (cols fastest), out cols x rows (rows fastest).
 struct QuantTransParams {
-    const void* x;
-    int x_type;
+    RowTensor x;
     uint64_t x_ld, out_ld;   // elements between rows of x / of out
     void* out;
     int out_type;
@@ -56,6 +62,7 @@ struct QuantTransParams {
     const float* given;
     uint32_t given_stride;
     uint32_t rows, cols;
+    uint32_t row0;           // first of the rows this launch quantises (the maxima are of all)
     float top;
     Fp8HwCast hw;
 };
@@ -66,14 +73,14 @@ struct RowLaunch {
     bool dependent_launch;
 };
 
-// `vec`: every row of every tensor may be read and written eight elements at a time.
+// `vec`: the length, start and pitch of every row of every tensor allow aligned accesses of eight elements.
 cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec);
 // Blocks the gradient kernel runs with, i.e. rows of `partial`.
 uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols);
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks);
 cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols);
 // Number of kernels launched is returned in *launches.
-cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int* launches);
+cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, bool vec, int* launches);
 
 // Rows of `cols` bytes, src_ld bytes apart at any alignment, copied to rows dst_ld bytes apart (dst and dst_ld multiples of 16).
 cudaError_t launch_pad_rows(const RowLaunch& env, const void* src, void* dst, uint64_t rows, uint64_t cols, uint64_t src_ld, uint64_t dst_ld);

@@ -10,13 +10,13 @@ from intel_gaudi3_software_b200 import abi
 U = 2.0 ** -24
 # half a step of the output types, relative
 HALF = {abi.BF16: 2.0 ** -8, abi.FP32: 2.0 ** -24}
-# Additions a term of a row's sum passes through: at most 32 values per thread, then at most ten levels of pairwise sums.
-# Rows above 32768 columns (16384 where rows are read element by element) are summed with one more value for every 1024 columns.
-ROW_DEPTH = 42
+# Additions a term of a row's sum passes through: at most 64 values of its thread, five levels over the warp, at most 16 warps.
+# Rows above 32768 columns (8192 in the gradient): 32 warps, eight values for every 8192 columns.
+ROW_DEPTH = 64 + 5 + 16
 
 
 def row_depth(cols):
-    return max(ROW_DEPTH, cols // 1024 + 11)
+    return max(ROW_DEPTH, 8 * -(-cols // 8192) + 5 + 32)
 
 
 def top_of(dtype, bias=7, mode=abi.INFNAN_MINIMAL):
