@@ -42,6 +42,9 @@ struct Tuning {
     int host_pipeline = -1;   // 0: host-tensor GEMMs are staged whole instead of pipelined
     int tile_n = -1;          // CTA-pair kernel: forced tile width (a multiple of 32 in [32, 256])
     int stream_k = -1;        // 1: cut the tiles of a ragged last wave along K (CTA-pair kernel) whenever a cut exists
+    int token_tile = -1;      // few-token products: tokens of a tile (> 0, rounded up to a multiple of 16)
+    int token_split = -1;     // few-token products: CTAs that share a tile's k blocks (1..8)
+    int token_ctas = -1;      // few-token products: CTAs per SM (1..3)
     int dependent_launch = -1;   // 0: the CTA-pair kernel is launched without programmatic stream serialisation
 };
 static int env_int(const char* name, int dflt) {
@@ -1200,7 +1203,8 @@ int mmeb200_set_option(mmeb200_ctx* c, const char* name, int value) {
     struct { const char* name; int Tuning::*field; } const table[] = {
         {"pair", &Tuning::pair}, {"block_n", &Tuning::block_n}, {"split_k", &Tuning::split_k}, {"epi_groups", &Tuning::epi_groups},
         {"raster_gm", &Tuning::raster_gm}, {"tma_store", &Tuning::tma_store}, {"host_pipeline", &Tuning::host_pipeline},
-        {"tile_n", &Tuning::tile_n}, {"stream_k", &Tuning::stream_k}, {"dependent_launch", &Tuning::dependent_launch}};
+        {"tile_n", &Tuning::tile_n}, {"stream_k", &Tuning::stream_k}, {"dependent_launch", &Tuning::dependent_launch},
+        {"token_tile", &Tuning::token_tile}, {"token_split", &Tuning::token_split}, {"token_ctas", &Tuning::token_ctas}};
     for (const auto& t : table)
         if (strcmp(t.name, name) == 0) {
             c->tune.*(t.field) = value < 0 ? -1 : value;

@@ -20,7 +20,7 @@ static int g_max_pairs[64] = {};
 
 static LaunchResult configure(const LaunchEnv& env, int* pairs) {
     auto kern = gemm_tcgen05_pair_kernel<INST_KIND, INST_PAIR_EPI, INST_PAIR_CUT != 0, INST_PAIR_SCALED != 0>;
-    constexpr int smem = PairSmem<INST_PAIR_EPI>::kTotal;
+    constexpr int smem = PairSmem<INST_PAIR_EPI>::kTotal + (INST_PAIR_SCALED ? int(kScaledSmemBytes) : 0);
     constexpr int threads = PairSmem<INST_PAIR_EPI>::kThreads;
     int& cached = g_max_pairs[env.device & 63];
     if (cached == 0) {
@@ -57,7 +57,7 @@ LaunchResult INST_NAME(const LaunchEnv& env, const GemmParams& p, uint64_t tiles
     int cap = 0;
     const LaunchResult r = configure(env, &cap);
     if (r.cuda != cudaSuccess || r.code != LAUNCH_OK) return r;
-    constexpr int smem = PairSmem<INST_PAIR_EPI>::kTotal;
+    constexpr int smem = PairSmem<INST_PAIR_EPI>::kTotal + (INST_PAIR_SCALED ? int(kScaledSmemBytes) : 0);
     constexpr int threads = PairSmem<INST_PAIR_EPI>::kThreads;
     const unsigned pairs = unsigned(tiles < uint64_t(cap) ? tiles : uint64_t(cap));
     cudaLaunchConfig_t cfg;

@@ -74,7 +74,6 @@ struct ScaledOut {
     const void* col_bias;       // nullptr: none
     uint32_t row_stride, col_stride;
     uint32_t bias_bf16;         // element type of col_bias: bf16, else fp32
-    uint32_t col_vec;           // col_scale and col_bias may be read 16 bytes at a time
 };
 
 struct GemmParams {
@@ -603,53 +602,40 @@ __device__ __forceinline__ float scaled_acc(uint32_t v) {
     if constexpr (KIND == KIND_I8) return __int2float_rn(int(v));
     else return __uint_as_float(v);
 }
-// 32 accumulator columns from col0 on of a row whose scale is xs -> packed bf16 or fp32 outputs, rounded once.
-// Only the first `ncols` columns exist; the rest of v is left undefined.
+// Scales and biases of the tile's columns, staged in shared memory by the group of epilogue warps that shares them: read from
+// global memory once per tile, while its MMAs still run, and not once per row block behind them.
+constexpr uint32_t kScaledCols = 256;
+constexpr uint32_t kScaledSmemBytes = kScaledCols * 2 * sizeof(float);   // [columns] scales, then [columns] biases
+__device__ __forceinline__ void stage_columns(const GemmParams& p, float* cols, uint32_t count, uint32_t n0, uint32_t thread) {
+    for (uint32_t i = thread; i < count; i += 128) {
+        const uint32_t n = n0 + i;
+        const bool there = n < p.N;
+        cols[i] = there ? p.scaled.col_scale[uint64_t(n) * p.scaled.col_stride] : 0.0f;
+        cols[kScaledCols + i] = there && p.scaled.col_bias ? scaled_bias(p.scaled, n) : 0.0f;
+    }
+}
+// 32 accumulator columns of a row whose scale is xs -> packed bf16 or fp32 outputs, rounded once. cols: the staged scales of
+// these columns.
 template <int KIND>
-__device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const GemmParams& p, float xs, uint32_t col0, uint32_t out_elem) {
-    const ScaledOut& so = p.scaled;
-    const bool whole = so.col_vec && col0 + 32 <= p.N;
-    const float same = so.col_stride ? 0.0f : so.col_scale[0];
+__device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const float* cols, bool has_bias, float xs, uint32_t out_elem) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-        float w[4], b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (whole) {
-            const float4 t = __ldg(reinterpret_cast<const float4*>(so.col_scale + col0) + q);
-            w[0] = t.x; w[1] = t.y; w[2] = t.z; w[3] = t.w;
-            if (so.col_bias) {
-                if (so.bias_bf16) {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(so.col_bias) + col0) + q);
-                    b[0] = __uint_as_float(u.x << 16); b[1] = __uint_as_float(u.x & 0xFFFF0000u);
-                    b[2] = __uint_as_float(u.y << 16); b[3] = __uint_as_float(u.y & 0xFFFF0000u);
-                } else {
-                    const float4 u = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(so.col_bias) + col0) + q);
-                    b[0] = u.x; b[1] = u.y; b[2] = u.z; b[3] = u.w;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t n = col0 + 4 * q + e;
-                w[e] = same;
-                if (n < p.N) {
-                    if (so.col_stride) w[e] = so.col_scale[n];
-                    if (so.col_bias) b[e] = scaled_bias(so, n);
-                }
-            }
-        }
-        float y[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = scaled_acc<KIND>(v[4 * q + e]) * xs * w[e];
-        if (so.col_bias) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] += b[e];
+        const float4 w = reinterpret_cast<const float4*>(cols)[q];
+        float2 y0 = make_float2(scaled_acc<KIND>(v[4 * q]), scaled_acc<KIND>(v[4 * q + 1]));
+        float2 y1 = make_float2(scaled_acc<KIND>(v[4 * q + 2]), scaled_acc<KIND>(v[4 * q + 3]));
+        y0 = __fmul2_rn(__fmul2_rn(y0, make_float2(xs, xs)), make_float2(w.x, w.y));
+        y1 = __fmul2_rn(__fmul2_rn(y1, make_float2(xs, xs)), make_float2(w.z, w.w));
+        if (has_bias) {
+            const float4 b = reinterpret_cast<const float4*>(cols + kScaledCols)[q];
+            y0 = __fadd2_rn(y0, make_float2(b.x, b.y));
+            y1 = __fadd2_rn(y1, make_float2(b.z, b.w));
         }
         if (out_elem == 2) {   // words 2q, 2q + 1 lie below every value still to be read
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q]) : "f"(y[1]), "f"(y[0]));
-            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q + 1]) : "f"(y[3]), "f"(y[2]));
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q]) : "f"(y0.y), "f"(y0.x));
+            asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q + 1]) : "f"(y1.y), "f"(y1.x));
         } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * q + e] = __float_as_uint(y[e]);
+            v[4 * q] = __float_as_uint(y0.x); v[4 * q + 1] = __float_as_uint(y0.y);
+            v[4 * q + 2] = __float_as_uint(y1.x); v[4 * q + 3] = __float_as_uint(y1.y);
         }
     }
 }
@@ -657,11 +643,11 @@ __device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const GemmPar
 // Epilogue of one output tile, run by one epilogue warp for its 32 rows: reads `tile_cols` accumulator columns (a
 // multiple of 32) from tensor memory (tmem_acc = the warp's lane window of the tile's accumulator), converts and stores
 // them. m0 is the first row of the CTA's 128-row block, n0 the first column.
-// SCALED: -1, or the KIND_* of a scaled product (epilogue_scaled takes the place of the cast).
+// SCALED: -1, or the KIND_* of a scaled product (epilogue_scaled takes the place of the cast; scaled_cols: stage_columns').
 template <bool FIX = false, int SCALED = -1>
 __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile_cols, uint32_t m0, uint32_t n0, uint32_t batch, uint32_t split,
                                               uint32_t tmem_acc, uint8_t* stage_out, uint32_t& store_buf, uint32_t sub, uint32_t lane,
-                                              uint32_t out_elem, const SkFix& fix = SkFix{nullptr, 0u, 0u}) {
+                                              uint32_t out_elem, const SkFix& fix = SkFix{nullptr, 0u, 0u}, const float* scaled_cols = nullptr) {
     const uint32_t row = m0 + sub * 32 + lane;
     uint32_t bi[3];
     {
@@ -714,7 +700,7 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile
                 tmem_ld_32x32b_x32(tmem_acc + ch * cols_per_chunk + l * 32, v);
                 if constexpr (FIX) tmem_ld_wait_add(v, fix, fix.col0 + ch * cols_per_chunk + l * 32, sub * 32 + lane);
                 else tmem_ld_wait();
-                if constexpr (SCALED >= 0) epilogue_scaled<SCALED>(v, p, xs, col0 + l * 32, out_elem);
+                if constexpr (SCALED >= 0) epilogue_scaled<SCALED>(v, scaled_cols + ch * cols_per_chunk + l * 32, p.scaled.col_bias != nullptr, xs, out_elem);
                 else epilogue_convert(v, p, out_elem, flat_row + col0 + l * 32);
                 if (out_elem == 4) {
 #pragma unroll
@@ -739,28 +725,65 @@ __device__ __forceinline__ void epilogue_tile(const GemmParams& p, uint32_t tile
             store_buf ^= 1;
         }
     }
-    // ---- direct stores: everything when no tensor map applies (unaligned outputs, split-K partials), else the
-    //      columns left over after the last whole 128-byte chunk of a narrowed tile
+    if constexpr (SCALED >= 0) {
+        // ---- outputs whose rows no tensor map describes: 32 x 32 blocks are turned in shared memory, so that a warp writes 32
+        //      consecutive columns of a row at a time (one row per lane would touch 32 rows with every store)
+        uint32_t* turn = reinterpret_cast<uint32_t*>(stage_out + sub * (2 * 32 * kRowBytes));   // 32 rows of 33 (fp32) or 17 (bf16) words
+        const uint32_t pitch = out_elem == 2 ? 17u : 33u, row0 = m0 + sub * 32;
 #pragma unroll 1
-    for (uint32_t c0 = done_cols; c0 < tile_cols; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(tmem_acc + c0, v);
-        if constexpr (FIX) tmem_ld_wait_add(v, fix, fix.col0 + c0, sub * 32 + lane);
-        else tmem_ld_wait();
-        const uint32_t col0 = n0 + c0;
-        if (row >= p.M || col0 >= p.N) continue;
-        const uint32_t ncols = min(32u, p.N - col0);
-        uint32_t elem = 4;
-        uint8_t* dst;
-        if (p.split_k > 1) {
-            dst = reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) + base_off + col0);
-        } else {
-            elem = out_elem;
-            dst = reinterpret_cast<uint8_t*>(p.out) + (base_off + col0) * out_elem;
-            if constexpr (SCALED >= 0) epilogue_scaled<SCALED>(v, p, xs, col0, out_elem);
-            else epilogue_convert(v, p, out_elem, flat_row + col0);
+        for (uint32_t c0 = done_cols; c0 < tile_cols; c0 += 32) {
+            const uint32_t col0 = n0 + c0;
+            if (col0 >= p.N || row0 >= p.M) break;   // uniform over the warp
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem_acc + c0, v);
+            tmem_ld_wait();
+            epilogue_scaled<SCALED>(v, scaled_cols + c0, p.scaled.col_bias != nullptr, xs, out_elem);
+            __syncwarp();   // the block before has been read
+#pragma unroll
+            for (int j = 0; j < 16; ++j) turn[lane * pitch + j] = v[j];
+            if (out_elem == 4) {
+#pragma unroll
+                for (int j = 16; j < 32; ++j) turn[lane * pitch + j] = v[j];
+            }
+            __syncwarp();
+            const uint32_t rows = min(32u, p.M - row0);
+            if (col0 + lane < p.N) {
+                uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + (uint64_t(row0) * p.out_ld + col0 + lane) * out_elem;
+                const uint64_t step = p.out_ld * out_elem;
+                if (out_elem == 4) {
+#pragma unroll 8
+                    for (uint32_t r = 0; r < rows; ++r, dst += step) *reinterpret_cast<uint32_t*>(dst) = turn[r * 33 + lane];
+                } else {
+                    const uint32_t half = (lane & 1) * 16;
+#pragma unroll 8
+                    for (uint32_t r = 0; r < rows; ++r, dst += step) *reinterpret_cast<uint16_t*>(dst) = uint16_t(turn[r * 17 + (lane >> 1)] >> half);
+                }
+            }
         }
-        store_row32(v, dst, elem, ncols);   // v[0 .. 8*elem) holds 32 packed outputs
+    }
+    if constexpr (SCALED < 0) {
+        // ---- direct stores: everything when no tensor map applies (unaligned outputs, split-K partials), else the
+        //      columns left over after the last whole 128-byte chunk of a narrowed tile
+#pragma unroll 1
+        for (uint32_t c0 = done_cols; c0 < tile_cols; c0 += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(tmem_acc + c0, v);
+            if constexpr (FIX) tmem_ld_wait_add(v, fix, fix.col0 + c0, sub * 32 + lane);
+            else tmem_ld_wait();
+            const uint32_t col0 = n0 + c0;
+            if (row >= p.M || col0 >= p.N) continue;
+            const uint32_t ncols = min(32u, p.N - col0);
+            uint32_t elem = 4;
+            uint8_t* dst;
+            if (p.split_k > 1) {
+                dst = reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) + base_off + col0);
+            } else {
+                elem = out_elem;
+                dst = reinterpret_cast<uint8_t*>(p.out) + (base_off + col0) * out_elem;
+                epilogue_convert(v, p, out_elem, flat_row + col0);
+            }
+            store_row32(v, dst, elem, ncols);   // v[0 .. 8*elem) holds 32 packed outputs
+        }
     }
 }
 

@@ -203,12 +203,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairSmem<EPI_GROUPS>
         sched.init(p, pair);
         TileCoord tc;
         uint32_t kind = WORK_TILE, slot = 0, above_slot = kNoSlot;
+        bool gave_up = false;
+        float* scaled_cols = SCALED ? reinterpret_cast<float*>(smem + S::kTotal) + grp * kGroupCols : nullptr;
         while (sched.next(p, pair, num_pairs, tc, kind, slot, above_slot)) {
-            bool ready = mbar_wait_bounded(&tmem_full_bar[acc], acc_phase, kWaitLimitNs);
+            if constexpr (SCALED) {
+                named_barrier(1 + grp, 128);   // the tile before has been scaled
+                stage_columns(p, scaled_cols, kGroupCols, tc.n0 * p.tile_n + grp * kGroupCols, threadIdx.x & 127);
+                named_barrier(1 + grp, 128);
+            }
+            bool ready = !gave_up && mbar_wait_bounded(&tmem_full_bar[acc], acc_phase, kWaitLimitNs);
             ready = __all_sync(0xffffffffu, ready);
             if (!ready) {
                 atomicCAS(p.status, 0u, WAIT_EPILOGUE_TMEM_FULL);
-                break;
+                if constexpr (SCALED) {   // the group's barriers still need this warp for every tile
+                    gave_up = true;
+                    continue;
+                } else {
+                    break;
+                }
             }
             tc_fence_after_sync();
             const uint32_t tmem_acc = tmem_base + acc * kPairBlockN + grp * kGroupCols + ((sub * 32) << 16);
@@ -237,7 +249,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairSmem<EPI_GROUPS>
                 }
             } else {
                 epilogue_tile<false, SCALED ? KIND : -1>(p, group_cols, tc.m0 * 2 + rank * kBlockM, tc.n0 * p.tile_n + grp * kGroupCols, tc.batch, tc.split,
-                                                         tmem_acc, stage_out, store_buf, sub, lane, out_elem);
+                                                         tmem_acc, stage_out, store_buf, sub, lane, out_elem, SkFix{nullptr, 0u, 0u}, scaled_cols);
             }
             tc_fence_before_sync();
             __syncwarp();

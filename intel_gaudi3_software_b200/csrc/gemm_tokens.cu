@@ -5,15 +5,16 @@
 
 namespace mmeb200 {
 
-constexpr int kTokenSmem = 227 * 1024;
+constexpr int kTokenSmem = 227 * 1024;   // of a CTA alone on an SM
 
-static uint32_t stages_for(uint32_t tok) {
-    const uint32_t bytes = kTokenWBytes + tok * kRowBytes, n = (kTokenSmem - kTokenBarrierBytes) / bytes;
+uint32_t gemm_tokens_stages(uint32_t tok, uint32_t ctas) {
+    const uint32_t smem = ctas == 1 ? kTokenSmem : 228 * 1024 / ctas - 1024;   // 1 KB of every CTA is the system's
+    const uint32_t n = (smem - kTokenBarrierBytes) / (kTokenWBytes + tok * kRowBytes);
     return n < kTokenMaxStages ? n : kTokenMaxStages;
 }
 
 template <int KIND>
-static cudaError_t configure(const LaunchEnv& env, uint32_t tok, uint32_t splits, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs) {
+static cudaError_t configure(const LaunchEnv& env, uint32_t tok, uint32_t splits, uint32_t ctas, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs) {
     static bool done[64] = {};
     if (!done[env.device & 63]) {
         const cudaError_t e = cudaFuncSetAttribute(gemm_tokens_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTokenSmem);
@@ -22,7 +23,7 @@ static cudaError_t configure(const LaunchEnv& env, uint32_t tok, uint32_t splits
     }
     memset(cfg, 0, sizeof *cfg);
     cfg->blockDim = dim3(kTokenThreads);
-    cfg->dynamicSmemBytes = stages_for(tok) * (kTokenWBytes + tok * kRowBytes) + kTokenBarrierBytes;
+    cfg->dynamicSmemBytes = gemm_tokens_stages(tok, ctas) * (kTokenWBytes + tok * kRowBytes) + kTokenBarrierBytes;
     cfg->stream = env.stream;
     attrs[0].id = cudaLaunchAttributeClusterDimension;
     attrs[0].val.clusterDim.x = splits; attrs[0].val.clusterDim.y = 1; attrs[0].val.clusterDim.z = 1;
@@ -37,10 +38,10 @@ template <int KIND>
 static LaunchResult launch(const LaunchEnv& env, TokenGemmParams& p) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attrs[2];
-    cudaError_t e = configure<KIND>(env, p.tok, p.splits, &cfg, attrs);
+    cudaError_t e = configure<KIND>(env, p.tok, p.splits, p.ctas, &cfg, attrs);
     if (e != cudaSuccess) return {e, LAUNCH_OK, "cudaFuncSetAttribute(few-token kernel)"};
     p.stage_bytes = kTokenWBytes + p.tok * kRowBytes;
-    p.stages = stages_for(p.tok);
+    p.stages = gemm_tokens_stages(p.tok, p.ctas);
     p.tmem_cols = 32;
     while (p.tmem_cols < p.tok) p.tmem_cols *= 2;
     cfg.gridDim = dim3(p.splits * ((p.N + kBlockM - 1) / kBlockM), (p.M + p.tok - 1) / p.tok);
@@ -53,10 +54,10 @@ LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmPa
 }
 
 template <int KIND>
-static int capacity(const LaunchEnv& env, uint32_t tok, uint32_t splits) {
+static int capacity(const LaunchEnv& env, uint32_t tok, uint32_t splits, uint32_t ctas) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attrs[2];
-    if (configure<KIND>(env, tok, splits, &cfg, attrs) != cudaSuccess) return 0;
+    if (configure<KIND>(env, tok, splits, ctas, &cfg, attrs) != cudaSuccess) return 0;
     cfg.gridDim = dim3(splits * unsigned(env.sm_count));
     cfg.numAttrs = 1;
     int n = 0;
@@ -70,8 +71,8 @@ LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& 
     return {cudaGetLastError(), LAUNCH_OK, "empty-sum kernel launch"};
 }
 
-int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits) {
-    return kind == KIND_I8 ? capacity<KIND_I8>(env, tok, splits) : capacity<KIND_F8>(env, tok, splits);
+int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
+    return kind == KIND_I8 ? capacity<KIND_I8>(env, tok, splits, ctas) : capacity<KIND_F8>(env, tok, splits, ctas);
 }
 
 }  // namespace mmeb200

@@ -11,6 +11,9 @@
 // sums for them, adds them in rank order (integer sums are exact anyway; fp32 sums have a fixed order) and writes them
 // out. No workspace in global memory, no second launch, no atomics.
 //
+// Two CTAs share an SM wherever a tile has at most 128 tokens: one's set-up and epilogue run under the other's stream, and a
+// number of CTAs that is not a multiple of the SMs' still keeps HBM busy to the end.
+//
 // CTA layout (192 threads): warp 0 feeds the ring by TMA, warp 1 allocates tensor memory and issues the MMAs, warps 2-5 are
 // the epilogue (lane = channel). Every mbarrier wait is bounded as in the other GEMM kernels.
 #pragma once
@@ -23,11 +26,10 @@ constexpr uint32_t kTokenBarrierBytes = 256;
 constexpr uint32_t kTokenWBytes = kBlockM * kRowBytes;
 constexpr uint32_t kTokenMaxStages = 12;
 
-// The outputs of one token: 32 lanes write 32 consecutive channels.
-__device__ __forceinline__ void token_store(const TokenGemmParams& p, uint32_t m, uint32_t n, float acc, float xs, float ws, float bias) {
-    float y = acc * xs * ws;
-    if (p.scaled.col_bias) y += bias;
-    if (p.out_bf16) {
+// One output: 32 lanes write 32 consecutive channels of a token.
+template <bool BF16>
+__device__ __forceinline__ void token_put(const TokenGemmParams& p, uint32_t m, uint32_t n, float y) {
+    if constexpr (BF16) {
         uint32_t w;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(0.0f), "f"(y));
         static_cast<uint16_t*>(p.out)[uint64_t(m) * p.out_ld + n] = uint16_t(w);
@@ -35,9 +37,33 @@ __device__ __forceinline__ void token_store(const TokenGemmParams& p, uint32_t m
         static_cast<float*>(p.out)[uint64_t(m) * p.out_ld + n] = y;
     }
 }
-
+// COUNT consecutive tokens of this lane's channel: acc * (the token's scale, held by lane `place` + j) * ws + bias. `exist` of
+// them exist. All values first, then all stores: nothing waits between two of them.
+template <int KIND, bool BF16, int COUNT>
+__device__ __forceinline__ void token_put_all(const TokenGemmParams& p, const uint32_t* v, uint32_t m, uint32_t exist, uint32_t n, float scales, uint32_t place, float ws,
+                                              float bias) {
+    float y[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) y[j] = fmaf(scaled_acc<KIND>(v[j]) * __shfl_sync(0xffffffffu, scales, place + j), ws, bias);
+    if (n < p.N) {
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j)
+            if (uint32_t(j) < exist) token_put<BF16>(p, m + j, n, y[j]);
+    }
+}
+template <int KIND, int COUNT>
+__device__ __forceinline__ void token_store(const TokenGemmParams& p, const uint32_t* v, uint32_t m, uint32_t exist, uint32_t n, float scales, uint32_t place, float ws,
+                                            float bias) {
+    if (p.out_bf16) token_put_all<KIND, true, COUNT>(p, v, m, exist, n, scales, place, ws, bias);
+    else token_put_all<KIND, false, COUNT>(p, v, m, exist, n, scales, place, ws, bias);
+}
 template <int KIND>
-__global__ void __launch_bounds__(kTokenThreads, 1) gemm_tokens_kernel(const __grid_constant__ TokenGemmParams p) {
+__device__ __forceinline__ uint32_t token_add(uint32_t a, uint32_t b) {
+    if constexpr (KIND == KIND_I8) return a + b;
+    else return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+template <int KIND>
+__global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __grid_constant__ TokenGemmParams p) {
     griddep_launch_dependents();
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {   // uniform over the cluster
@@ -130,53 +156,63 @@ __global__ void __launch_bounds__(kTokenThreads, 1) gemm_tokens_kernel(const __g
     }
 
     const uint32_t tokens = min(p.tok, p.M - m0);
+    // the scale of a token, held by the lane of its place among 32 tokens
+    auto token_scale = [&](uint32_t first) {
+        const uint32_t t = first + lane;
+        return t < tokens ? p.scaled.row_scale[uint64_t(m0 + t) * p.scaled.row_stride] * p.scale : 0.0f;
+    };
     if (p.splits == 1) {
         if (warp >= 2 && ready) {
+            float xs = 0.0f;
             for (uint32_t c0 = 0; c0 < tokens; c0 += 16) {
                 uint32_t v[16];
                 tmem_ld_32x32b_x16(tmem_base + c0 + ((sub * 32) << 16), v);
+                if ((c0 & 31) == 0) xs = token_scale(c0);
                 tmem_ld_wait();
-#pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    const uint32_t m = m0 + c0 + j;
-                    if (c0 + j < tokens && n < p.N)
-                        token_store(p, m, n, scaled_acc<KIND>(v[j]), p.scaled.row_scale[uint64_t(m) * p.scaled.row_stride] * p.scale, ws, bias);
-                }
+                token_store<KIND, 16>(p, v, m0 + c0, tokens - c0, n, xs, c0 & 16, ws, bias);
             }
         }
     } else {
         // Every CTA's stages are idle (its MMAs have completed) before anyone writes into them.
         cluster_sync_all();
-        const uint32_t share = (tokens + p.splits - 1) / p.splits;   // tokens a rank owns
-        uint32_t* inbox = reinterpret_cast<uint32_t*>(smem);         // [source rank][token of the share][channel]
+        const uint32_t share = ((tokens + p.splits - 1) / p.splits + 3) & ~3u;   // tokens a rank owns, in fours
+        const uint32_t channel = sub * 32 + lane;
+        uint4* inbox = reinterpret_cast<uint4*>(smem) + channel;                  // [source rank][four tokens][channel]
         if (warp >= 2 && ready) {
-            const uint32_t channel = sub * 32 + lane;
-            for (uint32_t c0 = 0; c0 < tokens; c0 += 16) {
-                uint32_t v[16];
-                tmem_ld_32x32b_x16(tmem_base + c0 + ((sub * 32) << 16), v);
-                tmem_ld_wait();
+            const uint32_t mine = smem_u32(inbox + rank * (share / 4) * kBlockM);   // the slot of this rank
+            // each rank begins with its own share and goes round, so that no two ranks write to the same CTA at once
+            for (uint32_t i = 0; i < p.splits; ++i) {
+                const uint32_t owner = rank + i < p.splits ? rank + i : rank + i - p.splits, first = owner * share;
+                const uint32_t to = mapa_shared(mine, owner);
+                for (uint32_t t = 0; t < share && first + t < tokens; t += 16) {
+                    uint32_t v[16];
 #pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    if (c0 + j < tokens) {
-                        const uint32_t owner = (c0 + j) / share, t = (c0 + j) - owner * share;
-                        st_shared_cluster_u32(mapa_shared(smem_u32(inbox + (rank * share + t) * kBlockM + channel), owner), v[j]);
-                    }
+                    for (uint32_t j = 0; j < 16; j += 4)
+                        if (t + j < share && first + t + j < tokens) tmem_ld_32x32b_x4(tmem_base + first + t + j + ((sub * 32) << 16), v + j);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j += 4)
+                        if (t + j < share && first + t + j < tokens) st_shared_cluster_v4(to + (t + j) * (kBlockM * 4), v[j], v[j + 1], v[j + 2], v[j + 3]);
                 }
             }
         }
         cluster_sync_all();
         if (warp >= 2) {
-            const uint32_t channel = sub * 32 + lane;
-            for (uint32_t t = 0; t < share; ++t) {
-                const uint32_t m = m0 + rank * share + t;
-                if (rank * share + t >= tokens) break;
-                uint32_t sum = inbox[t * kBlockM + channel];
+            const uint32_t first = rank * share, count = first < tokens ? min(share, tokens - first) : 0;
+            float xs = 0.0f;
+            for (uint32_t t = 0; t < count; t += 4) {
+                if ((t & 31) == 0) xs = token_scale(first + t);
+                uint4 sum = inbox[(t / 4) * kBlockM];
+#pragma unroll 7
                 for (uint32_t r = 1; r < p.splits; ++r) {
-                    const uint32_t v = inbox[(r * share + t) * kBlockM + channel];
-                    if constexpr (KIND == KIND_I8) sum += v;
-                    else sum = __float_as_uint(__uint_as_float(sum) + __uint_as_float(v));
+                    const uint4 v = inbox[(r * share + t) / 4 * kBlockM];
+                    sum.x = token_add<KIND>(sum.x, v.x);
+                    sum.y = token_add<KIND>(sum.y, v.y);
+                    sum.z = token_add<KIND>(sum.z, v.z);
+                    sum.w = token_add<KIND>(sum.w, v.w);
                 }
-                if (n < p.N) token_store(p, m, n, scaled_acc<KIND>(sum), p.scaled.row_scale[uint64_t(m) * p.scaled.row_stride] * p.scale, ws, bias);
+                const uint32_t four[4] = {sum.x, sum.y, sum.z, sum.w};
+                token_store<KIND, 4>(p, four, m0 + first + t, count - t, n, xs, t & 31, ws, bias);
             }
         }
     }
@@ -195,7 +231,9 @@ static __global__ void __launch_bounds__(256) gemm_empty_sum_kernel(const __grid
     const uint64_t total = uint64_t(p.M) * p.N;
     for (uint64_t i = uint64_t(blockIdx.x) * 256 + threadIdx.x; i < total; i += uint64_t(gridDim.x) * 256) {
         const uint32_t m = uint32_t(i / p.N), n = uint32_t(i % p.N);
-        token_store(p, m, n, 0.0f, 0.0f, 0.0f, p.scaled.col_bias ? scaled_bias(p.scaled, n) : 0.0f);
+        const float y = p.scaled.col_bias ? scaled_bias(p.scaled, n) : 0.0f;
+        if (p.out_bf16) token_put<true>(p, m, n, y);
+        else token_put<false>(p, m, n, y);
     }
 }
 

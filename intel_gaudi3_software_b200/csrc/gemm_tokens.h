@@ -15,6 +15,7 @@ struct TokenGemmParams {
     uint32_t num_k_blocks;      // 128-byte blocks of K
     uint32_t tok;               // tokens of a tile (a multiple of 16, at most 256)
     uint32_t splits;            // CTAs of a cluster, each with its share of the k blocks
+    uint32_t ctas;              // CTAs that share an SM (1..3): sets how much shared memory each has for its ring
     uint32_t stages, stage_bytes;
     uint32_t tmem_cols;
     uint32_t idesc;
@@ -31,6 +32,8 @@ LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmPa
 // out = bias (or zero) for operands without a common dimension.
 LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p);
 // Most CTAs the device runs at once in clusters of `splits` with tiles of `tok` tokens (0 on failure).
-int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits);
+int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas);
+// Stages of the ring of a CTA, one of `ctas` on its SM; fewer than three do not keep the tensor cores fed.
+uint32_t gemm_tokens_stages(uint32_t tok, uint32_t ctas);
 
 }  // namespace mmeb200

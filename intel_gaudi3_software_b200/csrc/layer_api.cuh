@@ -298,7 +298,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     p.norm = norm; p.eps = eps; p.per_col = 1.0f / float(cols); p.top = top; p.hw = hw;
     p.mode = out->dtype == DT_BF16 ? NORM_BF16 : out->dtype == DT_FP32 ? NORM_F32 : out->dtype == MMEB200_INT8 ? (given ? NORM_I8_GIVEN : NORM_I8) : given ? NORM_F8_GIVEN : NORM_F8;
     p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.residual, p.dims) && layer_vectors(p.sum, p.dims) && layer_vectors(p.out, p.dims);
+    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.residual, p.dims) && layer_vectors(p.sum, p.dims) && layer_vectors(p.out, p.dims) && p.gamma_whole;
     CUDA_OK(c, launch_norm(layer_launch(c), p, vec));
     c->launches++;
     return st.finish();
@@ -380,7 +380,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         }
     }
     p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.dy, p.dims) && layer_vectors(p.dsum, p.dims) && layer_vectors(p.dx, p.dims) &&
+    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.dy, p.dims) && layer_vectors(p.dsum, p.dims) && layer_vectors(p.dx, p.dims) && p.gamma_whole &&
                      reinterpret_cast<uintptr_t>(p.partial) % 16 == 0;
     CUDA_OK(c, launch_norm_grad(layer_launch(c), p, vec, blocks));
     c->launches++;
@@ -450,26 +450,65 @@ int layer_pad_operand(mmeb200_ctx* c, TmaOperand* o, uint8_t* dst) {
     return 0;
 }
 
-// Few tokens or few tiles: the cluster kernel (gemm_tokens.cuh).
-int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, uint32_t idesc_fmt_x, uint32_t idesc_fmt_w, TokenGemmParams& p) {
-    p.num_k_blocks = uint32_t((ox.inner + kRowBytes - 1) / kRowBytes);
-    const uint32_t m_tiles = (p.M + 255) / 256;
-    p.tok = (((p.M + m_tiles - 1) / m_tiles) + 15) & ~15u;
-    const uint64_t tiles = uint64_t((p.N + kBlockM - 1) / kBlockM) * ((p.M + p.tok - 1) / p.tok);
-    if (tiles * 8 >= (uint64_t(1) << 31) || (p.M + p.tok - 1) / p.tok > 65535) return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");
-    // As many CTAs per tile as the device still runs at once, each with at least four k blocks.
-    static int caps[64][2][9] = {};
-    p.splits = 1;
-    for (uint32_t s = 2; s <= 8; ++s) {
-        int& cap = caps[c->device & 63][kind == KIND_I8][s];
-        if (cap == 0) {
-            cap = gemm_tokens_capacity(launch_env(c), kind, 256, s);
-            if (cap == 0) cap = -1;
-        }
-        const uint32_t per = (p.num_k_blocks + s - 1) / s;
-        if (cap > 0 && tiles * s <= uint64_t(cap) && per >= 4 && per * (s - 1) < p.num_k_blocks) p.splits = s;
+// Which kernel a product takes, and with what tile and split: the choice whose estimated time is least. Both estimates are in
+// SM clocks, from the same few rates: a k block (128 bytes of K) of 128 x 128 products is 256 clocks of the tensor cores, an
+// SM takes in about 60 bytes per clock from L2, the device about 3400 bytes per clock from HBM.
+struct ProductPlan {
+    bool pair;
+    uint32_t tok, splits, ctas;
+    double clocks;
+};
+int layer_token_capacity(mmeb200_ctx* c, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
+    static int caps[64][2][4][9] = {};   // of the full ring, which all tiles nearly have
+    int& cap = caps[c->device & 63][kind == KIND_I8][ctas][splits];
+    if (cap == 0) {
+        cap = gemm_tokens_capacity(launch_env(c), kind, tok, splits, ctas);
+        if (cap == 0) cap = -1;
     }
-    p.idesc = kind == KIND_I8 ? make_instr_desc_i8(kBlockM, p.tok) : make_instr_desc(idesc_fmt_w, idesc_fmt_x, 0, 0, kBlockM, p.tok);
+    return cap;
+}
+ProductPlan layer_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t N, uint32_t kb, uint32_t out_bytes) {
+    const double sms = c->sm_count, bytes = 128.0 * kb * (double(M) + N) + double(M) * N * out_bytes, floor_clocks = bytes / 3400;
+    ProductPlan best{false, 0, 0, 0, 1e300};
+    const bool may_pair = c->tune.pair != 0 && M >= 256 && N >= 256;
+    if (may_pair) {
+        const double tiles = double((M + 255) / 256) * ((N + 255) / 256), waves = ceil(tiles / floor(sms / 2));
+        best = {true, 0, 0, 0, std::max(floor_clocks, waves * (kb * 540.0 + 1500)) + 6000};
+        if (c->tune.pair == 1) return best;
+    }
+    const double channels = (uint64_t(N) + kBlockM - 1) / kBlockM;
+    for (uint32_t want : {16u, 32u, 48u, 64u, 96u, 128u, 192u, 256u}) {
+        // the smallest tile with as many token tiles as tiles of `want` tokens would give
+        const uint32_t m_tiles = (M + want - 1) / want, tok = ((M + m_tiles - 1) / m_tiles + 15) & ~15u;
+        const double stage = kBlockM * kRowBytes + tok * kRowBytes, tiles = channels * m_tiles;
+        if (m_tiles > 65535 || tiles * 8 >= 2147483648.0) continue;
+        if (c->tune.token_tile > 0 && tok != ((uint32_t(c->tune.token_tile) + 15) & ~15u)) continue;
+        const double k_clocks = std::max(stage / 60, 2.0 * tok);
+        for (uint32_t ctas = 1; ctas <= 3; ++ctas) {
+            if (c->tune.token_ctas > 0 ? ctas != uint32_t(c->tune.token_ctas) : ctas == 3) continue;
+            if (gemm_tokens_stages(tok, ctas) < 3) continue;
+            for (uint32_t s = 1; s <= 8 && s <= kb; ++s) {
+                const uint32_t per = (kb + s - 1) / s;
+                if (per * (s - 1) >= kb) continue;   // no share may be empty
+                if (c->tune.token_split > 0 && s != uint32_t(c->tune.token_split)) continue;
+                if (s > 1 && layer_token_capacity(c, kind, tok, s, ctas) <= 0) continue;
+                const double on_sm = ceil(tiles * s / sms);   // CTAs of the busiest SM
+                const double epilogue = s == 1 ? 12.0 * tok : 1500 + 14.0 * tok + 14.0 * tok / s;
+                const double clocks = std::max(floor_clocks, on_sm * per * k_clocks) + ceil(on_sm / ctas) * (2500 + epilogue);
+                if (clocks < best.clocks) best = {false, tok, s, ctas, clocks};
+            }
+        }
+    }
+    return best;
+}
+
+// Few tokens or few tiles: the cluster kernel (gemm_tokens.cuh).
+int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, const ProductPlan& plan, TokenGemmParams& p) {
+    p.num_k_blocks = uint32_t((ox.inner + kRowBytes - 1) / kRowBytes);
+    p.tok = plan.tok;
+    p.splits = plan.splits;
+    p.ctas = plan.ctas;
+    p.idesc = kind == KIND_I8 ? make_instr_desc_i8(kBlockM, p.tok) : make_instr_desc(ow.hw_fmt, ox.hw_fmt, 0, 0, kBlockM, p.tok);
     p.status = c->d_status;
     TRY(encode_tiled(c, &p.tm_w, ow, kRowBytes, kBlockM));
     TRY(encode_tiled(c, &p.tm_x, ox, kRowBytes, p.tok));
@@ -554,7 +593,6 @@ int run_scaled_gemm(mmeb200_ctx* c, mmeb200_tensor* out, const mmeb200_tensor* x
     p.scaled.col_stride = num_elems(w_scale) == 1 ? 0 : 1;
     p.scaled.col_bias = tb ? tb->data : nullptr;
     p.scaled.bias_bf16 = tb && tb->dtype == DT_BF16;
-    p.scaled.col_vec = p.scaled.col_stride == 1 && reinterpret_cast<uintptr_t>(p.scaled.col_scale) % 16 == 0 && reinterpret_cast<uintptr_t>(p.scaled.col_bias) % 16 == 0;
     p.out = to->data; p.out_bf16 = to->dtype == DT_BF16; p.out_ld = to->strides[1];
     if (K == 0) {
         TRY(launch_status(c, launch_gemm_empty_sum(launch_env(c), p)));
@@ -570,11 +608,10 @@ int run_scaled_gemm(mmeb200_ctx* c, mmeb200_tensor* out, const mmeb200_tensor* x
         if (!x_fits) TRY(layer_pad_operand(c, &ox, static_cast<uint8_t*>(scratch)));
         if (!w_fits) TRY(layer_pad_operand(c, &ow, static_cast<uint8_t*>(scratch) + xb));
     }
-    const uint64_t pair_tiles = ((M + 255) / 256) * ((N + 255) / 256);
-    bool pair = M > 256 && N >= 256 && pair_tiles >= uint64_t(c->sm_count) / 4;
-    if (c->tune.pair >= 0) pair = c->tune.pair != 0 && M >= 256 && N >= 256;
-    if (pair) TRY(layer_pair_product(c, kind, ox, ow, p, to));
-    else TRY(layer_token_product(c, kind, ox, ow, ox.hw_fmt, ow.hw_fmt, p));
+    const ProductPlan plan = layer_plan(c, kind, p.M, p.N, uint32_t((K + kRowBytes - 1) / kRowBytes), p.out_bf16 ? 2 : 4);
+    if (plan.pair) TRY(layer_pair_product(c, kind, ox, ow, p, to));
+    else if (plan.tok) TRY(layer_token_product(c, kind, ox, ow, plan, p));
+    else return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");
     if (scratch) TRY(layer_scratch_used(c));
     return st.finish();
 }

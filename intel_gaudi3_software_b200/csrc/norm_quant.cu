@@ -19,8 +19,8 @@ cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec) {
 
 uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols) {
     const uint32_t per_block = cols <= 1024 ? 4 : 1;
-    // no more blocks than the SMs hold at once: a block walks its rows to the end
-    const uint32_t resident = std::max(1u, (cols <= 1024 ? 512u : 640u) / grad_threads(cols));
+    // as many blocks as the SMs hold at once (128 registers a thread): a block walks its rows to the end
+    const uint32_t resident = std::max(1u, 512u / grad_threads(cols));
     return std::min<uint32_t>((rows + per_block - 1) / per_block, uint32_t(sm_count) * resident);
 }
 
@@ -34,10 +34,10 @@ cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool
 }
 
 struct ColumnSums { const float* partial; float* out; uint32_t blocks, cols; };
-static __global__ void __launch_bounds__(256) column_sums_kernel(const __grid_constant__ ColumnSums p) { column_sums(p.partial, p.out, p.blocks, p.cols); }
+static __global__ void __launch_bounds__(1024) column_sums_kernel(const __grid_constant__ ColumnSums p) { column_sums(p.partial, p.out, p.blocks, p.cols); }
 cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols) {
     const ColumnSums p{partial, out, blocks, cols};
-    return launch_rows(env, column_sums_kernel, p, dim3((cols + 31) / 32), 256, 0);
+    return launch_rows(env, column_sums_kernel, p, dim3((cols + 31) / 32), 1024, 0);
 }
 
 cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, bool vec, int* launches) {

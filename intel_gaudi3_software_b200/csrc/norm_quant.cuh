@@ -99,15 +99,18 @@ struct RowIn<ROW_NONE, SHIFT> {
     __device__ __forceinline__ RowIn(const RowTensor&, uint64_t) {}
     __device__ __forceinline__ void load(Raw&, uint32_t) const {}
 };
+// The eight elements of a piece are worked on as four pairs: sm_100a adds and multiplies two floats per instruction, and the
+// row kernels are as near the issue rate as they are to HBM's.
 template <int TYPE, int W>
-__device__ __forceinline__ void unpack(const uint32_t (&w)[W], float (&f)[8]) {
+__device__ __forceinline__ void unpack(const uint32_t (&w)[W], float2 (&f)[4]) {
     static_assert(W == 2 * RowElem<TYPE>::kBytes, "packed words");
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        if constexpr (TYPE == ROW_F32) f[e] = __uint_as_float(w[e]);
-        else f[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16));
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == ROW_F32) f[i] = make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     }
 }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // A row that is written. A warp writes its run step by step (32 pieces each), in order, all lanes together (SHIFT).
 // `start`: its first step; `last`: no step follows whose first piece is full.
@@ -182,44 +185,54 @@ struct RowOut {
     }
 };
 
-// gamma is read by every row and sits in the caches; its type is a runtime value.
-__device__ __forceinline__ void load_gamma(float (&g)[8], const void* base, int type, bool whole, uint32_t at, int n) {
-    if (type == ROW_NONE) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) g[e] = 1.0f;
-    } else if (whole && n == 8) {
+// gamma is read by every row and sits in the caches; its type is a runtime value. SHIFT = false: it starts on 16 bytes.
+template <bool SHIFT>
+__device__ __forceinline__ void load_gamma(float2 (&g)[4], const void* base, int type, bool whole, uint32_t at, int n) {
+    if (!SHIFT || (whole && n == 8)) {
         if (type == ROW_BF16) {
             const uint4 q = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
             const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e) g[e] = __uint_as_float((e & 1) ? (w[e >> 1] & 0xFFFF0000u) : (w[e >> 1] << 16));
+            unpack<ROW_BF16>(w, g);
         } else {
             const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
             const float4 a = __ldg(q), b = __ldg(q + 1);
-            g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
-            g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+            g[0] = make_float2(a.x, a.y); g[1] = make_float2(a.z, a.w);
+            g[2] = make_float2(b.x, b.y); g[3] = make_float2(b.z, b.w);
         }
     } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            g[e] = 1.0f;
-            if (e < n) g[e] = type == ROW_BF16 ? __uint_as_float(uint32_t(static_cast<const uint16_t*>(base)[at + e]) << 16) : static_cast<const float*>(base)[at + e];
+            float t = 1.0f;
+            if (e < n) t = type == ROW_BF16 ? __uint_as_float(uint32_t(static_cast<const uint16_t*>(base)[at + e]) << 16) : static_cast<const float*>(base)[at + e];
+            if (e & 1) g[e >> 1].y = t;
+            else g[e >> 1].x = t;
         }
     }
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+__device__ __forceinline__ uint32_t pack_bf16(float2 v) {
     uint32_t w;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(hi), "f"(lo));
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(v.y), "f"(v.x));
     return w;
 }
-__device__ __forceinline__ void pack_bf16x8(const float (&f)[8], uint32_t (&w)[4]) {
+// Eight floats, packed as the type keeps them.
+template <int TYPE, int W>
+__device__ __forceinline__ void pack(const float2 (&f)[4], uint32_t (&w)[W]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == ROW_F32) { w[2 * i] = __float_as_uint(f[i].x); w[2 * i + 1] = __float_as_uint(f[i].y); }
+        else w[i] = pack_bf16(f[i]);
+    }
 }
+
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -271,35 +284,43 @@ static __device__ __noinline__ uint32_t codes_by_division(float v0, float v1, fl
 //   fp8:  where product * (1 - 2^-22) and product * (1 + 2^-22) have the same code, it is the quotient's (the cast is monotone).
 // The few quads with an element that fails its test are divided. GIVEN: the step is the caller's, quotients may be anything.
 template <bool I8, bool GIVEN>
-__device__ __forceinline__ uint32_t make_codes(float v0, float v1, float v2, float v3, const CodeStep& s, const Fp8HwCast& hw) {
+__device__ __forceinline__ uint32_t make_codes(float2 v0, float2 v1, const CodeStep& s, const Fp8HwCast& hw) {
     if (s.recip == 0.0f) return 0u;
-    float x[4] = {v0, v1, v2, v3};
+    float2 x[2] = {v0, v1};
     uint32_t w;
     bool sure;
     if constexpr (I8) {
-        float m[4], worst = 0.0f;
+        float2 m[2];
+        float worst = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (GIVEN) x[e] = x[e] == x[e] ? x[e] : 0.0f;   // a NaN has no code (rows with one have no step of their own)
-            float t = x[e] * s.recip;
-            if constexpr (GIVEN) t = fminf(fmaxf(t, -127.0f), 127.0f);
-            m[e] = t + kRoundMagic;
-            worst = fmaxf(worst, fabsf(t - (m[e] - kRoundMagic)));
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (GIVEN) {   // a NaN has no code (rows with one have no step of their own)
+                x[i].x = x[i].x == x[i].x ? x[i].x : 0.0f;
+                x[i].y = x[i].y == x[i].y ? x[i].y : 0.0f;
+            }
+            float2 t = __fmul2_rn(x[i], both(s.recip));
+            if constexpr (GIVEN) {
+                t.x = fminf(fmaxf(t.x, -127.0f), 127.0f);
+                t.y = fminf(fmaxf(t.y, -127.0f), 127.0f);
+            }
+            m[i] = __fadd2_rn(t, both(kRoundMagic));
+            const float2 back = __fadd2_rn(m[i], both(-kRoundMagic)), off = __ffma2_rn(back, both(-1.0f), t);
+            worst = fmaxf(worst, fmaxf(fabsf(off.x), fabsf(off.y)));
         }
         sure = worst <= 0.5f - 0x1p-15f && s.recip == s.recip;
-        w = pack_low_bytes(m[0], m[1], m[2], m[3]);
+        w = pack_low_bytes(m[0].x, m[0].y, m[1].x, m[1].y);
     } else {
         float lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float t = x[e] * s.recip;
-            lo[e] = t * (1.0f - 0x1p-22f);
-            hi[e] = t * (1.0f + 0x1p-22f);
+        for (int i = 0; i < 2; ++i) {
+            const float2 t = __fmul2_rn(x[i], both(s.recip)), l = __fmul2_rn(t, both(1.0f - 0x1p-22f)), h = __fmul2_rn(t, both(1.0f + 0x1p-22f));
+            lo[2 * i] = l.x; lo[2 * i + 1] = l.y;
+            hi[2 * i] = h.x; hi[2 * i + 1] = h.y;
         }
         w = f32x4_to_fp8_hw(lo, hw);
         sure = w == f32x4_to_fp8_hw(hi, hw) && s.recip == s.recip;
     }
-    if (!sure) w = codes_by_division<I8>(x[0], x[1], x[2], x[3], s.step, hw);
+    if (!sure) w = codes_by_division<I8>(x[0].x, x[0].y, x[1].x, x[1].y, s.step, hw);
     return w;
 }
 
@@ -353,7 +374,7 @@ template <int XT, int RT>
 struct RowKept {
     static constexpr int kType = RT != ROW_NONE ? RT : XT, kWords = 2 * RowElem<kType>::kBytes;
     uint32_t w[kWords];
-    __device__ __forceinline__ void values(float (&h)[8]) const { unpack<kType>(w, h); }
+    __device__ __forceinline__ void values(float2 (&h)[4]) const { unpack<kType>(w, h); }
 };
 // x + residual, rounded to the stream's type, which is what the norm sees.
 template <int XT, int RT, bool SHIFT>
@@ -367,16 +388,12 @@ __device__ __forceinline__ void stream_piece(const RowIn<XT, SHIFT>& xin, const 
     } else {
         uint32_t rw[RowIn<RT, SHIFT>::kWords];
         rin.words(r, rw);
-        float f[8], g[8];
+        float2 f[4], g[4];
         unpack<XT>(xw, f);
         unpack<RT>(rw, g);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += g[e];
-        if constexpr (RT == ROW_BF16) pack_bf16x8(f, h.w);
-        else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h.w[e] = __float_as_uint(f[e]);
-        }
+        for (int i = 0; i < 4; ++i) f[i] = __fadd2_rn(f[i], g[i]);
+        pack<RT>(f, h.w);
     }
 }
 // A row's last piece may be partial: its missing elements count as zeros.
@@ -390,71 +407,69 @@ __device__ __forceinline__ void clear_missing(RowKept<XT, RT>& h, int n) {
         }
 }
 // Adds a piece to its row's sums.
-template <bool TOPS, int XT, int RT>
-__device__ __forceinline__ void sum_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float& sum, float& top) {
-    float h[8];
+template <bool TOPS, bool SHIFT, int XT, int RT>
+__device__ __forceinline__ void sum_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float2& sum, float& top) {
+    float2 h[4];
     kept.values(h);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = fmaf(h[e], h[e], sum);
+    for (int i = 0; i < 4; ++i) sum = __ffma2_rn(h[i], h[i], sum);
     if constexpr (TOPS) {
         if (p.gamma_type != ROW_NONE) {
-            float g[8];
-            load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
+            float2 g[4];
+            load_gamma<SHIFT>(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] *= g[e];
+            for (int i = 0; i < 4; ++i) h[i] = __fmul2_rn(h[i], g[i]);
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max_nan(top, fabsf(h[e]));
+        for (int i = 0; i < 4; ++i) top = max_nan(top, fabsf(h[i].x), fabsf(h[i].y));
     }
 }
 // v = h * gamma of a piece.
-template <int XT, int RT>
-__device__ __forceinline__ void scaled_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float (&v)[8]) {
+template <bool SHIFT, int XT, int RT>
+__device__ __forceinline__ void scaled_piece(const NormParams& p, const RowKept<XT, RT>& kept, uint32_t c, int n, float2 (&v)[4]) {
     kept.values(v);
     if (p.gamma_type != ROW_NONE && n) {
-        float g[8];
-        load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
+        float2 g[4];
+        load_gamma<SHIFT>(g, p.gamma, p.gamma_type, p.gamma_whole, c, n);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= g[e];
+        for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(v[i], g[i]);
     }
 }
 
 // The warp's run of pieces: piece i of a lane starts at column c0 + 256 i.
+template <bool SHIFT>
 struct WarpRun {
     uint32_t c0, cols;
     __device__ __forceinline__ uint32_t col(uint32_t i) const { return c0 + 256 * i + (threadIdx.x & 31) * 8; }
     __device__ __forceinline__ bool any(uint32_t i) const { return c0 + 256 * i < cols; }
     __device__ __forceinline__ bool whole(uint32_t i) const { return c0 + 256 * i + 256 <= cols; }
-    __device__ __forceinline__ int size(uint32_t i) const { return piece_size(col(i), cols); }
+    __device__ __forceinline__ int size(uint32_t i) const { return SHIFT ? piece_size(col(i), cols) : col(i) < cols ? 8 : 0; }
     // step i is the last of `steps` that hands nothing on to a full piece
     __device__ __forceinline__ bool last(uint32_t i, uint32_t steps) const { return i + 1 == steps || c0 + 256 * (i + 1) + 8 > cols; }
 };
 
 // The second pass over a row: `piece(i, n, v)` gives the values h * gamma of piece i.
 template <int MODE, bool SHIFT, int UNROLL, typename F>
-__device__ __forceinline__ void write_row(const NormParams& p, uint64_t at, const WarpRun& run, uint32_t pieces, const RowFactors& f, F&& piece) {
+__device__ __forceinline__ void write_row(const NormParams& p, uint64_t at, const WarpRun<SHIFT>& run, uint32_t pieces, const RowFactors& f, F&& piece) {
     constexpr int kType = MODE == NORM_BF16 ? ROW_BF16 : MODE == NORM_F32 ? ROW_F32 : ROW_I8;
     RowOut<kType, SHIFT> out(p.out, at);
 #pragma unroll UNROLL
     for (uint32_t i = 0; i < pieces; ++i) {
         const int n = run.size(i);
         if (SHIFT ? run.any(i) : n != 0) {
-            float v[8];
+            float2 v[4];
             uint32_t w[RowOut<kType, SHIFT>::kWords];
             piece(i, n, v);
             if constexpr (MODE == NORM_I8 || MODE == NORM_F8) {
 #pragma unroll
-                for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8, false>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], f.step, p.hw);
+                for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8, false>(v[2 * q], v[2 * q + 1], f.step, p.hw);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] *= f.inv;
-                if constexpr (MODE == NORM_BF16) pack_bf16x8(v, w);
-                else if constexpr (MODE == NORM_F32) {
+                for (int k = 0; k < 4; ++k) v[k] = __fmul2_rn(v[k], both(f.inv));
+                if constexpr (MODE == NORM_BF16 || MODE == NORM_F32) pack<kType>(v, w);
+                else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(v[e]);
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8_GIVEN, true>(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3], f.step, p.hw);
+                    for (int q = 0; q < 2; ++q) w[q] = make_codes<MODE == NORM_I8_GIVEN, true>(v[2 * q], v[2 * q + 1], f.step, p.hw);
                 }
             }
             out.store(run.col(i), n, w, run.whole(i), i == 0, run.last(i, pieces));
@@ -463,7 +478,7 @@ __device__ __forceinline__ void write_row(const NormParams& p, uint64_t at, cons
 }
 // What differs between the kinds of output is decided once per row, not once per piece.
 template <bool SHIFT, int UNROLL, typename F>
-__device__ __forceinline__ void write_row_any(const NormParams& p, uint64_t at, const WarpRun& run, uint32_t pieces, const RowFactors& f, F&& piece) {
+__device__ __forceinline__ void write_row_any(const NormParams& p, uint64_t at, const WarpRun<SHIFT>& run, uint32_t pieces, const RowFactors& f, F&& piece) {
     switch (p.mode) {
         case NORM_BF16: write_row<NORM_BF16, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
         case NORM_F32: write_row<NORM_F32, SHIFT, UNROLL>(p, at, run, pieces, f, piece); break;
@@ -476,12 +491,13 @@ __device__ __forceinline__ void write_row_any(const NormParams& p, uint64_t at, 
 
 // The first pass: reads x and the residual, writes the stream, takes the sums. NV pieces per lane, loads G pieces at a time.
 template <bool TOPS, int XT, int RT, bool SHIFT, int NV>
-__device__ __forceinline__ float2 read_row(const NormParams& p, uint32_t row, const WarpRun& run, RowKept<XT, RT> (&kept)[NV]) {
-    constexpr int G = NV < 2 ? 1 : 2, KT = RowKept<XT, RT>::kType;
+__device__ __forceinline__ float2 read_row(const NormParams& p, uint32_t row, const WarpRun<SHIFT>& run, RowKept<XT, RT> (&kept)[NV]) {
+    constexpr int G = NV < 2 ? 1 : (!SHIFT && XT != ROW_F32 && RT != ROW_F32) ? 4 : 2, KT = RowKept<XT, RT>::kType;
     const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat));
     const RowIn<RT, SHIFT> rin(p.residual, RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0);
     RowOut<KT, SHIFT> sout(p.sum, RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0);
-    float sum = 0.0f, top = 0.0f;
+    float2 sum = both(0.0f);
+    float top = 0.0f;
 #pragma unroll
     for (int i0 = 0; i0 < NV; i0 += G) {
         typename RowIn<XT, SHIFT>::Raw x[G];
@@ -499,33 +515,33 @@ __device__ __forceinline__ float2 read_row(const NormParams& p, uint32_t row, co
             if (n) {
                 stream_piece<XT, RT, SHIFT>(xin, x[j], rin, r[j], kept[i]);
                 if (SHIFT && n < 8) clear_missing(kept[i], n);
-                sum_piece<TOPS>(p, kept[i], run.col(i), n, sum, top);
+                sum_piece<TOPS, SHIFT>(p, kept[i], run.col(i), n, sum, top);
             }
             if constexpr (RT != ROW_NONE) {
                 if (p.sum.ptr && (SHIFT ? run.any(i) : n != 0)) sout.store(run.col(i), n, kept[i].w, run.whole(i), i == 0, run.last(i, NV));
             }
         }
     }
-    return make_float2(sum, top);
+    return make_float2(sum.x + sum.y, top);
 }
 
 // A row per warp (BLOCK = false: four rows per block) or per block, NV pieces per lane, kept in registers between the row's
 // one read and its one write.
 template <int XT, int RT, bool SHIFT, int NV, bool BLOCK, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(THREADS, THREADS == 512 && RowKept<XT, RT>::kType == ROW_BF16 && !(SHIFT && NV == 8) ? 2 : 1) norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ float2 scratch[32];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= p.rows) return;   // whole warps, never part of a block that synchronises
-    const WarpRun run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
+    const WarpRun<SHIFT> run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
     RowKept<XT, RT> kept[NV];
     float2 s = (p.mode == NORM_I8 || p.mode == NORM_F8) ? read_row<true, XT, RT, SHIFT, NV>(p, row, run, kept) : read_row<false, XT, RT, SHIFT, NV>(p, row, run, kept);
     s = reduce_row<BLOCK, true>(s.x, s.y, blockDim.x >> 5, scratch);
     const RowFactors f = row_factors(p, s.x, s.y, row);
     if (p.scale && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) p.scale[row] = f.scale;
     write_row_any<SHIFT, NV>(p, row_offset(p.out, row, p.dims, p.flat), run, NV, f,
-                         [&](uint32_t i, int n, float (&v)[8]) { scaled_piece(p, kept[i], run.col(i), n, v); });
+                         [&](uint32_t i, int n, float2 (&v)[4]) { scaled_piece<SHIFT>(p, kept[i], run.col(i), n, v); });
 }
 
 // Rows too long for registers: the row is read a second time (from L2, mostly) once its sums are known. The second read
@@ -538,12 +554,13 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t row = blockIdx.x, pieces = (p.cols + 32 * 256 - 1) / (32 * 256);   // per lane
-    const WarpRun run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
+    const WarpRun<SHIFT> run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
     const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat));
     const RowIn<RT, SHIFT> rin(p.residual, RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0);
     const uint64_t so = RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0;
     const bool tops = p.mode == NORM_I8 || p.mode == NORM_F8, has_sum = RT != ROW_NONE && p.sum.ptr != nullptr;
-    float sum = 0.0f, top = 0.0f;
+    float2 sum = both(0.0f);
+    float top = 0.0f;
     {
         RowOut<KT, SHIFT> sout(p.sum, so);
 #pragma unroll 1
@@ -557,20 +574,20 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
                 rin.load(r, run.col(i));
                 stream_piece<XT, RT, SHIFT>(xin, x, rin, r, kept);
                 if (SHIFT && n < 8) clear_missing(kept, n);
-                if (tops) sum_piece<true>(p, kept, run.col(i), n, sum, top);
-                else sum_piece<false>(p, kept, run.col(i), n, sum, top);
+                if (tops) sum_piece<true, SHIFT>(p, kept, run.col(i), n, sum, top);
+                else sum_piece<false, SHIFT>(p, kept, run.col(i), n, sum, top);
             }
             if constexpr (RT != ROW_NONE) {
                 if (has_sum && (SHIFT || n)) sout.store(run.col(i), n, kept.w, run.whole(i), i == 0, run.last(i, pieces));
             }
         }
     }
-    const float2 s = reduce_row<true, true>(sum, top, 32, scratch);   // its barrier also orders the stores of `sum` and the reads below
+    const float2 s = reduce_row<true, true>(sum.x + sum.y, top, 32, scratch);   // its barrier also orders the stores of `sum` and the reads below
     const RowFactors f = row_factors(p, s.x, s.y, row);
     if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
     const RowIn<KT, SHIFT> again(p.sum, so);
     const uint64_t oo = row_offset(p.out, row, p.dims, p.flat);
-    write_row_any<SHIFT, 1>(p, oo, run, pieces, f, [&](uint32_t i, int n, float (&v)[8]) {
+    write_row_any<SHIFT, 1>(p, oo, run, pieces, f, [&](uint32_t i, int n, float2 (&v)[4]) {
         RowKept<XT, RT> kept;
 #pragma unroll
         for (int k = 0; k < RowKept<XT, RT>::kWords; ++k) kept.w[k] = 0;
@@ -587,7 +604,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
                 stream_piece<XT, RT, SHIFT>(xin, x, rin, r, kept);
             }
         }
-        scaled_piece(p, kept, run.col(i), n, v);
+        scaled_piece<SHIFT>(p, kept, run.col(i), n, v);
     });
 }
 
@@ -596,21 +613,39 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
 // mean(a * u) = inv * mean(a * x), so both sums of a row (x^2 and a * x) are taken in one pass. A block walks rows b, b +
 // blocks, ...; every thread keeps the sums of its own columns of dgamma, and the block's partial sums (one row of `partial`)
 // are added in a fixed order by column_sums: results do not depend on timing.
+__device__ __forceinline__ void clear_missing(float2 (&x)[4], float2 (&y)[4], int n) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (2 * k >= n) x[k].x = y[k].x = 0.0f;
+        if (2 * k + 1 >= n) x[k].y = y[k].y = 0.0f;
+    }
+}
+// a (dy * gamma) becomes dx; acc += dy * u.
+template <bool DSUM>
+__device__ __forceinline__ void grad_piece(const float2 (&x)[4], const float2 (&y)[4], float2 (&a)[4], const float2 (&add)[4], float inv, float mean_au, float2 (&acc)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 u = __fmul2_rn(x[k], both(inv)), t = __ffma2_rn(u, both(-mean_au), a[k]);
+        if constexpr (DSUM) a[k] = __ffma2_rn(t, both(inv), add[k]);
+        else a[k] = __fmul2_rn(t, both(inv));
+        acc[k] = __ffma2_rn(y[k], u, acc[k]);
+    }
+}
 // XT: type of x, dy, dsum and dx; DSUM: whether there is a gradient of the sum. A row per warp or per block, as in norm_kernel.
 template <int XT, bool DSUM, bool SHIFT, int NV, bool BLOCK, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
     constexpr int kRowsPerBlock = BLOCK ? 1 : 4, ST = DSUM ? XT : ROW_NONE, W = 2 * RowElem<XT>::kBytes;
     __shared__ float2 scratch[2][32];
     extern __shared__ float block_sums[];   // a row per warp: [cols], the four warps' sums of dgamma
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t sub = BLOCK ? 0 : (threadIdx.x >> 5);
-    const WarpRun run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
-    float acc[NV][8];
+    const WarpRun<SHIFT> run{BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0u, p.cols};
+    float2 acc[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[i][e] = 0.0f;
+        for (int k = 0; k < 4; ++k) acc[i][k] = both(0.0f);
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x * kRowsPerBlock + sub; row < p.rows; row += gridDim.x * kRowsPerBlock, turn ^= 1) {
         const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat)), yin(p.dy, row_offset(p.dy, row, p.dims, p.flat));
@@ -633,59 +668,58 @@ __global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constan
                     yin.words(yr[i], ys[i]);
                 }
         }
-        float squares = 0.0f, dot = 0.0f;
+        float2 squares = both(0.0f), dot = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int n = run.size(i);
             if (n) {
-                float g[8], x[8], y[8];
-                load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+                float2 g[4], x[4], y[4];
                 unpack<XT>(xs[i], x);
                 unpack<XT>(ys[i], y);
+                if (SHIFT && n < 8) clear_missing(x, y, n);
+                if (p.gamma_type != ROW_NONE) {
+                    load_gamma<SHIFT>(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (SHIFT && e >= n) x[e] = y[e] = 0.0f;
-                    squares = fmaf(x[e], x[e], squares);
-                    dot = fmaf(y[e] * g[e], x[e], dot);
+                    for (int k = 0; k < 4; ++k) y[k] = __fmul2_rn(y[k], g[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    squares = __ffma2_rn(x[k], x[k], squares);
+                    dot = __ffma2_rn(y[k], x[k], dot);
                 }
             }
         }
-        const float2 s = reduce_row<BLOCK, false>(squares, dot, blockDim.x >> 5, scratch[turn]);   // two buffers: the next row's sums may start before all have read
+        // two buffers: the next row's sums may start before all have read
+        const float2 s = reduce_row<BLOCK, false>(squares.x + squares.y, dot.x + dot.y, blockDim.x >> 5, scratch[turn]);
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
-        auto write = [&](auto& out) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int n = run.size(i);
-                if (SHIFT ? run.any(i) : n != 0) {
-                    float d[8], x[8], y[8], g[8];
-                    unpack<XT>(xs[i], x);
-                    unpack<XT>(ys[i], y);
-                    load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
-                    float sv[8];
-                    if constexpr (DSUM) {
-                        uint32_t sw[W];
-                        sin.words(ds[i], sw);
-                        unpack<XT>(sw, sv);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float u = x[e] * inv, t = fmaf(-u, mean_au, y[e] * g[e]);
-                        d[e] = DSUM ? fmaf(t, inv, sv[e]) : t * inv;
-                        acc[i][e] = fmaf(y[e], u, acc[i][e]);   // of missing elements: never read
-                    }
-                    uint32_t w[W];
-                    if constexpr (XT == ROW_BF16) pack_bf16x8(d, w);
-                    else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(d[e]);
-                    }
-                    out.store(run.col(i), n, w, run.whole(i), i == 0, run.last(i, NV));
-                }
-            }
-        };
         RowOut<XT, SHIFT> out(p.dx, row_offset(p.dx, row, p.dims, p.flat));
-        write(out);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int n = run.size(i);
+            if (SHIFT ? run.any(i) : n != 0) {
+                float2 x[4], y[4], a[4], add[4];
+                unpack<XT>(xs[i], x);
+                unpack<XT>(ys[i], y);
+                if constexpr (DSUM) {
+                    uint32_t sw[W];
+                    sin.words(ds[i], sw);
+                    unpack<XT>(sw, add);
+                }
+                if (p.gamma_type != ROW_NONE) {
+                    load_gamma<SHIFT>(a, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[k] = __fmul2_rn(a[k], y[k]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[k] = y[k];
+                }
+                grad_piece<DSUM>(x, y, a, add, inv, mean_au, acc[i]);   // the sums of missing elements are never read
+                uint32_t w[W];
+                pack<XT>(a, w);
+                out.store(run.col(i), n, w, run.whole(i), i == 0, run.last(i, NV));
+            }
+        }
     }
     if (!p.partial) return;
     float* mine = p.partial + uint64_t(blockIdx.x) * p.cols;
@@ -697,7 +731,8 @@ __global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constan
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const uint32_t c = run.col(i) + e;
-                        if (c < p.cols) block_sums[c] = w ? block_sums[c] + acc[i][e] : acc[i][e];
+                        const float mine_c = (e & 1) ? acc[i][e >> 1].y : acc[i][e >> 1].x;
+                        if (c < p.cols) block_sums[c] = w ? block_sums[c] + mine_c : mine_c;
                     }
             }
             __syncthreads();
@@ -708,12 +743,12 @@ __global__ void __launch_bounds__(THREADS) norm_grad_kernel(const __grid_constan
         for (int i = 0; i < NV; ++i) {
             const uint32_t c = run.col(i);
             if (!SHIFT && c < p.cols) {   // cols is a multiple of eight, and a block's row of `partial` starts on 16 bytes
-                reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
-                reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[i][4], acc[i][5], acc[i][6], acc[i][7]);
+                reinterpret_cast<float4*>(mine + c)[0] = make_float4(acc[i][0].x, acc[i][0].y, acc[i][1].x, acc[i][1].y);
+                reinterpret_cast<float4*>(mine + c)[1] = make_float4(acc[i][2].x, acc[i][2].y, acc[i][3].x, acc[i][3].y);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (c + e < p.cols) mine[c + e] = acc[i][e];
+                    if (c + e < p.cols) mine[c + e] = (e & 1) ? acc[i][e >> 1].y : acc[i][e >> 1].x;
             }
         }
     }
@@ -727,41 +762,43 @@ __global__ void __launch_bounds__(1024) norm_grad_long_kernel(const __grid_const
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t pieces = (p.cols + 32 * 256 - 1) / (32 * 256);
-    const WarpRun run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
+    const WarpRun<SHIFT> run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
     float* mine = p.partial ? p.partial + uint64_t(blockIdx.x) * p.cols : nullptr;
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
         const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat)), yin(p.dy, row_offset(p.dy, row, p.dims, p.flat));
         const RowIn<ST, SHIFT> sin(p.dsum, DSUM ? row_offset(p.dsum, row, p.dims, p.flat) : 0);
-        auto read = [&](uint32_t i, int n, float (&x)[8], float (&y)[8], float (&g)[8]) {
+        auto read = [&](uint32_t i, int n, float2 (&x)[4], float2 (&y)[4], float2 (&a)[4]) {
             typename RowIn<XT, SHIFT>::Raw xr, yr;
             uint32_t xw[W], yw[W];
             xin.load(xr, run.col(i));
             yin.load(yr, run.col(i));
-            load_gamma(g, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = both(1.0f);
+            if (p.gamma_type != ROW_NONE) load_gamma<SHIFT>(a, p.gamma, p.gamma_type, p.gamma_whole, run.col(i), n);
             xin.words(xr, xw);
             yin.words(yr, yw);
             unpack<XT>(xw, x);
             unpack<XT>(yw, y);
+            if (SHIFT && n < 8) clear_missing(x, y, n);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (SHIFT && e >= n) x[e] = y[e] = 0.0f;
+            for (int k = 0; k < 4; ++k) a[k] = __fmul2_rn(a[k], y[k]);
         };
-        float squares = 0.0f, dot = 0.0f;
+        float2 squares = both(0.0f), dot = both(0.0f);
 #pragma unroll 1
         for (uint32_t i = 0; i < pieces && run.any(i); ++i) {
             const int n = run.size(i);
             if (n) {
-                float x[8], y[8], g[8];
-                read(i, n, x, y, g);
+                float2 x[4], y[4], a[4];
+                read(i, n, x, y, a);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    squares = fmaf(x[e], x[e], squares);
-                    dot = fmaf(y[e] * g[e], x[e], dot);
+                for (int k = 0; k < 4; ++k) {
+                    squares = __ffma2_rn(x[k], x[k], squares);
+                    dot = __ffma2_rn(a[k], x[k], dot);
                 }
             }
         }
-        const float2 s = reduce_row<true, false>(squares, dot, 32, scratch[turn]);
+        const float2 s = reduce_row<true, false>(squares.x + squares.y, dot.x + dot.y, 32, scratch[turn]);
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
         const bool first = row == blockIdx.x;
@@ -774,47 +811,50 @@ __global__ void __launch_bounds__(1024) norm_grad_long_kernel(const __grid_const
 #pragma unroll
             for (int k = 0; k < W; ++k) w[k] = 0;
             if (n) {
-                float x[8], y[8], g[8], d[8], sv[8];
-                read(i, n, x, y, g);
+                float2 x[4], y[4], a[4], add[4], acc[4];
+                read(i, n, x, y, a);
                 if constexpr (DSUM) {
                     typename RowIn<ST, SHIFT>::Raw sr;
                     uint32_t sw[W];
                     sin.load(sr, c);
                     sin.words(sr, sw);
-                    unpack<XT>(sw, sv);
+                    unpack<XT>(sw, add);
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = x[e] * inv, t = fmaf(-u, mean_au, y[e] * g[e]);
-                    d[e] = DSUM ? fmaf(t, inv, sv[e]) : t * inv;
-                    if (mine && e < n) mine[c + e] = first ? y[e] * u : fmaf(y[e], u, mine[c + e]);
-                }
-                if constexpr (XT == ROW_BF16) pack_bf16x8(d, w);
-                else {
+                for (int k = 0; k < 4; ++k) acc[k] = both(0.0f);
+                if (mine && !first) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) w[e] = __float_as_uint(d[e]);
+                    for (int e = 0; e < 8; ++e)
+                        if (e < n) ((e & 1) ? acc[e >> 1].y : acc[e >> 1].x) = mine[c + e];
                 }
+                grad_piece<DSUM>(x, y, a, add, inv, mean_au, acc);
+                if (mine) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < n) mine[c + e] = (e & 1) ? acc[e >> 1].y : acc[e >> 1].x;
+                }
+                pack<XT>(a, w);
             }
             if (SHIFT || n) out.store(c, n, w, run.whole(i), i == 0, run.last(i, pieces));
         }
     }
 }
-// out[c] = sum over blocks, in block order within each of eight interleaved shares, then share by share: a fixed order.
+// out[c] = sum over blocks: 32 interleaved shares, each in block order, then share by share: a fixed order.
 __device__ __forceinline__ void column_sums(const float* partial, float* out, uint32_t blocks, uint32_t cols) {
-    __shared__ float part[8][33];
+    __shared__ float part[32][33];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t lane = threadIdx.x & 31, share = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (c < cols) {
-#pragma unroll 4
-        for (uint32_t b = share; b < blocks; b += 8) s += partial[uint64_t(b) * cols + c];
+#pragma unroll 8
+        for (uint32_t b = share; b < blocks; b += 32) s += partial[uint64_t(b) * cols + c];
     }
     part[share][lane] = s;
     __syncthreads();
     if (share == 0 && c < cols) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) s += part[i][lane];
+        for (int i = 1; i < 32; ++i) s += part[i][lane];
         out[c] = s;
     }
 }
@@ -824,7 +864,7 @@ __device__ __forceinline__ void column_sums(const float* partial, float* out, ui
 // is above infinity's, so it stays), then the codes through a tile in shared memory, then the steps in place of the maxima.
 // x is read twice; the second pass walks the rows from the end, so that it begins with what the first left in L2.
 template <int XT, bool SHIFT>
-__device__ __forceinline__ void column_values(const QuantTransParams& p, uint32_t row, const typename RowIn<XT, SHIFT>::Raw& x, float (&v)[8]) {
+__device__ __forceinline__ void column_values(const QuantTransParams& p, uint32_t row, const typename RowIn<XT, SHIFT>::Raw& x, float2 (&v)[4]) {
     const RowIn<XT, SHIFT> in(p.x, uint64_t(row) * p.x_ld);
     uint32_t w[RowIn<XT, SHIFT>::kWords];
     in.words(x, w);
@@ -838,9 +878,9 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 256 + lane * 8;
     const int n = piece_size(c, p.cols);
     const uint32_t rows_per = (p.rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * rows_per, r1 = min(p.rows, r0 + rows_per);
-    float top[8];
+    float2 top[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top[e] = 0.0f;
+    for (int k = 0; k < 4; ++k) top[k] = both(0.0f);
     if (n) {
 #pragma unroll 1
         for (uint32_t r = r0 + warp; r < r1; r += 32) {
@@ -851,15 +891,16 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
 #pragma unroll
             for (int j = 0; j < 4; ++j)
                 if (r + 8 * j < r1) {
-                    float v[8];
+                    float2 v[4];
                     column_values<XT, SHIFT>(p, r + 8 * j, x[j], v);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) top[e] = max_nan(top[e], fabsf(v[e]));   // of missing columns: never read
+                    for (int k = 0; k < 4; ++k)   // of missing columns: never read
+                        top[k] = make_float2(max_nan(top[k].x, fabsf(v[k].x)), max_nan(top[k].y, fabsf(v[k].y)));
                 }
         }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[warp][e * 32 + lane] = top[e];
+    for (int e = 0; e < 8; ++e) part[warp][e * 32 + lane] = (e & 1) ? top[e >> 1].y : top[e >> 1].x;
     __syncthreads();
     const uint32_t mine = blockIdx.x * 256 + (threadIdx.x & 31) * 8 + (threadIdx.x >> 5);
     float t = part[0][threadIdx.x];
@@ -892,7 +933,7 @@ __global__ void __launch_bounds__(256) quant_trans_kernel(const __grid_constant_
         if (r0 >= p.rows) continue;   // uniform over the block
         const uint32_t r = r0 + rq * 4;
         typename RowIn<XT, SHIFT>::Raw x[4];
-        float v[4][8];
+        float2 v[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (exists && r + j < p.rows) RowIn<XT, SHIFT>(p.x, uint64_t(p.row0 + r + j) * p.x_ld).load(x[j], cc);
@@ -902,11 +943,15 @@ __global__ void __launch_bounds__(256) quant_trans_kernel(const __grid_constant_
             if (exists && r + j < p.rows) column_values<XT, SHIFT>(p, p.row0 + r + j, x[j], v[j]);
             else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = 0.0f;
+                for (int k = 0; k < 4; ++k) v[j][k] = both(0.0f);
             }
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) tile[(cg * 8 + e) * kPitch + rq] = make_codes<I8, GIVEN>(v[0][e], v[1][e], v[2][e], v[3][e], steps[cg * 8 + e], p.hw);
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t c = cg * 8 + 2 * k;
+            tile[c * kPitch + rq] = make_codes<I8, GIVEN>(make_float2(v[0][k].x, v[1][k].x), make_float2(v[2][k].x, v[3][k].x), steps[c], p.hw);
+            tile[(c + 1) * kPitch + rq] = make_codes<I8, GIVEN>(make_float2(v[0][k].y, v[1][k].y), make_float2(v[2][k].y, v[3][k].y), steps[c + 1], p.hw);
+        }
         __syncthreads();
         const uint32_t rows = min(128u, p.rows - r0), cols = min(64u, p.cols - c0);
         // nine 16-byte words cover a column's 128 bytes at any alignment

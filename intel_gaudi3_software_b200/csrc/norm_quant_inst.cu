@@ -33,7 +33,7 @@ cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& p, uint32_t
     const size_t sums = p.cols <= 1024 ? p.cols * sizeof(float) : 0;
     if (p.cols <= 256) return launch_rows(env, norm_grad_kernel<XT, DSUM, SHIFT, 1, false, 128>, p, g, threads, sums);
     if (p.cols <= 1024) return launch_rows(env, norm_grad_kernel<XT, DSUM, SHIFT, 4, false, 128>, p, g, threads, sums);
-    if (p.cols <= 8192) return launch_rows(env, norm_grad_kernel<XT, DSUM, SHIFT, 2, true, 512>, p, g, threads, 0);
+    if (p.cols <= 8192) return launch_rows(env, norm_grad_kernel<XT, DSUM, SHIFT, 4, true, 256>, p, g, threads, 0);
     return launch_rows(env, norm_grad_long_kernel<XT, DSUM, SHIFT>, p, g, threads, 0);
 }
 template cudaError_t norm_grad_of<INST_XT, INST_GRAD != 0, INST_SHIFT != 0>(const RowLaunch&, const NormGradParams&, uint32_t);

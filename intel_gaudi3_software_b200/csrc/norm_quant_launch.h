@@ -25,7 +25,7 @@ inline cudaError_t launch_rows(const RowLaunch& env, void (*kern)(P), const P& p
 }
 
 // Threads of a gradient block that works on one row at a time; rows of up to 1024 columns take a warp each, four to a block.
-inline uint32_t grad_threads(uint32_t cols) { return cols <= 1024 ? 128 : cols <= 8192 ? 32 * ((cols + 511) / 512) : 1024; }
+inline uint32_t grad_threads(uint32_t cols) { return cols <= 1024 ? 128 : cols <= 8192 ? 32 * ((cols + 1023) / 1024) : 1024; }
 
 template <int XT, int RT, bool SHIFT>
 cudaError_t norm_of(const RowLaunch& env, const NormParams& p);
