@@ -44,13 +44,24 @@ struct Tuning {
     int stream_k = -1;        // 1: cut the tiles of a ragged last wave along K (CTA-pair kernel) whenever a cut exists
     int token_tile = -1;      // few-token products: tokens of a tile (> 0, rounded up to a multiple of 16)
     int token_split = -1;     // few-token products: CTAs that share a tile's k blocks (1..8)
-    int token_ctas = -1;      // few-token products: CTAs per SM (1..3)
+    int token_ctas = -1;      // few-token products: CTAs per SM (1 or 2)
     int dependent_launch = -1;   // 0: the CTA-pair kernel is launched without programmatic stream serialisation
 };
 static int env_int(const char* name, int dflt) {
     const char* e = getenv(name);
     return e ? atoi(e) : dflt;
 }
+
+// How a scaled product runs (layer_api.cuh), and the plans made last.
+struct ProductPlan {
+    bool pair;
+    uint32_t tok, splits, ctas;
+    double us;   // estimated
+};
+struct PlanSlot {
+    uint64_t key[2];
+    ProductPlan plan;
+};
 
 struct mmeb200_ctx {
     int device = 0, chip = 2, sm_count = 148;
@@ -87,6 +98,7 @@ struct mmeb200_ctx {
     void* layer_ws = nullptr;
     size_t layer_ws_bytes = 0;
     cudaEvent_t layer_ws_used = nullptr;
+    PlanSlot plans[64] = {};
 
     int fail(int code, const char* fmt, ...) {
         char buf[512];
@@ -1208,6 +1220,7 @@ int mmeb200_set_option(mmeb200_ctx* c, const char* name, int value) {
     for (const auto& t : table)
         if (strcmp(t.name, name) == 0) {
             c->tune.*(t.field) = value < 0 ? -1 : value;
+            memset(c->plans, 0, sizeof c->plans);
             return 0;
         }
     return c->fail(MMEB200_ERR_INVALID_ARG, "unknown option '%s'", name);

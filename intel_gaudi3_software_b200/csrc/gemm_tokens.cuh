@@ -11,17 +11,17 @@
 // sums for them, adds them in rank order (integer sums are exact anyway; fp32 sums have a fixed order) and writes them
 // out. No workspace in global memory, no second launch, no atomics.
 //
-// Two CTAs share an SM wherever a tile has at most 128 tokens: one's set-up and epilogue run under the other's stream, and a
-// number of CTAs that is not a multiple of the SMs' still keeps HBM busy to the end.
+// Where there are more CTAs than SMs, two of them share an SM (with half the ring each): one's set-up and epilogue run under
+// the other's stream, and a number of CTAs that is not a multiple of the SMs' still keeps HBM busy to the end.
 //
-// CTA layout (192 threads): warp 0 feeds the ring by TMA, warp 1 allocates tensor memory and issues the MMAs, warps 2-5 are
-// the epilogue (lane = channel). Every mbarrier wait is bounded as in the other GEMM kernels.
+// CTA layout (320 threads): warp 0 feeds the ring by TMA, warp 1 allocates tensor memory and issues the MMAs, warps 2-9 are
+// the epilogue (lane = channel; two warps per 32 channels share the tokens: one alone is bound by its instructions' latency). Every mbarrier wait is bounded as in the other GEMM kernels.
 #pragma once
 #include "gemm_tokens.h"
 
 namespace mmeb200 {
 
-constexpr int kTokenThreads = 192;
+constexpr int kTokenThreads = 320;
 constexpr uint32_t kTokenBarrierBytes = 256;
 constexpr uint32_t kTokenWBytes = kBlockM * kRowBytes;
 constexpr uint32_t kTokenMaxStages = 12;
@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t token_add(uint32_t a, uint32_t b) {
     else return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
 }
 template <int KIND>
-__global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __grid_constant__ TokenGemmParams p) {
+__global__ void __launch_bounds__(kTokenThreads, 2) gemm_tokens_kernel(const __grid_constant__ TokenGemmParams p) {
     griddep_launch_dependents();
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_u32(smem) & 1023u) {   // uniform over the cluster
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __g
     const uint32_t tmem_base = *tmem_holder;
     griddep_wait();
 
-    const uint32_t sub = warp & 3, n = n0 + sub * 32 + lane;   // epilogue: this lane's channel
+    const uint32_t sub = warp & 3, grp = (warp - 2) >> 2, n = n0 + sub * 32 + lane;   // epilogue: this lane's channel
     float ws = 0.0f, bias = 0.0f;
     bool ready = true;
     if (warp == 0) {
@@ -163,13 +163,12 @@ __global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __g
     };
     if (p.splits == 1) {
         if (warp >= 2 && ready) {
-            float xs = 0.0f;
-            for (uint32_t c0 = 0; c0 < tokens; c0 += 16) {
+            for (uint32_t c0 = grp * 16; c0 < tokens; c0 += 32) {
                 uint32_t v[16];
                 tmem_ld_32x32b_x16(tmem_base + c0 + ((sub * 32) << 16), v);
-                if ((c0 & 31) == 0) xs = token_scale(c0);
+                const float xs = token_scale(c0);
                 tmem_ld_wait();
-                token_store<KIND, 16>(p, v, m0 + c0, tokens - c0, n, xs, c0 & 16, ws, bias);
+                token_store<KIND, 16>(p, v, m0 + c0, tokens - c0, n, xs, 0, ws, bias);
             }
         }
     } else {
@@ -181,7 +180,7 @@ __global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __g
         if (warp >= 2 && ready) {
             const uint32_t mine = smem_u32(inbox + rank * (share / 4) * kBlockM);   // the slot of this rank
             // each rank begins with its own share and goes round, so that no two ranks write to the same CTA at once
-            for (uint32_t i = 0; i < p.splits; ++i) {
+            for (uint32_t i = grp; i < p.splits; i += 2) {
                 const uint32_t owner = rank + i < p.splits ? rank + i : rank + i - p.splits, first = owner * share;
                 const uint32_t to = mapa_shared(mine, owner);
                 for (uint32_t t = 0; t < share && first + t < tokens; t += 16) {
@@ -200,8 +199,8 @@ __global__ void __launch_bounds__(kTokenThreads, 3) gemm_tokens_kernel(const __g
         if (warp >= 2) {
             const uint32_t first = rank * share, count = first < tokens ? min(share, tokens - first) : 0;
             float xs = 0.0f;
-            for (uint32_t t = 0; t < count; t += 4) {
-                if ((t & 31) == 0) xs = token_scale(first + t);
+            for (uint32_t t = 4 * grp; t < count; t += 8) {
+                if ((t & 31) == 4 * grp) xs = token_scale(first + t - 4 * grp);
                 uint4 sum = inbox[(t / 4) * kBlockM];
 #pragma unroll 7
                 for (uint32_t r = 1; r < p.splits; ++r) {

@@ -15,7 +15,7 @@ struct TokenGemmParams {
     uint32_t num_k_blocks;      // 128-byte blocks of K
     uint32_t tok;               // tokens of a tile (a multiple of 16, at most 256)
     uint32_t splits;            // CTAs of a cluster, each with its share of the k blocks
-    uint32_t ctas;              // CTAs that share an SM (1..3): sets how much shared memory each has for its ring
+    uint32_t ctas;              // CTAs that share an SM (1 or 2): sets how much shared memory each has for its ring
     uint32_t stages, stage_bytes;
     uint32_t tmem_cols;
     uint32_t idesc;

@@ -450,14 +450,6 @@ int layer_pad_operand(mmeb200_ctx* c, TmaOperand* o, uint8_t* dst) {
     return 0;
 }
 
-// Which kernel a product takes, and with what tile and split: the choice whose estimated time is least. Both estimates are in
-// SM clocks, from the same few rates: a k block (128 bytes of K) of 128 x 128 products is 256 clocks of the tensor cores, an
-// SM takes in about 60 bytes per clock from L2, the device about 3400 bytes per clock from HBM.
-struct ProductPlan {
-    bool pair;
-    uint32_t tok, splits, ctas;
-    double clocks;
-};
 int layer_token_capacity(mmeb200_ctx* c, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
     static int caps[64][2][4][9] = {};   // of the full ring, which all tiles nearly have
     int& cap = caps[c->device & 63][kind == KIND_I8][ctas][splits];
@@ -467,39 +459,67 @@ int layer_token_capacity(mmeb200_ctx* c, uint32_t kind, uint32_t tok, uint32_t s
     }
     return cap;
 }
-ProductPlan layer_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t N, uint32_t kb, uint32_t out_bytes) {
-    const double sms = c->sm_count, bytes = 128.0 * kb * (double(M) + N) + double(M) * N * out_bytes, floor_clocks = bytes / 3400;
+// Which kernel a product takes, and with what tile and split: the choice with the least estimated time, a function of the
+// sizes alone. The estimates (microseconds) are sums of a few measured rates, which reproduce the measured times of some
+// twenty shapes from 8 x 512 x 512 to 8192^3, both kernels forced in turn, mostly within 15 %:
+//   few-token kernel: 2.5 to launch; then the larger of HBM's 6050 bytes/ns for what is read and written once and of what the
+//     busiest SM takes in, 130 bytes/ns; then its epilogue, 25 ns per token of the tile, or the exchange of a split tile.
+//     Two CTAs per SM hide one's epilogue behind the other's loads, but share an SM where the device has SMs to spare.
+//   CTA-pair kernel: 0.355 per k block and wave of 256 x 256 tiles, or the epilogue where that takes longer.
+// (int8 256 x 8192 x 8192: 20 us on the first, 36 us on the second; 512 x 8192 x 8192: 33 and 28 us.)
+ProductPlan layer_make_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t N, uint32_t kb, uint32_t out_bytes, bool rows_aligned) {
+    const double sms = c->sm_count, hbm = (128.0 * kb * (double(M) + N) + double(M) * N * out_bytes) / 6.05e6;
     ProductPlan best{false, 0, 0, 0, 1e300};
-    const bool may_pair = c->tune.pair != 0 && M >= 256 && N >= 256;
-    if (may_pair) {
-        const double tiles = double((M + 255) / 256) * ((N + 255) / 256), waves = ceil(tiles / floor(sms / 2));
-        best = {true, 0, 0, 0, std::max(floor_clocks, waves * (kb * 540.0 + 1500)) + 6000};
+    if (c->tune.pair != 0 && M >= 256 && N >= 256) {
+        const double tiles = double((M + 255) / 256) * ((N + 255) / 256), waves = ceil(tiles / floor(sms / 2)), epilogue = rows_aligned ? 4.3 : 6.0;
+        best = {true, 0, 0, 0, 3.0 + std::max(hbm, waves * std::max(kb * 0.355, epilogue)) + (rows_aligned ? 2.0 : epilogue)};
         if (c->tune.pair == 1) return best;
     }
-    const double channels = (uint64_t(N) + kBlockM - 1) / kBlockM;
-    for (uint32_t want : {16u, 32u, 48u, 64u, 96u, 128u, 192u, 256u}) {
+    const double channels = double((uint64_t(N) + kBlockM - 1) / kBlockM);
+    uint32_t before = 0;
+    for (uint32_t want : {256u, 192u, 128u, 112u, 96u, 80u, 64u, 48u, 32u, 16u}) {
+        if (c->tune.token_tile > 0) want = std::min(256u, (uint32_t(c->tune.token_tile) + 15) & ~15u);
         // the smallest tile with as many token tiles as tiles of `want` tokens would give
-        const uint32_t m_tiles = (M + want - 1) / want, tok = ((M + m_tiles - 1) / m_tiles + 15) & ~15u;
+        const uint32_t m_tiles = (M + want - 1) / want, tok = c->tune.token_tile > 0 ? want : ((M + m_tiles - 1) / m_tiles + 15) & ~15u;
         const double stage = kBlockM * kRowBytes + tok * kRowBytes, tiles = channels * m_tiles;
-        if (m_tiles > 65535 || tiles * 8 >= 2147483648.0) continue;
-        if (c->tune.token_tile > 0 && tok != ((uint32_t(c->tune.token_tile) + 15) & ~15u)) continue;
-        const double k_clocks = std::max(stage / 60, 2.0 * tok);
-        for (uint32_t ctas = 1; ctas <= 3; ++ctas) {
-            if (c->tune.token_ctas > 0 ? ctas != uint32_t(c->tune.token_ctas) : ctas == 3) continue;
-            if (gemm_tokens_stages(tok, ctas) < 3) continue;
-            for (uint32_t s = 1; s <= 8 && s <= kb; ++s) {
-                const uint32_t per = (kb + s - 1) / s;
-                if (per * (s - 1) >= kb) continue;   // no share may be empty
-                if (c->tune.token_split > 0 && s != uint32_t(c->tune.token_split)) continue;
-                if (s > 1 && layer_token_capacity(c, kind, tok, s, ctas) <= 0) continue;
-                const double on_sm = ceil(tiles * s / sms);   // CTAs of the busiest SM
-                const double epilogue = s == 1 ? 12.0 * tok : 1500 + 14.0 * tok + 14.0 * tok / s;
-                const double clocks = std::max(floor_clocks, on_sm * per * k_clocks) + ceil(on_sm / ctas) * (2500 + epilogue);
-                if (clocks < best.clocks) best = {false, tok, s, ctas, clocks};
+        const double memory = hbm + 0.25 * (m_tiles - 1) * 128.0 * kb * N / 6.05e6;   // a quarter of the weights' further reads misses L2
+        if (tok == before || m_tiles > 65535 || tiles * 8 >= 2147483648.0) continue;
+        before = tok;
+        for (uint32_t s = 1; s <= 8 && s <= kb; ++s) {
+            const uint32_t per = (kb + s - 1) / s;
+            if (per * (s - 1) >= kb) continue;   // no share may be empty
+            if (c->tune.token_split > 0) {
+                if (s != std::min(uint32_t(c->tune.token_split), 8u) && s != 1) continue;   // 1 where that many do not exist
+            } else if (tiles * (s - 1) > 2 * sms) {
+                break;   // more CTAs than the device takes at once gain nothing
+            }
+            const double ctas_all = tiles * s, epilogue = s == 1 ? 0.025 * tok : 0.9 + tok * (0.010 + 0.040 / s);
+            const bool wanted = c->tune.token_split > 0 && s == std::min(uint32_t(c->tune.token_split), 8u);
+            for (uint32_t ctas = 1; ctas <= 2; ++ctas) {
+                if (gemm_tokens_stages(tok, ctas) < 3) continue;
+                if (c->tune.token_ctas > 0 && ctas != std::min(uint32_t(c->tune.token_ctas), 2u) && gemm_tokens_stages(tok, 2) >= 3) continue;
+                int held = int(sms) * int(ctas);
+                if (s > 1 && (held = layer_token_capacity(c, kind, tok, s, ctas)) <= 0) continue;
+                const double waves = ceil(ctas_all / held);
+                const double on_sm = ctas == 1 ? waves : std::max(ceil(ctas_all / sms), ctas_all * 2 > sms ? 2.0 : 1.0);
+                double us = 2.5 + std::max(memory, on_sm * per * stage / 130e3) + epilogue * waves + (waves - 1) * 1.5;
+                if (wanted) us *= 1e-6;   // the knob's choice wins
+                if (us < best.us) best = {false, tok, s, ctas, us};
             }
         }
     }
     return best;
+}
+// The estimates take a few microseconds; a program repeats the same few sizes.
+ProductPlan layer_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t N, uint32_t kb, uint32_t out_bytes, bool rows_aligned) {
+    const uint64_t key[2] = {uint64_t(M) << 32 | N, uint64_t(kb) << 32 | kind << 8 | out_bytes << 4 | uint32_t(rows_aligned) << 1 | 1u};
+    auto& slot = c->plans[(key[0] * 0x9E3779B97F4A7C15ull ^ key[1] * 0xC2B2AE3D27D4EB4Full) >> 58];
+    if (slot.key[0] != key[0] || slot.key[1] != key[1]) {
+        slot.plan = layer_make_plan(c, kind, M, N, kb, out_bytes, rows_aligned);
+        slot.key[0] = key[0];
+        slot.key[1] = key[1];
+    }
+    return slot.plan;
 }
 
 // Few tokens or few tiles: the cluster kernel (gemm_tokens.cuh).
@@ -513,6 +533,14 @@ int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, con
     TRY(encode_tiled(c, &p.tm_w, ow, kRowBytes, kBlockM));
     TRY(encode_tiled(c, &p.tm_x, ox, kRowBytes, p.tok));
     return launch_status(c, launch_gemm_tokens(launch_env(c), kind, p));
+}
+
+// Whether a tensor map can describe the output.
+bool layer_tma_output(const TokenGemmParams& t, const mmeb200_ctx* c, TmaOperand* out = nullptr) {
+    TmaOperand od;
+    od.ptr = t.out; od.elem = t.out_bf16 ? 2 : 4; od.inner = t.N; od.rows = t.M; od.row_stride = t.out_ld;
+    if (out) *out = od;
+    return c->tune.tma_store != 0 && (uint64_t(t.N) * od.elem) % 16 == 0 && tma_compatible(od);
 }
 
 // Many tiles: the CTA-pair kernel of the other GEMMs, with the scaling epilogue.
@@ -533,9 +561,7 @@ int layer_pair_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, cons
     TRY(encode_tiled(c, &p.tm_b, ow, kRowBytes, 128));
     p.b_cta_bytes = 128 * kRowBytes;
     TmaOperand od;
-    od.ptr = t.out; od.elem = t.out_bf16 ? 2 : 4; od.inner = p.N; od.rows = p.M; od.row_stride = t.out_ld;
-    if (c->tune.tma_store != 0 && (uint64_t(p.N) * od.elem) % 16 == 0 && tma_compatible(od) && encode_tiled(c, &p.tm_out, od, kRowBytes / od.elem, 32, od.elem == 2 ? 2 : 0) == 0)
-        p.tma_store = 1;
+    if (layer_tma_output(t, c, &od) && encode_tiled(c, &p.tm_out, od, kRowBytes / od.elem, 32, od.elem == 2 ? 2 : 0) == 0) p.tma_store = 1;
     bool two_groups = p.num_k_blocks <= 12;
     if (c->tune.epi_groups > 0) two_groups = c->tune.epi_groups == 2;
     return launch_status(c, launch_gemm_pair_scaled(launch_env(c), kind, two_groups ? 2 : 1, p, uint64_t(p.m_tiles) * p.n_tiles));
@@ -608,7 +634,7 @@ int run_scaled_gemm(mmeb200_ctx* c, mmeb200_tensor* out, const mmeb200_tensor* x
         if (!x_fits) TRY(layer_pad_operand(c, &ox, static_cast<uint8_t*>(scratch)));
         if (!w_fits) TRY(layer_pad_operand(c, &ow, static_cast<uint8_t*>(scratch) + xb));
     }
-    const ProductPlan plan = layer_plan(c, kind, p.M, p.N, uint32_t((K + kRowBytes - 1) / kRowBytes), p.out_bf16 ? 2 : 4);
+    const ProductPlan plan = layer_plan(c, kind, p.M, p.N, uint32_t((K + kRowBytes - 1) / kRowBytes), p.out_bf16 ? 2 : 4, layer_tma_output(p, c));
     if (plan.pair) TRY(layer_pair_product(c, kind, ox, ow, p, to));
     else if (plan.tok) TRY(layer_token_product(c, kind, ox, ow, plan, p));
     else return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");

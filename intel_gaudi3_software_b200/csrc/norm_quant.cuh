@@ -112,6 +112,36 @@ __device__ __forceinline__ void unpack(const uint32_t (&w)[W], float2 (&f)[4]) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+// Elements [from, to) of a packed piece, one by one. Out of line: only the ends of a warp's run come here, and inlined at every
+// store the code would not stay in the instruction cache.
+static __device__ __noinline__ void put_elements_16(uint16_t* a, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int from, int to) {
+    const uint32_t w[4] = {w0, w1, w2, w3};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e >= from && e < to) a[e] = uint16_t(w[e >> 1] >> (16 * (e & 1)));
+}
+static __device__ __noinline__ void put_elements_8(uint8_t* a, uint32_t w0, uint32_t w1, int from, int to) {
+    const uint32_t w[2] = {w0, w1};
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e >= from && e < to) a[e] = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+}
+static __device__ __noinline__ void put_elements_32(uint32_t* a, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, int from, int to) {
+    const uint32_t w[4] = {w0, w1, w2, w3};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (e >= from && e < to) a[e] = w[e];
+}
+template <int TYPE, int W>
+__device__ __forceinline__ void put_elements(uint8_t* a, const uint32_t (&v)[W], int from, int to) {
+    if constexpr (W == 2) put_elements_8(a, v[0], v[1], from, to);
+    else if constexpr (W == 4) put_elements_16(reinterpret_cast<uint16_t*>(a), v[0], v[1], v[2], v[3], from, to);
+    else {
+        put_elements_32(reinterpret_cast<uint32_t*>(a), v[0], v[1], v[2], v[3], from, to);
+        put_elements_32(reinterpret_cast<uint32_t*>(a) + 4, v[4], v[5], v[6], v[7], from - 4, to - 4);
+    }
+}
+
 // A row that is written. A warp writes its run step by step (32 pieces each), in order, all lanes together (SHIFT).
 // `start`: its first step; `last`: no step follows whose first piece is full.
 template <int TYPE, bool SHIFT>
@@ -137,15 +167,6 @@ struct RowOut {
             for (int i = 0; i < kWords / 4; ++i) reinterpret_cast<uint4*>(a)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
         }
     }
-    __device__ __forceinline__ static void put_elements(uint8_t* a, const uint32_t (&v)[kWords], int from, int to) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e >= from && e < to) {
-                if constexpr (kBytes == 4) reinterpret_cast<uint32_t*>(a)[e] = v[e];
-                else if constexpr (kBytes == 2) reinterpret_cast<uint16_t*>(a)[e] = uint16_t(v[e >> 1] >> (16 * (e & 1)));
-                else a[e] = uint8_t(v[e >> 2] >> (8 * (e & 3)));
-            }
-    }
     // n: elements of this lane's piece that exist; whole: the warp's 32 pieces are full
     __device__ __forceinline__ void store(uint32_t c, int n, const uint32_t (&v)[kWords], bool whole, bool start, bool last) {
         uint8_t* a = row + uint64_t(c) * kBytes;
@@ -153,7 +174,7 @@ struct RowOut {
             if (n) put(a, v);
         } else if (off == 0) {
             if (n == 8) put(a, v);
-            else put_elements(a, v, 0, n);
+            else put_elements<TYPE>(a, v, 0, n);
         } else {
             const uint32_t lane = threadIdx.x & 31;
             uint32_t both[kTail + kWords], out[kWords];
@@ -179,7 +200,7 @@ struct RowOut {
                 if (head || n < 8) from = 0;
                 else if (tail_mine) from = 8 - left;
                 if (n == 8 && !tail_mine && from == 0) to = 8 - left;
-                if (from < to) put_elements(a, v, from, to);
+                if (from < to) put_elements<TYPE>(a, v, from, to);
             }
         }
     }
@@ -544,7 +565,73 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 && RowKept<XT, RT>::kT
                          [&](uint32_t i, int n, float2 (&v)[4]) { scaled_piece<SHIFT>(p, kept[i], run.col(i), n, v); });
 }
 
-// Rows too long for registers: the row is read a second time (from L2, mostly) once its sums are known. The second read
+// The same with the row kept in shared memory (every lane its own pieces) and the pieces walked by a loop: the form for rows at
+// any alignment, whose shifts and ends would not fit the instruction cache unrolled, and for rows so long that registers
+// would leave one block per SM.
+template <int XT, int RT, bool SHIFT>
+__global__ void __launch_bounds__(512, 2) norm_loop_kernel(const __grid_constant__ NormParams p) {
+    constexpr int KT = RowKept<XT, RT>::kType, Q = RowKept<XT, RT>::kWords / 4;   // 16-byte words of a kept piece
+    __shared__ float2 scratch[32];
+    extern __shared__ uint4 keep[];   // [piece of a lane][16-byte word][thread]
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t row = blockIdx.x, threads = blockDim.x, pieces = (p.cols + threads * 8 - 1) / (threads * 8);   // per lane
+    const WarpRun<SHIFT> run{(threadIdx.x >> 5) * 256 * pieces, p.cols};
+    const bool tops = p.mode == NORM_I8 || p.mode == NORM_F8;
+    float2 sum = both(0.0f);
+    float top = 0.0f;
+    {
+        const RowIn<XT, SHIFT> xin(p.x, row_offset(p.x, row, p.dims, p.flat));
+        const RowIn<RT, SHIFT> rin(p.residual, RT != ROW_NONE ? row_offset(p.residual, row, p.dims, p.flat) : 0);
+        RowOut<KT, SHIFT> sout(p.sum, RT != ROW_NONE ? row_offset(p.sum, row, p.dims, p.flat) : 0);
+        const bool has_sum = RT != ROW_NONE && p.sum.ptr != nullptr;
+#pragma unroll 1
+        for (uint32_t i0 = 0; i0 < pieces; i0 += 2) {
+            typename RowIn<XT, SHIFT>::Raw x[2];
+            typename RowIn<RT, SHIFT>::Raw r[2];
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j)
+                if (i0 + j < pieces && run.size(i0 + j)) {
+                    xin.load(x[j], run.col(i0 + j));
+                    rin.load(r[j], run.col(i0 + j));
+                }
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                const uint32_t i = i0 + j;
+                if (i < pieces && run.any(i)) {
+                    const int n = run.size(i);
+                    RowKept<XT, RT> kept;
+                    if (n) {
+                        stream_piece<XT, RT, SHIFT>(xin, x[j], rin, r[j], kept);
+                        if (SHIFT && n < 8) clear_missing(kept, n);
+#pragma unroll
+                        for (int k = 0; k < Q; ++k)
+                            keep[(i * Q + k) * threads + threadIdx.x] = make_uint4(kept.w[4 * k], kept.w[4 * k + 1], kept.w[4 * k + 2], kept.w[4 * k + 3]);
+                        if (tops) sum_piece<true, SHIFT>(p, kept, run.col(i), n, sum, top);
+                        else sum_piece<false, SHIFT>(p, kept, run.col(i), n, sum, top);
+                    }
+                    if constexpr (RT != ROW_NONE) {
+                        if (has_sum && (SHIFT || n)) sout.store(run.col(i), n, kept.w, run.whole(i), i == 0, run.last(i, pieces));
+                    }
+                }
+            }
+        }
+    }
+    const float2 s = reduce_row<true, true>(sum.x + sum.y, top, threads >> 5, scratch);
+    const RowFactors f = row_factors(p, s.x, s.y, row);
+    if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
+    write_row_any<SHIFT, 1>(p, row_offset(p.out, row, p.dims, p.flat), run, pieces, f, [&](uint32_t i, int n, float2 (&v)[4]) {
+        RowKept<XT, RT> kept;
+#pragma unroll
+        for (int k = 0; k < Q; ++k) {
+            const uint4 q = n ? keep[(i * Q + k) * threads + threadIdx.x] : make_uint4(0, 0, 0, 0);
+            kept.w[4 * k] = q.x; kept.w[4 * k + 1] = q.y; kept.w[4 * k + 2] = q.z; kept.w[4 * k + 3] = q.w;
+        }
+        scaled_piece<SHIFT>(p, kept, run.col(i), n, v);
+    });
+}
+
+// Rows too long for shared memory: the row is read a second time (from L2, mostly) once its sums are known. The second read
 // takes the stream from `sum` where it was written (in place, x and the residual may be gone by then). A warp reads and
 // writes the same elements in both passes.
 template <int XT, int RT, bool SHIFT>

@@ -10,16 +10,29 @@ namespace mmeb200 {
 
 #if defined(INST_NORM)
 
-// Pieces of eight elements: at most four to a lane (eight in the longest rows), few enough for registers, enough for the loads
-// in flight to cover the latency of HBM and for the row's reduction to be a small part of the work. Short rows take one
-// warp each, longer ones as many warps as they have runs of pieces.
+// Short rows take one warp each. Aligned rows are kept in registers, at most four pieces of eight elements to a lane: few enough
+// for registers, enough for the loads in flight to cover the latency of HBM and for the row's reduction to be a small part of
+// the work. Longer rows, and rows at any alignment, are kept in shared memory.
 template <int XT, int RT, bool SHIFT>
 cudaError_t norm_of(const RowLaunch& env, const NormParams& p) {
     const dim3 warps((p.rows + 3) / 4), blocks(p.rows);
     if (p.cols <= 256) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 1, false, 128>, p, warps, 128, 0);
-    if (p.cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 4, false, 128>, p, warps, 128, 0);
-    if (p.cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 4, true, 512>, p, blocks, 32 * ((p.cols + 1023) / 1024), 0);
-    if (p.cols <= 32768) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 8, true, 512>, p, blocks, 32 * ((p.cols + 2047) / 2048), 0);
+    if constexpr (!SHIFT) {
+        if (p.cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 4, false, 128>, p, warps, 128, 0);
+        if (p.cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, SHIFT, 4, true, 512>, p, blocks, 32 * ((p.cols + 1023) / 1024), 0);
+    }
+    // a warp for every 1024 columns, at most 16 of them
+    const unsigned threads = std::min(512u, 32 * ((p.cols + 1023) / 1024));
+    const size_t keep = size_t((p.cols + threads * 8 - 1) / (threads * 8)) * threads * 8 * RowElem<RowKept<XT, RT>::kType>::kBytes;
+    if (keep <= 200 * 1024) {
+        static bool done[64] = {};
+        if (!done[env.device & 63]) {
+            const cudaError_t e = cudaFuncSetAttribute(norm_loop_kernel<XT, RT, SHIFT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+            if (e != cudaSuccess) return e;
+            done[env.device & 63] = true;
+        }
+        return launch_rows(env, norm_loop_kernel<XT, RT, SHIFT>, p, blocks, threads, keep);
+    }
     return launch_rows(env, norm_long_kernel<XT, RT, SHIFT>, p, blocks, 1024, 0);
 }
 template cudaError_t norm_of<INST_XT, INST_NORM, INST_SHIFT != 0>(const RowLaunch&, const NormParams&);

@@ -10,13 +10,12 @@ from intel_gaudi3_software_b200 import abi
 U = 2.0 ** -24
 # half a step of the output types, relative
 HALF = {abi.BF16: 2.0 ** -8, abi.FP32: 2.0 ** -24}
-# Additions a term of a row's sum passes through: at most 64 values of its thread, five levels over the warp, at most 16 warps.
-# Rows above 32768 columns (8192 in the gradient): 32 warps, eight values for every 8192 columns.
-ROW_DEPTH = 64 + 5 + 16
+# Additions a term of a row's sum passes through: the values of its thread (two interleaved sums: half of at most 32 up to
+# 16384 columns, eight for every 4096 columns above), the two sums' join, five levels over the warp, at most 32 warps.
 
 
 def row_depth(cols):
-    return max(ROW_DEPTH, 8 * -(-cols // 8192) + 5 + 32)
+    return max(32, 8 * -(-cols // 4096)) + 1 + 5 + 32
 
 
 def top_of(dtype, bias=7, mode=abi.INFNAN_MINIMAL):
