@@ -161,7 +161,6 @@ RowTensor layer_rows(const mmeb200_tensor* t) {
     r.ptr = t->data;
     r.type = layer_row_type(t->dtype);
     for (int d = 0; d < 4; ++d) r.stride[d] = t->strides[d + 1];
-    r.bytes = span_elems(t) * unsigned(layer_elem_size(t));
     return r;
 }
 // Merges dims 1..4 into one where every tensor's strides allow it, so that a row's place needs no division.
@@ -188,13 +187,20 @@ void layer_flatten(uint32_t (&dims)[4], uint32_t* flat, std::initializer_list<Ro
     }
     *flat = n == 0;
 }
-// Eight elements at a time: 16 bytes of bf16 or fp32, 8 bytes of codes.
-bool layer_vectors(const RowTensor& t, const uint32_t (&dims)[4]) {
-    if (!t.ptr) return true;
-    if (reinterpret_cast<uintptr_t>(t.ptr) % (t.type >= ROW_I8 ? 8 : 16)) return false;
-    for (int d = 0; d < 4; ++d)
-        if (dims[d] > 1 && t.stride[d] % 8) return false;
-    return true;
+// How many elements at once the rows of these tensors and gamma allow: eight (16 bytes of bf16 or fp32, 8 bytes of codes), two,
+// or one.
+int layer_vector(uint32_t cols, const uint32_t (&dims)[4], std::initializer_list<const RowTensor*> all, const void* gamma, const void* partial) {
+    for (const uint32_t vec : {8u, 2u}) {
+        bool fits = cols % vec == 0 && reinterpret_cast<uintptr_t>(gamma) % (vec == 8 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(partial) % (vec == 8 ? 16 : 8) == 0;
+        for (const RowTensor* t : all) {
+            if (!t->ptr) continue;
+            const uint32_t elem = t->type >= ROW_I8 ? 1 : t->type == ROW_BF16 ? 2 : 4;
+            fits = fits && reinterpret_cast<uintptr_t>(t->ptr) % std::min(16u, vec * elem) == 0;
+            for (int d = 0; d < 4; ++d) fits = fits && (dims[d] == 1 || t->stride[d] % vec == 0);
+        }
+        if (fits) return int(vec);
+    }
+    return 1;
 }
 RowLaunch layer_launch(const mmeb200_ctx* c) { return RowLaunch{c->device, c->sm_count, c->stream, c->tune.dependent_launch != 0}; }
 
@@ -286,8 +292,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     NormParams p;
     memset(&p, 0, sizeof p);
     p.x = layer_rows(dx); p.residual = layer_rows(dres); p.sum = layer_rows(dsum); p.out = layer_rows(dout);
-    p.gamma = dgam ? dgam->data : nullptr;
-    p.gamma_type = dgam ? layer_row_type(dgam->dtype) : ROW_NONE;
+    p.gamma = layer_rows(dgam);
     if (dscale) {
         if (given) { p.given = static_cast<const float*>(dscale->data); p.given_stride = num_elems(dscale) == 1 ? 0 : 1; }
         else p.scale = static_cast<float*>(dscale->data);
@@ -297,8 +302,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     layer_flatten(p.dims, &p.flat, {&p.x, &p.residual, &p.sum, &p.out});
     p.norm = norm; p.eps = eps; p.per_col = 1.0f / float(cols); p.top = top; p.hw = hw;
     p.mode = out->dtype == DT_BF16 ? NORM_BF16 : out->dtype == DT_FP32 ? NORM_F32 : out->dtype == MMEB200_INT8 ? (given ? NORM_I8_GIVEN : NORM_I8) : given ? NORM_F8_GIVEN : NORM_F8;
-    p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.residual, p.dims) && layer_vectors(p.sum, p.dims) && layer_vectors(p.out, p.dims) && p.gamma_whole;
+    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.residual, &p.sum, &p.out}, p.gamma.ptr, nullptr);
     CUDA_OK(c, launch_norm(layer_launch(c), p, vec));
     c->launches++;
     return st.finish();
@@ -329,7 +333,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         TRY(layer_check_vector(c, dgamma, "dgamma", cols));
     }
     if (!(eps >= 0.0f) || eps > 3.4e38f) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
-    const uint32_t blocks = norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols));
+    const uint32_t blocks = norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), x->dtype == DT_FP32);
     const uint64_t need = uint64_t(blocks) * cols;
     if (workspace) {
         TRY(layer_check(c, workspace, "workspace", true, false));
@@ -365,8 +369,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
     NormGradParams p;
     memset(&p, 0, sizeof p);
     p.x = layer_rows(tx); p.dy = layer_rows(ty); p.dsum = layer_rows(ts); p.dx = layer_rows(to);
-    p.gamma = tg ? tg->data : nullptr;
-    p.gamma_type = tg ? layer_row_type(tg->dtype) : ROW_NONE;
+    p.gamma = layer_rows(tg);
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     for (int d = 0; d < 4; ++d) p.dims[d] = x->sizes[d + 1];
     layer_flatten(p.dims, &p.flat, {&p.x, &p.dy, &p.dsum, &p.dx});
@@ -379,9 +382,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
             p.partial = static_cast<float*>(scratch);
         }
     }
-    p.gamma_whole = reinterpret_cast<uintptr_t>(p.gamma) % 16 == 0;
-    const bool vec = cols % 8 == 0 && layer_vectors(p.x, p.dims) && layer_vectors(p.dy, p.dims) && layer_vectors(p.dsum, p.dims) && layer_vectors(p.dx, p.dims) && p.gamma_whole &&
-                     reinterpret_cast<uintptr_t>(p.partial) % 16 == 0;
+    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.dy, &p.dsum, &p.dx}, p.gamma.ptr, p.partial);
     CUDA_OK(c, launch_norm_grad(layer_launch(c), p, vec, blocks));
     c->launches++;
     if (dgamma) {
@@ -428,7 +429,7 @@ int run_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, con
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     int launches = 0;
     const uint32_t dims[4] = {p.rows, 1, 1, 1};
-    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, cols % 8 == 0 && layer_vectors(p.x, dims), &launches));
+    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, layer_vector(p.cols, dims, {&p.x}, nullptr, nullptr), &launches));
     c->launches += uint64_t(launches);
     return st.finish();
 }
@@ -666,7 +667,7 @@ extern "C" int mmeb200_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200
 }
 extern "C" size_t mmeb200_rms_norm_grad_workspace(const mmeb200_ctx* c, uint64_t rows, uint64_t cols) {
     if (!c || rows >= (uint64_t(1) << 31) || cols >= (uint64_t(1) << 31)) return 0;
-    return size_t(norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols))) * cols * sizeof(float);
+    return size_t(std::max(norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), false), norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), true))) * cols * sizeof(float);
 }
 extern "C" int mmeb200_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, const mmeb200_tensor* x, int op, int scale_mode) {
     return layer_entry(c, [&] { return run_quantize(c, out, scale, x, op, scale_mode); });

@@ -7,30 +7,28 @@
 namespace mmeb200 {
 
 template <int XT, int RT>
-static cudaError_t norm_of(const RowLaunch& env, const NormParams& p, bool vec) {
-    return vec ? norm_of<XT, RT, false>(env, p) : norm_of<XT, RT, true>(env, p);
+static cudaError_t norm_with(const RowLaunch& env, const NormParams& p, int vec) {
+    return vec == 8 ? norm_of<XT, RT, 8>(env, p) : vec == 2 ? norm_of<XT, RT, 2>(env, p) : norm_of<XT, RT, 1>(env, p);
 }
-cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec) {
+cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec) {
     const int rt = p.residual.ptr ? p.residual.type : ROW_NONE;
     if (p.x.type == ROW_BF16)
-        return rt == ROW_NONE ? norm_of<ROW_BF16, ROW_NONE>(env, p, vec) : rt == ROW_BF16 ? norm_of<ROW_BF16, ROW_BF16>(env, p, vec) : norm_of<ROW_BF16, ROW_F32>(env, p, vec);
-    return rt == ROW_NONE ? norm_of<ROW_F32, ROW_NONE>(env, p, vec) : rt == ROW_BF16 ? norm_of<ROW_F32, ROW_BF16>(env, p, vec) : norm_of<ROW_F32, ROW_F32>(env, p, vec);
+        return rt == ROW_NONE ? norm_with<ROW_BF16, ROW_NONE>(env, p, vec) : rt == ROW_BF16 ? norm_with<ROW_BF16, ROW_BF16>(env, p, vec) : norm_with<ROW_BF16, ROW_F32>(env, p, vec);
+    return rt == ROW_NONE ? norm_with<ROW_F32, ROW_NONE>(env, p, vec) : rt == ROW_BF16 ? norm_with<ROW_F32, ROW_BF16>(env, p, vec) : norm_with<ROW_F32, ROW_F32>(env, p, vec);
 }
 
-uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols) {
-    const uint32_t per_block = cols <= 1024 ? 4 : 1;
-    // as many blocks as the SMs hold at once (128 registers a thread): a block walks its rows to the end
-    const uint32_t resident = std::max(1u, 512u / grad_threads(cols));
-    return std::min<uint32_t>((rows + per_block - 1) / per_block, uint32_t(sm_count) * resident);
+uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32) {
+    const GradShape g = grad_shape(cols, fp32);
+    // as many blocks as the SMs hold at once: a block walks its rows to the end
+    return uint32_t(std::min<uint64_t>((uint64_t(rows) + g.rows_per_block - 1) / g.rows_per_block, uint64_t(sm_count) * g.blocks_per_sm));
 }
-
-template <int XT>
-static cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks) {
-    if (p.dsum.ptr) return vec ? norm_grad_of<XT, true, false>(env, p, blocks) : norm_grad_of<XT, true, true>(env, p, blocks);
-    return vec ? norm_grad_of<XT, false, false>(env, p, blocks) : norm_grad_of<XT, false, true>(env, p, blocks);
+template <int XT, bool DSUM>
+static cudaError_t norm_grad_with(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
+    return vec == 8 ? norm_grad_of<XT, DSUM, 8>(env, p, blocks) : vec == 2 ? norm_grad_of<XT, DSUM, 2>(env, p, blocks) : norm_grad_of<XT, DSUM, 1>(env, p, blocks);
 }
-cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks) {
-    return p.x.type == ROW_BF16 ? norm_grad_of<ROW_BF16>(env, p, vec, blocks) : norm_grad_of<ROW_F32>(env, p, vec, blocks);
+cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
+    if (p.x.type == ROW_BF16) return p.dsum.ptr ? norm_grad_with<ROW_BF16, true>(env, p, vec, blocks) : norm_grad_with<ROW_BF16, false>(env, p, vec, blocks);
+    return p.dsum.ptr ? norm_grad_with<ROW_F32, true>(env, p, vec, blocks) : norm_grad_with<ROW_F32, false>(env, p, vec, blocks);
 }
 
 struct ColumnSums { const float* partial; float* out; uint32_t blocks, cols; };
@@ -40,10 +38,13 @@ cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float
     return launch_rows(env, column_sums_kernel, p, dim3((cols + 31) / 32), 1024, 0);
 }
 
-cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, bool vec, int* launches) {
+template <int XT>
+static cudaError_t quant_trans_with(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
+    return vec == 8 ? quant_trans_of<XT, 8>(env, p, launches) : vec == 2 ? quant_trans_of<XT, 2>(env, p, launches) : quant_trans_of<XT, 1>(env, p, launches);
+}
+cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
     *launches = 0;
-    if (p.x.type == ROW_BF16) return vec ? quant_trans_of<ROW_BF16, false>(env, p, launches) : quant_trans_of<ROW_BF16, true>(env, p, launches);
-    return vec ? quant_trans_of<ROW_F32, false>(env, p, launches) : quant_trans_of<ROW_F32, true>(env, p, launches);
+    return p.x.type == ROW_BF16 ? quant_trans_with<ROW_BF16>(env, p, vec, launches) : quant_trans_with<ROW_F32>(env, p, vec, launches);
 }
 
 // A product's operand whose rows do not start on 16 bytes, copied to rows that do. A thread makes 16 bytes of the copy from

@@ -19,14 +19,11 @@ struct RowTensor {
     void* ptr;
     int type;              // ROW_*
     uint32_t stride[4];    // elements, dims 1..4
-    uint64_t bytes;        // from the first element to the last
 };
 
 struct NormParams {
     RowTensor x, residual, sum, out;
-    const void* gamma;     // nullptr: ones
-    int gamma_type;
-    uint32_t gamma_whole;  // gamma starts on 16 bytes
+    RowTensor gamma;       // one row; ptr nullptr: ones
     float* scale;          // 8-bit outputs: the step of every row (written)
     const float* given;    // 8-bit outputs with a given scale: read instead; given_stride 0 = one for all rows
     uint32_t given_stride;
@@ -42,13 +39,12 @@ struct NormParams {
 
 struct NormGradParams {
     RowTensor dx, dy, x, dsum;
-    const void* gamma;
-    int gamma_type;
-    uint32_t gamma_whole;
+    RowTensor gamma;
     float* partial;        // [blocks][cols]; nullptr: no gradient of gamma wanted
     uint32_t rows, cols;
     uint32_t dims[4];
     uint32_t flat;
+    uint32_t steps;        // set by the launcher
     float eps, per_col;
 };
 
@@ -73,14 +69,14 @@ struct RowLaunch {
     bool dependent_launch;
 };
 
-// `vec`: the length, start and pitch of every row of every tensor allow aligned accesses of eight elements.
-cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, bool vec);
+// `vec` (8, 2 or 1): the length, start and pitch of every row of every tensor, gamma included, allow accesses of so many elements.
+cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec);
 // Blocks the gradient kernel runs with, i.e. rows of `partial`.
-uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols);
-cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, bool vec, uint32_t blocks);
+uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32);
+cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks);
 cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols);
 // Number of kernels launched is returned in *launches.
-cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, bool vec, int* launches);
+cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches);
 
 // Rows of `cols` bytes, src_ld bytes apart at any alignment, copied to rows dst_ld bytes apart (dst and dst_ld multiples of 16).
 cudaError_t launch_pad_rows(const RowLaunch& env, const void* src, void* dst, uint64_t rows, uint64_t cols, uint64_t src_ld, uint64_t dst_ld);
