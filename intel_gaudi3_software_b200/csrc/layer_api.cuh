@@ -225,6 +225,10 @@ int layer_codes(mmeb200_ctx* c, const mmeb200_tensor* out, float* top, Fp8HwCast
     return 0;
 }
 
+// Whether codes up to the type's largest finite value come from the hardware conversion alone (the 1-4-3 convention without
+// infinities has codes above the hardware format's largest).
+bool layer_direct(const mmeb200_tensor* out) { return dtype_is_fp8(out->dtype) && !(out->dtype == DT_FP8_143 && out->inf_nan_mode == MMEB200_INFNAN_NONE); }
+
 // The scale argument of an 8-bit output, or its absence for a float output.
 int layer_check_out_scale(mmeb200_ctx* c, const mmeb200_tensor* out, const mmeb200_tensor* scale, int scale_mode, uint64_t rows) {
     if (!layer_is_eight(out->dtype)) {
@@ -301,6 +305,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     for (int d = 0; d < 4; ++d) p.dims[d] = x->sizes[d + 1];
     layer_flatten(p.dims, &p.flat, {&p.x, &p.residual, &p.sum, &p.out});
     p.norm = norm; p.eps = eps; p.per_col = 1.0f / float(cols); p.top = top; p.hw = hw;
+    p.fp8_direct = layer_direct(out);
     p.mode = out->dtype == DT_BF16 ? NORM_BF16 : out->dtype == DT_FP32 ? NORM_F32 : out->dtype == MMEB200_INT8 ? (given ? NORM_I8_GIVEN : NORM_I8) : given ? NORM_F8_GIVEN : NORM_F8;
     const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.residual, &p.sum, &p.out}, p.gamma.ptr, nullptr);
     CUDA_OK(c, launch_norm(layer_launch(c), p, vec));
@@ -411,6 +416,7 @@ int run_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, con
     QuantTransParams p;
     memset(&p, 0, sizeof p);
     TRY(layer_codes(c, out, &p.top, &p.hw));
+    p.fp8_direct = layer_direct(out);
     TRY(layer_check_distinct(c, out, "output"));
     TRY(layer_check_overlap(c, out, "output", x, "x", false));
     TRY(layer_check_overlap(c, out, "output", scale, "scale", false));

@@ -158,16 +158,16 @@ __device__ __forceinline__ uint8_t* row_of(const RowTensor& t, uint32_t row, con
 }
 
 // ------------------------------------------------------------------------------------------ 8-bit codes
-// How values become codes: `step`, and its reciprocal where that decides them. recip = 0: no codes (a step that is zero,
-// negative or no finite number), NaN: the reciprocal is no normal number, every code is divided for.
+// How values become codes: `step`, and minus its reciprocal. 0: no codes (a step that is zero, negative or no finite number);
+// NaN: so large or small a step that the quotient has to be divided for.
 struct CodeStep {
-    float step, recip;
+    float step, nrecip;
 };
 __device__ __forceinline__ CodeStep make_code_step(float step) {
     CodeStep s;
     s.step = step;
-    if (!(step > 0.0f && step < __uint_as_float(0x7F800000u))) s.recip = 0.0f;
-    else s.recip = (step >= 0x1p-126f && step <= 0x1p126f) ? __frcp_rn(step) : __uint_as_float(0x7FC00000u);
+    if (!(step > 0.0f && step < __uint_as_float(0x7F800000u))) s.nrecip = 0.0f;
+    else s.nrecip = (step >= 0x1p-60f && step <= 0x1p60f) ? -__frcp_rn(step) : __uint_as_float(0x7FC00000u);
     return s;
 }
 constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to the nearest whole number, ties to even
@@ -175,64 +175,56 @@ constexpr float kRoundMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to 
 __device__ __forceinline__ uint32_t pack_low_bytes(float a, float b, float c, float d) {
     return __byte_perm(__byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040), __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040), 0x5410);
 }
-// Four codes by the definition: the correctly rounded quotient, then the code. Out of line: few values come here.
+// Minus the correctly rounded quotients v / step, in two operations more than a multiplication: with y the correctly rounded
+// reciprocal and q = v * y, the remainder r = v - q * step is exact in one fused multiply-add, and q + r * y rounds to the
+// quotient (P. W. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, IBM J. Res. Dev. 34,
+// 1990). Steps between 2^-60 and 2^60 keep every remainder that can decide a code a normal number. Worked with the sign
+// turned, zeros keep theirs.
+__device__ __forceinline__ float2 minus_quotient(float2 v, const CodeStep& s) {
+    const float2 q = __fmul2_rn(v, both(s.nrecip)), r = __ffma2_rn(q, both(s.step), v);
+    return __ffma2_rn(r, both(s.nrecip), q);
+}
+__device__ __forceinline__ uint32_t int8_codes(float2 nq0, float2 nq1) {   // |quotient| <= 127
+    const float2 a = __ffma2_rn(nq0, both(-1.0f), both(kRoundMagic)), b = __ffma2_rn(nq1, both(-1.0f), both(kRoundMagic));
+    return pack_low_bytes(a.x, a.y, b.x, b.y);
+}
+// Four fp8 codes of quotients that stay below the hardware conversion's own limit (hw.scale: the exponent bias).
+__device__ __forceinline__ uint32_t fp8_codes(float2 nq0, float2 nq1, const Fp8HwCast& hw) {
+    const float2 a = __fmul2_rn(nq0, both(hw.scale)), b = __fmul2_rn(nq1, both(hw.scale));
+    uint16_t lo, hi;
+    if (hw.e5m2) {
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+        asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
+    } else {
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(a.y), "f"(a.x));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(b.y), "f"(b.x));
+    }
+    return (uint32_t(lo) | uint32_t(hi) << 16) ^ 0x80808080u;
+}
+// Four codes under any step and of any value: given steps, steps of extreme size, conventions whose codes pass the hardware's.
 template <bool I8>
 static __device__ __noinline__ uint32_t codes_by_division(float v0, float v1, float v2, float v3, float step, const Fp8HwCast& hw) {
     float t[4] = {__fdiv_rn(v0, step), __fdiv_rn(v1, step), __fdiv_rn(v2, step), __fdiv_rn(v3, step)};
     if constexpr (I8) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = fminf(fmaxf(t[e], -127.0f), 127.0f) + kRoundMagic;
+        for (int e = 0; e < 4; ++e) t[e] = t[e] == t[e] ? fminf(fmaxf(t[e], -127.0f), 127.0f) + kRoundMagic : kRoundMagic;   // a NaN has no code
         return pack_low_bytes(t[0], t[1], t[2], t[3]);
     } else {
         return f32x4_to_fp8_hw(t, hw);
     }
 }
-// The four codes of v / step, packed. v * recip is within 2^-23 of the quotient, relatively, and the 32-bit quotient within
-// 2^-24 of the exact one, so
-//   int8: for |quotient| <= 127 the product is off by at most 2^-15.4; unless it lies closer than 2^-15 to the middle between two
-//         whole numbers it rounds as the quotient does (one multiplication and three additions per element);
-//   fp8:  where product * (1 - 2^-22) and product * (1 + 2^-22) have the same code, it is the quotient's (the cast is monotone).
-// The few quads with an element that fails its test are divided. GIVEN: the step is the caller's, quotients may be anything.
-template <bool I8, bool GIVEN>
+// SURE: the step is the values' own (no quotient beyond the largest code) and has a reciprocal (fast_step).
+template <bool I8, bool SURE>
 __device__ __forceinline__ uint32_t make_codes(float2 v0, float2 v1, const CodeStep& s, const Fp8HwCast& hw) {
-    if (s.recip == 0.0f) return 0u;
-    float2 x[2] = {v0, v1};
-    uint32_t w;
-    bool sure;
-    if constexpr (I8) {
-        float2 m[2];
-        float worst = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if constexpr (GIVEN) {   // a NaN has no code (rows with one have no step of their own)
-                x[i].x = x[i].x == x[i].x ? x[i].x : 0.0f;
-                x[i].y = x[i].y == x[i].y ? x[i].y : 0.0f;
-            }
-            float2 t = __fmul2_rn(x[i], both(s.recip));
-            if constexpr (GIVEN) {
-                t.x = fminf(fmaxf(t.x, -127.0f), 127.0f);
-                t.y = fminf(fmaxf(t.y, -127.0f), 127.0f);
-            }
-            m[i] = __fadd2_rn(t, both(kRoundMagic));
-            const float2 back = __fadd2_rn(m[i], both(-kRoundMagic)), off = __ffma2_rn(back, both(-1.0f), t);
-            worst = fmaxf(worst, fmaxf(fabsf(off.x), fabsf(off.y)));
-        }
-        sure = worst <= 0.5f - 0x1p-15f && s.recip == s.recip;
-        w = pack_low_bytes(m[0].x, m[0].y, m[1].x, m[1].y);
+    if constexpr (SURE) {
+        if constexpr (I8) return int8_codes(minus_quotient(v0, s), minus_quotient(v1, s));
+        else return fp8_codes(minus_quotient(v0, s), minus_quotient(v1, s), hw);
     } else {
-        float lo[4], hi[4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float2 t = __fmul2_rn(x[i], both(s.recip)), l = __fmul2_rn(t, both(1.0f - 0x1p-22f)), h = __fmul2_rn(t, both(1.0f + 0x1p-22f));
-            lo[2 * i] = l.x; lo[2 * i + 1] = l.y;
-            hi[2 * i] = h.x; hi[2 * i + 1] = h.y;
-        }
-        w = f32x4_to_fp8_hw(lo, hw);
-        sure = w == f32x4_to_fp8_hw(hi, hw) && s.recip == s.recip;
+        return s.nrecip == 0.0f ? 0u : codes_by_division<I8>(v0.x, v0.y, v1.x, v1.y, s.step, hw);
     }
-    if (!sure) w = codes_by_division<I8>(x[0].x, x[0].y, x[1].x, x[1].y, s.step, hw);
-    return w;
 }
+// (int8: direct = true; fp8: no quotient of a row's own step passes the hardware conversion's limit)
+__device__ __forceinline__ bool fast_step(const CodeStep& s, bool direct) { return direct && s.nrecip < 0.0f; }
 
 // ------------------------------------------------------------------------------------------ reductions
 // Sums over the threads of a row: a warp, or the `warps` warps of the block (BLOCK). The order is fixed. MAX: the second is a
@@ -334,8 +326,10 @@ __device__ __forceinline__ void read_steps(const NormParams& p, const NormRows<X
             }
             float2 h[4];
             kept[j].values(h);
+            if (p.norm) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum = __ffma2_rn(h[i], h[i], sum);
+                for (int i = 0; i < 4; ++i) sum = __ffma2_rn(h[i], h[i], sum);
+            }
             if (tops) {
                 if (p.gamma.ptr) {
                     float2 g[4];
@@ -350,7 +344,7 @@ __device__ __forceinline__ void read_steps(const NormParams& p, const NormRows<X
     }
 }
 // One step of the second pass: the finished values, as floats or codes.
-template <int MODE, int VEC, int XT, int RT>
+template <int MODE, bool FAST, int VEC, int XT, int RT>
 __device__ __forceinline__ void write_step(const NormParams& p, uint8_t* out, uint32_t c, const RowKept<XT, RT>& kept, const RowFactors& f) {
     constexpr int kType = MODE == NORM_BF16 ? ROW_BF16 : MODE == NORM_F32 ? ROW_F32 : ROW_I8;
     float2 v[4];
@@ -362,30 +356,34 @@ __device__ __forceinline__ void write_step(const NormParams& p, uint8_t* out, ui
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(v[i], g[i]);
     }
-    if constexpr (MODE == NORM_I8 || MODE == NORM_F8) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) w[k] = make_codes<MODE == NORM_I8, false>(v[2 * k], v[2 * k + 1], f.step, p.hw);
-    } else {
+    if constexpr (MODE != NORM_I8 && MODE != NORM_F8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = __fmul2_rn(v[k], both(f.inv));
-        if constexpr (MODE == NORM_BF16 || MODE == NORM_F32) pack<kType>(v, w);
-        else {
+    }
+    if constexpr (MODE == NORM_BF16 || MODE == NORM_F32) pack<kType>(v, w);
+    else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) w[k] = make_codes<MODE == NORM_I8_GIVEN, true>(v[2 * k], v[2 * k + 1], f.step, p.hw);
-        }
+        for (int k = 0; k < 2; ++k) w[k] = make_codes<MODE == NORM_I8 || MODE == NORM_I8_GIVEN, FAST>(v[2 * k], v[2 * k + 1], f.step, p.hw);
     }
     store_piece<kType, VEC>(out, c, p.cols, w);
 }
-// What differs between the kinds of output is decided once per row: `write(mode)` is called with the kind as a constant.
+// What differs between the kinds of output is decided once per row: `write(mode, fast)` is called with the kind as a constant,
+// and whether the row's codes can do without a test of the step.
 template <typename F>
-__device__ __forceinline__ void for_mode(int mode, F&& write) {
-    switch (mode) {
-        case NORM_BF16: write(std::integral_constant<int, NORM_BF16>()); break;
-        case NORM_F32: write(std::integral_constant<int, NORM_F32>()); break;
-        case NORM_I8: write(std::integral_constant<int, NORM_I8>()); break;
-        case NORM_F8: write(std::integral_constant<int, NORM_F8>()); break;
-        case NORM_I8_GIVEN: write(std::integral_constant<int, NORM_I8_GIVEN>()); break;
-        default: write(std::integral_constant<int, NORM_F8_GIVEN>()); break;
+__device__ __forceinline__ void for_mode(const NormParams& p, const RowFactors& f, F&& write) {
+    switch (p.mode) {
+        case NORM_BF16: write(std::integral_constant<int, NORM_BF16>(), std::false_type()); break;
+        case NORM_F32: write(std::integral_constant<int, NORM_F32>(), std::false_type()); break;
+        case NORM_I8:
+            if (fast_step(f.step, true)) write(std::integral_constant<int, NORM_I8>(), std::true_type());
+            else write(std::integral_constant<int, NORM_I8>(), std::false_type());
+            break;
+        case NORM_F8:
+            if (fast_step(f.step, p.fp8_direct)) write(std::integral_constant<int, NORM_F8>(), std::true_type());
+            else write(std::integral_constant<int, NORM_F8>(), std::false_type());
+            break;
+        case NORM_I8_GIVEN: write(std::integral_constant<int, NORM_I8_GIVEN>(), std::false_type()); break;
+        default: write(std::integral_constant<int, NORM_F8_GIVEN>(), std::false_type()); break;
     }
 }
 __device__ __forceinline__ uint8_t* out_row(const NormParams& p, uint32_t row) {
@@ -417,10 +415,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 && RowKept<XT, RT>::kT
     const RowFactors f = row_factors(p, s.x, s.y, row);
     if (p.scale && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) p.scale[row] = f.scale;
     uint8_t* out = out_row(p, row);
-    for_mode(p.mode, [&](auto mode) {
+    for_mode(p, f, [&](auto mode, auto fast) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (in_row<VEC>(c0 + i * 256, p.cols)) write_step<decltype(mode)::value, VEC>(p, out, c0 + i * 256, kept[i], f);
+            if (in_row<VEC>(c0 + i * 256, p.cols)) write_step<decltype(mode)::value, decltype(fast)::value, VEC>(p, out, c0 + i * 256, kept[i], f);
     });
 }
 
@@ -447,7 +445,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
     const RowFactors f = row_factors(p, s.x, s.y, row);
     if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
     uint8_t* out = out_row(p, row);
-    for_mode(p.mode, [&](auto mode) {
+    for_mode(p, f, [&](auto mode, auto fast) {
 #pragma unroll 1
         for (uint32_t c = first; in_row<VEC>(c, p.cols); c += 32 * 256) {
             RowKept<XT, RT> kept;
@@ -461,7 +459,7 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
                 load_piece<RT, VEC>(rows.residual, c, p.cols, r);
                 stream_values<XT, RT>(x, r, kept);
             }
-            write_step<decltype(mode)::value, VEC>(p, out, c, kept, f);
+            write_step<decltype(mode)::value, decltype(fast)::value, VEC>(p, out, c, kept, f);
         }
     });
 }
@@ -782,6 +780,11 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
 // Tiles of 128 rows x 256 columns: a warp takes four rows at a time, a lane eight of their columns, whose codes make one word per
 // column. The tile's columns leave as aligned 16-byte words (byte by byte at their ends).
 constexpr uint32_t kTransRows = 128;
+template <bool I8, bool GIVEN>
+__device__ __forceinline__ uint32_t column_codes(const QuantTransParams& p, float2 v0, float2 v1, const CodeStep& s) {
+    if (!GIVEN && fast_step(s, I8 || p.fp8_direct)) return make_codes<I8, true>(v0, v1, s, p.hw);
+    return make_codes<I8, false>(v0, v1, s, p.hw);
+}
 template <int XT, int VEC, bool I8, bool GIVEN>
 __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_constant__ QuantTransParams p) {
     constexpr int W = 2 * RowElem<XT>::kBytes;
@@ -816,8 +819,8 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint32_t even = 2 * k * 32 + lane, odd = even + 32;
-            tile[even * kPitch + g * 8 + warp] = make_codes<I8, GIVEN>(make_float2(v[0][k].x, v[1][k].x), make_float2(v[2][k].x, v[3][k].x), steps[even], p.hw);
-            tile[odd * kPitch + g * 8 + warp] = make_codes<I8, GIVEN>(make_float2(v[0][k].y, v[1][k].y), make_float2(v[2][k].y, v[3][k].y), steps[odd], p.hw);
+            tile[even * kPitch + g * 8 + warp] = column_codes<I8, GIVEN>(p, make_float2(v[0][k].x, v[1][k].x), make_float2(v[2][k].x, v[3][k].x), steps[even]);
+            tile[odd * kPitch + g * 8 + warp] = column_codes<I8, GIVEN>(p, make_float2(v[0][k].y, v[1][k].y), make_float2(v[2][k].y, v[3][k].y), steps[odd]);
         }
     }
     __syncthreads();

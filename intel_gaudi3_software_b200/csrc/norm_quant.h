@@ -35,6 +35,7 @@ struct NormParams {
     float eps, per_col;    // per_col: 1 / cols
     float top;             // largest code of the 8-bit output
     Fp8HwCast hw;          // ROW_F8
+    uint32_t fp8_direct;   // no quotient of a row's own step passes the hardware conversion's limit
 };
 
 struct NormGradParams {
@@ -61,6 +62,7 @@ struct QuantTransParams {
     uint32_t row0;           // first of the rows this launch quantises (the maxima are of all)
     float top;
     Fp8HwCast hw;
+    uint32_t fp8_direct;
 };
 
 struct RowLaunch {
