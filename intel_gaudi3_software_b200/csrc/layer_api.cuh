@@ -187,20 +187,23 @@ void layer_flatten(uint32_t (&dims)[4], uint32_t* flat, std::initializer_list<Ro
     }
     *flat = n == 0;
 }
-// How many elements at once the rows of these tensors and gamma allow: eight (16 bytes of bf16 or fp32, 8 bytes of codes), two,
-// or one.
-int layer_vector(uint32_t cols, const uint32_t (&dims)[4], std::initializer_list<const RowTensor*> all, const void* gamma, const void* partial) {
-    for (const uint32_t vec : {8u, 2u}) {
-        bool fits = cols % vec == 0 && reinterpret_cast<uintptr_t>(gamma) % (vec == 8 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(partial) % (vec == 8 ? 16 : 8) == 0;
-        for (const RowTensor* t : all) {
-            if (!t->ptr) continue;
-            const uint32_t elem = t->type >= ROW_I8 ? 1 : t->type == ROW_BF16 ? 2 : 4;
-            fits = fits && reinterpret_cast<uintptr_t>(t->ptr) % std::min(16u, vec * elem) == 0;
-            for (int d = 0; d < 4; ++d) fits = fits && (dims[d] == 1 || t->stride[d] % vec == 0);
+// How the rows of these tensors and gamma lie: 8, kPhased (where `phases` allows it) or 1 (norm_quant.h).
+int layer_vector(uint32_t cols, const uint32_t (&dims)[4], std::initializer_list<const RowTensor*> all, const void* gamma, const void* partial, bool phases) {
+    bool eight = cols % 8 == 0 && reinterpret_cast<uintptr_t>(partial) % 16 == 0;
+    const RowTensor* first = *all.begin();
+    const auto elements = [](const RowTensor* t) { return reinterpret_cast<uintptr_t>(t->ptr) / (t->type >= ROW_I8 ? 1 : t->type == ROW_BF16 ? 2 : 4); };
+    for (const RowTensor* t : all) {
+        if (!t->ptr) continue;
+        eight = eight && reinterpret_cast<uintptr_t>(t->ptr) % (t->type >= ROW_I8 ? 8 : 16) == 0;
+        phases = phases && (elements(t) - elements(first)) % 8 == 0;
+        for (int d = 0; d < 4; ++d) {
+            if (dims[d] == 1) continue;
+            eight = eight && t->stride[d] % 8 == 0;
+            phases = phases && (t->stride[d] - first->stride[d]) % 8 == 0;
         }
-        if (fits) return int(vec);
     }
-    return 1;
+    if (reinterpret_cast<uintptr_t>(gamma) % 16 != 0) return 1;
+    return eight ? 8 : phases ? kPhased : 1;
 }
 RowLaunch layer_launch(const mmeb200_ctx* c) { return RowLaunch{c->device, c->sm_count, c->stream, c->tune.dependent_launch != 0}; }
 
@@ -307,7 +310,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
     p.norm = norm; p.eps = eps; p.per_col = 1.0f / float(cols); p.top = top; p.hw = hw;
     p.fp8_direct = layer_direct(out);
     p.mode = out->dtype == DT_BF16 ? NORM_BF16 : out->dtype == DT_FP32 ? NORM_F32 : out->dtype == MMEB200_INT8 ? (given ? NORM_I8_GIVEN : NORM_I8) : given ? NORM_F8_GIVEN : NORM_F8;
-    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.residual, &p.sum, &p.out}, p.gamma.ptr, nullptr);
+    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.residual, &p.sum, &p.out}, p.gamma.ptr, nullptr, true);
     CUDA_OK(c, launch_norm(layer_launch(c), p, vec));
     c->launches++;
     return st.finish();
@@ -338,7 +341,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         TRY(layer_check_vector(c, dgamma, "dgamma", cols));
     }
     if (!(eps >= 0.0f) || eps > 3.4e38f) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
-    const uint32_t blocks = norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), x->dtype == DT_FP32);
+    uint32_t blocks = norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), x->dtype == DT_FP32);
     const uint64_t need = uint64_t(blocks) * cols;
     if (workspace) {
         TRY(layer_check(c, workspace, "workspace", true, false));
@@ -387,7 +390,9 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
             p.partial = static_cast<float*>(scratch);
         }
     }
-    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.dy, &p.dsum, &p.dx}, p.gamma.ptr, p.partial);
+    const uint32_t phased = norm_grad_phased_blocks(blocks, p.rows, p.cols, x->dtype == DT_FP32);
+    const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.dy, &p.dsum, &p.dx}, p.gamma.ptr, p.partial, p.flat && p.cols % 8 != 0 && phased > 0);
+    if (vec == kPhased) blocks = phased;
     CUDA_OK(c, launch_norm_grad(layer_launch(c), p, vec, blocks));
     c->launches++;
     if (dgamma) {
@@ -435,7 +440,7 @@ int run_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, con
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     int launches = 0;
     const uint32_t dims[4] = {p.rows, 1, 1, 1};
-    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, layer_vector(p.cols, dims, {&p.x}, nullptr, nullptr), &launches));
+    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, layer_vector(p.cols, dims, {&p.x}, nullptr, nullptr, false), &launches));
     c->launches += uint64_t(launches);
     return st.finish();
 }

@@ -8,7 +8,7 @@ namespace mmeb200 {
 
 template <int XT, int RT>
 static cudaError_t norm_with(const RowLaunch& env, const NormParams& p, int vec) {
-    return vec == 8 ? norm_of<XT, RT, 8>(env, p) : vec == 2 ? norm_of<XT, RT, 2>(env, p) : norm_of<XT, RT, 1>(env, p);
+    return vec == 8 ? norm_of<XT, RT, 8>(env, p) : vec == kPhased ? norm_of<XT, RT, kPhased>(env, p) : norm_of<XT, RT, 1>(env, p);
 }
 cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec) {
     const int rt = p.residual.ptr ? p.residual.type : ROW_NONE;
@@ -24,7 +24,12 @@ uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32)
 }
 template <int XT, bool DSUM>
 static cudaError_t norm_grad_with(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
-    return vec == 8 ? norm_grad_of<XT, DSUM, 8>(env, p, blocks) : vec == 2 ? norm_grad_of<XT, DSUM, 2>(env, p, blocks) : norm_grad_of<XT, DSUM, 1>(env, p, blocks);
+    return vec == 8 ? norm_grad_of<XT, DSUM, 8>(env, p, blocks) : vec == kPhased ? norm_grad_of<XT, DSUM, kPhased>(env, p, blocks) : norm_grad_of<XT, DSUM, 1>(env, p, blocks);
+}
+// A block walks rows that are `blocks` blocks apart and keeps the sums of its columns: phased rows need a multiple of eight blocks,
+// so that a block's rows have one phase.
+uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols, bool fp32) {
+    return uint64_t(blocks) * grad_shape(cols, fp32).rows_per_block >= rows ? blocks : blocks & ~7u;
 }
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
     if (p.x.type == ROW_BF16) return p.dsum.ptr ? norm_grad_with<ROW_BF16, true>(env, p, vec, blocks) : norm_grad_with<ROW_BF16, false>(env, p, vec, blocks);
@@ -40,7 +45,7 @@ cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float
 
 template <int XT>
 static cudaError_t quant_trans_with(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
-    return vec == 8 ? quant_trans_of<XT, 8>(env, p, launches) : vec == 2 ? quant_trans_of<XT, 2>(env, p, launches) : quant_trans_of<XT, 1>(env, p, launches);
+    return vec == 8 ? quant_trans_of<XT, 8>(env, p, launches) : quant_trans_of<XT, 1>(env, p, launches);
 }
 cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
     *launches = 0;

@@ -16,61 +16,101 @@
 namespace mmeb200 {
 
 // ------------------------------------------------------------------------------------------ elements
-// A warp works on steps of 256 consecutive columns, a lane on eight of them. VEC is how many consecutive elements the length,
-// start and pitch of every row allow to be moved at once: 8 (one or two 16-byte accesses per tensor and step), 2, or 1. With
-// fewer than eight a lane's elements are chunks of VEC, 32 * VEC columns apart, so that a warp's accesses stay contiguous; the
-// arithmetic is the same eight values in registers. (Reading odd rows as aligned words and shifting those into place took more
-// instructions than the narrow accesses do: int8 rows of 4999 columns, 8192 of them, 147 us against 86 us.)
+// A warp works on steps of 256 consecutive columns, a lane on eight of them. VEC says how rows allow elements to be moved.
+// 8: every row starts and ends on eight elements, one or two 16-byte accesses per tensor and step. kPhased: rows start anywhere,
+// but the same distance (the phase) past eight elements in every tensor, as rows of an odd length that lie one behind the other do:
+// columns are counted from the boundary before the row, and all but the pieces at a row's two ends move as with 8. 1: element by
+// element, a lane's elements 32 columns apart so that a warp's accesses stay contiguous. (bf16 rows of 4999 columns to int8 with a
+// residual, 8192 of them: 61 us phased, 83 us one by one; 5000 columns take 47 us.)
 template <int TYPE>
 struct RowElem;
 template <> struct RowElem<ROW_BF16> { static constexpr int kBytes = 2; };
 template <> struct RowElem<ROW_F32> { static constexpr int kBytes = 4; };
 template <> struct RowElem<ROW_I8> { static constexpr int kBytes = 1; };   // codes of either kind
 
+// The columns of a row as its lanes count them: [phase, end).
+template <int VEC>
+struct RowSpan {
+    static constexpr uint32_t phase = 0;
+    uint32_t end;
+    __device__ __forceinline__ RowSpan(const void*, int, uint32_t cols) : end(cols) {}
+    __device__ __forceinline__ bool touches(uint32_t, uint32_t) const { return true; }
+};
+template <>
+struct RowSpan<kPhased> {
+    uint32_t phase, end;
+    __device__ __forceinline__ RowSpan(const void* row, int bytes, uint32_t cols) : phase(uint32_t(reinterpret_cast<uintptr_t>(row) / bytes) & 7u), end(cols + phase) {}
+    __device__ __forceinline__ bool whole(uint32_t c) const { return c >= phase && c + 8 <= end; }
+    __device__ __forceinline__ bool has(uint32_t c) const { return c >= phase && c < end; }
+    __device__ __forceinline__ bool touches(uint32_t c, uint32_t n) const { return c + n > phase && c < end; }
+};
+
 // Column of element e of this lane within a step.
 template <int VEC>
-__device__ __forceinline__ uint32_t lane_column(int e) { return uint32_t(e / VEC) * (32 * VEC) + (threadIdx.x & 31) * VEC + uint32_t(e % VEC); }
+__device__ __forceinline__ uint32_t lane_column(int e) { return VEC == 1 ? uint32_t(e) * 32 + (threadIdx.x & 31) : (threadIdx.x & 31) * 8 + uint32_t(e); }
 
-// Whether a lane has anything to do in the step at c0. With VEC = 8 that decides the whole piece, with fewer it is the same for
-// all lanes and the chunks are looked at one by one.
+// Whether a lane has anything to do in the step at c0. With VEC = 1 it is the same for all lanes and the elements are looked at one
+// by one.
 template <int VEC>
-__device__ __forceinline__ bool in_row(uint32_t c0, uint32_t cols) { return c0 + (VEC == 8 ? (threadIdx.x & 31) * 8 : 0) < cols; }
+__device__ __forceinline__ bool in_row(uint32_t c0, const RowSpan<VEC>& span) { return c0 + (VEC == 1 ? 0 : (threadIdx.x & 31) * 8) < span.end; }
 
-// The eight elements of a lane, packed. Columns from `c0` on (in_row); those at or past `cols` read as zeros and are not written.
+template <int TYPE>
+__device__ __forceinline__ uint32_t load_element(const uint8_t* a) {
+    if constexpr (TYPE == ROW_BF16) return *reinterpret_cast<const uint16_t*>(a);
+    else return *reinterpret_cast<const uint32_t*>(a);
+}
+template <int TYPE, int W>
+__device__ __forceinline__ void store_element(uint8_t* a, const uint32_t (&w)[W], int e) {
+    if constexpr (TYPE == ROW_F32) *reinterpret_cast<uint32_t*>(a) = w[e];
+    else if constexpr (TYPE == ROW_BF16) *reinterpret_cast<uint16_t*>(a) = uint16_t(w[e >> 1] >> (16 * (e & 1)));
+    else *a = uint8_t(w[e >> 2] >> (8 * (e & 3)));
+}
+// The eight elements of a lane, packed. Columns from `c0` on (in_row); those outside the span read as zeros, of a phased row once
+// trim_piece has cleared them: there the aligned 16 bytes around a row's ends are read whole (none without a byte of the row), so
+// that no lane goes another way while loads are issued. `row` is where column 0 would be.
 template <int TYPE, int VEC, int W>
-__device__ __forceinline__ void load_piece(const void* row, uint32_t c0, uint32_t cols, uint32_t (&w)[W]) {
+__device__ __forceinline__ void load_piece(const void* row, uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[W]) {
     constexpr int kBytes = RowElem<TYPE>::kBytes;
     static_assert(W == 2 * kBytes, "packed words");
-    const uint8_t* a = static_cast<const uint8_t*>(row) + uint64_t(c0 + lane_column<VEC>(0)) * kBytes;
-    if constexpr (VEC == 8) {
+    const uint32_t c = c0 + lane_column<VEC>(0);
+    const uint8_t* a = static_cast<const uint8_t*>(row) + uint64_t(c) * kBytes;
+    if constexpr (VEC != 1) {
 #pragma unroll
         for (int i = 0; i < W / 4; ++i) {
-            const uint4 q = reinterpret_cast<const uint4*>(a)[i];
+            uint4 q = make_uint4(0u, 0u, 0u, 0u);
+            if (VEC == 8 || span.touches(c + i * (16 / kBytes), 16 / kBytes)) q = reinterpret_cast<const uint4*>(a)[i];
             w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
         }
     } else {
-        uint32_t t[VEC == 1 && TYPE == ROW_BF16 ? 8 : W];
+        uint32_t t[8];
 #pragma unroll
-        for (int j = 0; j < 8 / VEC; ++j) {
-            const bool there = c0 + lane_column<VEC>(j * VEC) < cols;
-            const uint8_t* b = a + j * 32 * VEC * kBytes;
-            if constexpr (VEC == 1 && TYPE == ROW_BF16) t[j] = there ? uint32_t(*reinterpret_cast<const uint16_t*>(b)) : 0u;
-            else if constexpr (VEC * kBytes == 4) t[j] = there ? *reinterpret_cast<const uint32_t*>(b) : 0u;
-            else {
-                const uint2 q = there ? *reinterpret_cast<const uint2*>(b) : make_uint2(0u, 0u);
-                t[2 * j] = q.x; t[2 * j + 1] = q.y;
-            }
-        }
+        for (int e = 0; e < 8; ++e) t[e] = c + e * 32 < span.end ? load_element<TYPE>(a + e * 32 * kBytes) : 0u;
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i] = (VEC == 1 && TYPE == ROW_BF16) ? __byte_perm(t[2 * i], t[2 * i + 1], 0x5410) : t[i];
+        for (int i = 0; i < W; ++i) w[i] = TYPE == ROW_BF16 ? __byte_perm(t[2 * i % 8], t[(2 * i + 1) % 8], 0x5410) : t[i % 8];
     }
 }
 template <int TYPE, int VEC, int W>
-__device__ __forceinline__ void store_piece(void* row, uint32_t c0, uint32_t cols, const uint32_t (&w)[W]) {
+__device__ __forceinline__ void trim_piece(uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[W]) {
+    if constexpr (VEC == kPhased) {
+        const uint32_t c = c0 + lane_column<VEC>(0);
+        if (!span.whole(c)) {
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if constexpr (TYPE == ROW_BF16) w[i] &= (span.has(c + 2 * i) ? 0xFFFFu : 0u) | (span.has(c + 2 * i + 1) ? 0xFFFF0000u : 0u);
+                else w[i] = span.has(c + i) ? w[i] : 0u;
+            }
+        }
+    }
+}
+template <int TYPE, int VEC, int W>
+__device__ __forceinline__ void store_piece(void* row, uint32_t c0, const RowSpan<VEC>& span, const uint32_t (&w)[W]) {
     constexpr int kBytes = RowElem<TYPE>::kBytes;
     static_assert(W == 2 * kBytes, "packed words");
-    uint8_t* a = static_cast<uint8_t*>(row) + uint64_t(c0 + lane_column<VEC>(0)) * kBytes;
-    if constexpr (VEC == 8) {
+    const uint32_t c = c0 + lane_column<VEC>(0);
+    uint8_t* a = static_cast<uint8_t*>(row) + uint64_t(c) * kBytes;
+    bool whole = VEC == 8;
+    if constexpr (VEC == kPhased) whole = span.whole(c);
+    if (whole) {
         if constexpr (W == 2) *reinterpret_cast<uint2*>(a) = make_uint2(w[0], w[1]);
         else {
 #pragma unroll
@@ -78,16 +118,32 @@ __device__ __forceinline__ void store_piece(void* row, uint32_t c0, uint32_t col
         }
     } else {
 #pragma unroll
-        for (int j = 0; j < 8 / VEC; ++j) {
-            if (c0 + lane_column<VEC>(j * VEC) < cols) {
-                uint8_t* b = a + j * 32 * VEC * kBytes;
-                constexpr int kChunk = VEC * kBytes;
-                if constexpr (kChunk == 1) *b = uint8_t(w[j >> 2] >> (8 * (j & 3)));
-                else if constexpr (kChunk == 2) *reinterpret_cast<uint16_t*>(b) = uint16_t(w[j >> 1] >> (16 * (j & 1)));
-                else if constexpr (kChunk == 4) *reinterpret_cast<uint32_t*>(b) = w[j];
-                else *reinterpret_cast<uint2*>(b) = make_uint2(w[2 * j], w[2 * j + 1]);
-            }
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t d = lane_column<VEC>(e) - lane_column<VEC>(0);
+            bool there = c + d < span.end;
+            if constexpr (VEC == kPhased) there = span.has(c + d);
+            if (there) store_element<TYPE>(a + d * kBytes, w, e);
         }
+    }
+}
+// The same to rows that keep no phase (fp32 partial sums, counted from the row's first column).
+template <int VEC>
+__device__ __forceinline__ void store_floats(float* row, uint32_t c0, const RowSpan<VEC>& span, const uint32_t (&w)[8]) {
+    if constexpr (VEC != kPhased) store_piece<ROW_F32, VEC>(row, c0, span, w);
+    else {
+        const uint32_t c = c0 + lane_column<VEC>(0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (span.has(c + e)) reinterpret_cast<uint32_t*>(row)[c + e - span.phase] = w[e];
+    }
+}
+template <int VEC>
+__device__ __forceinline__ void load_floats(const float* row, uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[8]) {
+    if constexpr (VEC != kPhased) load_piece<ROW_F32, VEC>(row, c0, span, w);
+    else {
+        const uint32_t c = c0 + lane_column<VEC>(0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = span.has(c + e) ? reinterpret_cast<const uint32_t*>(row)[c + e - span.phase] : 0u;
     }
 }
 
@@ -116,19 +172,102 @@ __device__ __forceinline__ void pack(const float2 (&f)[4], uint32_t (&w)[W]) {
         else w[i] = pack_bf16(f[i]);
     }
 }
-// gamma is read by every row and sits in the caches; its type is a runtime value.
+// gamma is read by every row and sits in the caches; its type is a runtime value. It has no phase: a phased row's eight elements
+// are cut out of the aligned words around them. Its words are fetched a step ahead of their use, before anything of the step
+// before is stored: past a store that might be to gamma the compiler moves no load.
 template <int VEC>
-__device__ __forceinline__ void load_gamma(const RowTensor& gamma, uint32_t c0, uint32_t cols, float2 (&g)[4]) {
-    if (gamma.type == ROW_BF16) {
-        uint32_t w[4];
-        load_piece<ROW_BF16, VEC>(gamma.ptr, c0, cols, w);
-        unpack<ROW_BF16>(w, g);
+struct GammaWords { uint32_t t[VEC == kPhased ? 12 : 8]; };
+template <int TYPE, int VEC>
+__device__ __forceinline__ void fetch_gamma_of(const void* gamma, uint32_t c0, const RowSpan<VEC>& span, GammaWords<VEC>& g) {
+    constexpr int kBytes = RowElem<TYPE>::kBytes, kWord = 16 / kBytes;   // elements per 16-byte access
+    const uint8_t* base = static_cast<const uint8_t*>(gamma);
+    const uint32_t c = c0 + lane_column<VEC>(0);
+    if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g.t[e] = c + e * 32 < span.end ? load_element<TYPE>(base + uint64_t(c + e * 32) * kBytes) : 0u;
     } else {
-        uint32_t w[8];
-        load_piece<ROW_F32, VEC>(gamma.ptr, c0, cols, w);
-        unpack<ROW_F32>(w, g);
+        constexpr int kWords = (TYPE == ROW_BF16 ? 1 : 2) + (VEC == kPhased ? 1 : 0);
+        // phased: words outside the row are never used; the nearest inside stands for them
+        const int first = int(c) - int((span.phase + kWord - 1) & ~(kWord - 1u)), last = int((span.end - span.phase - 1) & ~(kWord - 1u));
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            const uint4* at = reinterpret_cast<const uint4*>(base + uint64_t(c) * kBytes) + i;
+            if constexpr (VEC == kPhased) at = reinterpret_cast<const uint4*>(base + uint64_t(uint32_t(min(max(first + i * kWord, 0), last))) * kBytes);
+            const uint4 q = *at;
+            g.t[4 * i] = q.x; g.t[4 * i + 1] = q.y; g.t[4 * i + 2] = q.z; g.t[4 * i + 3] = q.w;
+        }
     }
 }
+template <int TYPE, int VEC>
+__device__ __forceinline__ void gamma_values_of(uint32_t c0, const RowSpan<VEC>& span, const GammaWords<VEC>& g, float2 (&v)[4]) {
+    constexpr int W = 2 * RowElem<TYPE>::kBytes;
+    uint32_t w[W];
+    if constexpr (VEC == 1) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = TYPE == ROW_BF16 ? __byte_perm(g.t[2 * i % 8], g.t[(2 * i + 1) % 8], 0x5410) : g.t[i % 8];
+    } else if constexpr (VEC == 8) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = g.t[i];
+    } else {
+        constexpr uint32_t kWord = TYPE == ROW_BF16 ? 8 : 4, kUnit = TYPE == ROW_BF16 ? 2 : 1;   // elements of 16 and of 4 bytes
+        constexpr int kHave = TYPE == ROW_BF16 ? 8 : 12;
+        const uint32_t cut = (0u - span.phase) & (kWord - 1);
+        uint32_t t[kHave];
+#pragma unroll
+        for (int i = 0; i < kHave; ++i) t[i] = g.t[i];
+#pragma unroll
+        for (int step = 2; step > 0; step /= 2) {
+            const bool move = cut & (step * kUnit);
+#pragma unroll
+            for (int i = 0; i + step < kHave; ++i) t[i] = move ? t[i + step] : t[i];
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i] = TYPE == ROW_BF16 ? __funnelshift_r(t[i], t[i + 1], (cut & 1) * 16) : t[i];
+        trim_piece<TYPE, VEC>(c0, span, w);   // (a NaN there would pass into the row's maximum)
+    }
+    unpack<TYPE>(w, v);
+}
+template <int VEC>
+__device__ __forceinline__ void fetch_gamma(const RowTensor& gamma, uint32_t c0, const RowSpan<VEC>& span, GammaWords<VEC>& g) {
+    if (!in_row<VEC>(c0, span)) return;
+    if (gamma.type == ROW_BF16) fetch_gamma_of<ROW_BF16, VEC>(gamma.ptr, c0, span, g);
+    else fetch_gamma_of<ROW_F32, VEC>(gamma.ptr, c0, span, g);
+}
+template <int VEC>
+__device__ __forceinline__ void gamma_values(const RowTensor& gamma, uint32_t c0, const RowSpan<VEC>& span, const GammaWords<VEC>& g, float2 (&v)[4]) {
+    if (gamma.type == ROW_BF16) gamma_values_of<ROW_BF16, VEC>(c0, span, g, v);
+    else gamma_values_of<ROW_F32, VEC>(c0, span, g, v);
+}
+// Both at once.
+template <int TYPE, int VEC>
+__device__ __forceinline__ void load_gamma_of(const void* gamma, uint32_t c0, const RowSpan<VEC>& span, float2 (&v)[4]) {
+    GammaWords<VEC> g;
+    fetch_gamma_of<TYPE, VEC>(gamma, c0, span, g);
+    gamma_values_of<TYPE, VEC>(c0, span, g, v);
+}
+template <int VEC>
+__device__ __forceinline__ void load_gamma(const RowTensor& gamma, uint32_t c0, const RowSpan<VEC>& span, float2 (&v)[4]) {
+    if (gamma.type == ROW_BF16) load_gamma_of<ROW_BF16, VEC>(gamma.ptr, c0, span, v);
+    else load_gamma_of<ROW_F32, VEC>(gamma.ptr, c0, span, v);
+}
+// A walk over a row's steps that takes gamma from the words fetched AHEAD, or (rows that need all registers) as it goes.
+template <int VEC, bool GAMMA, bool AHEAD>
+struct GammaWalk {
+    GammaWords<VEC> words;
+    __device__ __forceinline__ GammaWalk(const RowTensor& gamma, uint32_t c, const RowSpan<VEC>& span) {
+        if constexpr (GAMMA && AHEAD) fetch_gamma<VEC>(gamma, c, span, words);
+    }
+    // h *= gamma of the step at c, where `of` is what the walk held before it went on to the next
+    static __device__ __forceinline__ void multiply(const GammaWalk& of, const RowTensor& gamma, uint32_t c, const RowSpan<VEC>& span, float2 (&h)[4]) {
+        if constexpr (GAMMA) {
+            float2 g[4];
+            if constexpr (AHEAD) gamma_values<VEC>(gamma, c, span, of.words, g);
+            else load_gamma<VEC>(gamma, c, span, g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[i] = __fmul2_rn(h[i], g[i]);
+        }
+    }
+};
 
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
     float r;
@@ -278,6 +417,10 @@ struct RowKept {
     uint32_t w[kWords];
     __device__ __forceinline__ void values(float2 (&h)[4]) const { unpack<kType>(w, h); }
 };
+// Or, for codes of rows that leave registers enough, the finished products h * gamma: gamma is then read once per row.
+struct RowProducts {
+    float2 v[4];
+};
 // x + residual, rounded to the stream's type, which is what the norm sees.
 template <int XT, int RT>
 __device__ __forceinline__ void stream_values(const uint32_t (&x)[2 * RowElem<XT>::kBytes], const uint32_t (&r)[2 * RowElem<RT>::kBytes], RowKept<XT, RT>& h) {
@@ -288,74 +431,76 @@ __device__ __forceinline__ void stream_values(const uint32_t (&x)[2 * RowElem<XT
     for (int i = 0; i < 4; ++i) f[i] = __fadd2_rn(f[i], g[i]);
     pack<RT>(f, h.w);
 }
-// The rows of a norm's tensors.
-template <int XT, int RT>
+// The rows of a norm's tensors, each from where column 0 would be.
+template <int XT, int RT, int VEC>
 struct NormRows {
     const uint8_t *x, *residual;
     uint8_t* sum;
-    __device__ __forceinline__ NormRows(const NormParams& p, uint32_t row) {
-        x = row_of<XT>(p.x, row, p.dims, p.flat);
+    RowSpan<VEC> span;
+    __device__ __forceinline__ NormRows(const NormParams& p, uint32_t row) : x(row_of<XT>(p.x, row, p.dims, p.flat)), span(x, RowElem<XT>::kBytes, p.cols) {
+        x -= span.phase * RowElem<XT>::kBytes;
         if constexpr (RT != ROW_NONE) {
-            residual = row_of<RT>(p.residual, row, p.dims, p.flat);
-            sum = p.sum.ptr ? row_of<RT>(p.sum, row, p.dims, p.flat) : nullptr;
+            residual = row_of<RT>(p.residual, row, p.dims, p.flat) - span.phase * RowElem<RT>::kBytes;
+            sum = p.sum.ptr ? row_of<RT>(p.sum, row, p.dims, p.flat) - span.phase * RowElem<RT>::kBytes : nullptr;
         }
     }
 };
 // COUNT steps of the first pass from column c0 on: all loads first, then the stream's values (kept, and written), then the sums.
-template <int XT, int RT, int VEC, int COUNT>
-__device__ __forceinline__ void read_steps(const NormParams& p, const NormRows<XT, RT>& rows, uint32_t c0, bool tops, RowKept<XT, RT>* kept, float2& sum, float& top) {
+// TOPS: the largest |h * gamma| too. Kept: RowKept or RowProducts.
+template <int XT, int RT, int VEC, int COUNT, bool TOPS, bool GAMMA, bool AHEAD, typename Kept>
+__device__ __forceinline__ void read_steps(const NormParams& p, const NormRows<XT, RT, VEC>& rows, uint32_t c0, Kept* kept, float2& sum, float& top) {
     constexpr int WX = 2 * RowElem<XT>::kBytes, WR = RT != ROW_NONE ? 2 * RowElem<RT != ROW_NONE ? RT : XT>::kBytes : 1;
     uint32_t x[COUNT][WX], r[COUNT][WR];
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) {
-        if (in_row<VEC>(c0 + j * 256, p.cols)) {
-            load_piece<XT, VEC>(rows.x, c0 + j * 256, p.cols, x[j]);
-            if constexpr (RT != ROW_NONE) load_piece<RT, VEC>(rows.residual, c0 + j * 256, p.cols, r[j]);
+        if (in_row<VEC>(c0 + j * 256, rows.span)) {
+            load_piece<XT, VEC>(rows.x, c0 + j * 256, rows.span, x[j]);
+            if constexpr (RT != ROW_NONE) load_piece<RT, VEC>(rows.residual, c0 + j * 256, rows.span, r[j]);
         }
     }
+    using Walk = GammaWalk<VEC, TOPS && GAMMA, AHEAD>;
+    Walk gamma(p.gamma, c0, rows.span);
 #pragma unroll
     for (int j = 0; j < COUNT; ++j) {
         const uint32_t c = c0 + j * 256;
-        if (in_row<VEC>(c, p.cols)) {
+        const Walk now = gamma;
+        if (j + 1 < COUNT) gamma = Walk(p.gamma, c + 256, rows.span);
+        if (in_row<VEC>(c, rows.span)) {
+            RowKept<XT, RT> stream;
+            trim_piece<XT, VEC>(c, rows.span, x[j]);
             if constexpr (RT != ROW_NONE) {
-                stream_values<XT, RT>(x[j], r[j], kept[j]);
-                if (rows.sum) store_piece<RT, VEC>(rows.sum, c, p.cols, kept[j].w);
+                trim_piece<RT, VEC>(c, rows.span, r[j]);
+                stream_values<XT, RT>(x[j], r[j], stream);
+                if (rows.sum) store_piece<RT, VEC>(rows.sum, c, rows.span, stream.w);
             } else {
 #pragma unroll
-                for (int i = 0; i < WX; ++i) kept[j].w[i] = x[j][i];
+                for (int i = 0; i < WX; ++i) stream.w[i] = x[j][i];
             }
             float2 h[4];
-            kept[j].values(h);
+            stream.values(h);
             if (p.norm) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum = __ffma2_rn(h[i], h[i], sum);
             }
-            if (tops) {
-                if (p.gamma.ptr) {
-                    float2 g[4];
-                    load_gamma<VEC>(p.gamma, c, p.cols, g);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) h[i] = __fmul2_rn(h[i], g[i]);
-                }
+            if constexpr (TOPS) {
+                Walk::multiply(now, p.gamma, c, rows.span, h);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = max_nan(top, fabsf(h[i].x), fabsf(h[i].y));
+            }
+            if constexpr (std::is_same_v<Kept, RowProducts>) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kept[j].v[i] = h[i];
+            } else {
+                kept[j] = stream;
             }
         }
     }
 }
-// One step of the second pass: the finished values, as floats or codes.
-template <int MODE, bool FAST, int VEC, int XT, int RT>
-__device__ __forceinline__ void write_step(const NormParams& p, uint8_t* out, uint32_t c, const RowKept<XT, RT>& kept, const RowFactors& f) {
+// One step of the second pass: the finished values v (h * gamma), as floats or codes.
+template <int MODE, bool FAST, int VEC>
+__device__ __forceinline__ void write_values(const NormParams& p, uint8_t* out, uint32_t c, const RowSpan<VEC>& span, float2 (&v)[4], const RowFactors& f) {
     constexpr int kType = MODE == NORM_BF16 ? ROW_BF16 : MODE == NORM_F32 ? ROW_F32 : ROW_I8;
-    float2 v[4];
     uint32_t w[2 * RowElem<kType>::kBytes];
-    kept.values(v);
-    if (p.gamma.ptr) {
-        float2 g[4];
-        load_gamma<VEC>(p.gamma, c, p.cols, g);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __fmul2_rn(v[i], g[i]);
-    }
     if constexpr (MODE != NORM_I8 && MODE != NORM_F8) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = __fmul2_rn(v[k], both(f.inv));
@@ -365,61 +510,88 @@ __device__ __forceinline__ void write_step(const NormParams& p, uint8_t* out, ui
 #pragma unroll
         for (int k = 0; k < 2; ++k) w[k] = make_codes<MODE == NORM_I8 || MODE == NORM_I8_GIVEN, FAST>(v[2 * k], v[2 * k + 1], f.step, p.hw);
     }
-    store_piece<kType, VEC>(out, c, p.cols, w);
+    store_piece<kType, VEC>(out, c, span, w);
+}
+template <int MODE, bool FAST, int VEC, int COUNT, bool GAMMA, bool AHEAD, typename Kept>
+__device__ __forceinline__ void write_steps(const NormParams& p, uint8_t* out, uint32_t c0, const RowSpan<VEC>& span, const Kept* kept, const RowFactors& f) {
+    constexpr bool kProducts = std::is_same_v<Kept, RowProducts>;
+    using Walk = GammaWalk<VEC, !kProducts && GAMMA, AHEAD>;
+    Walk gamma(p.gamma, c0, span);
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+        const uint32_t c = c0 + i * 256;
+        const Walk now = gamma;
+        if (i + 1 < COUNT) gamma = Walk(p.gamma, c + 256, span);
+        if (in_row<VEC>(c, span)) {
+            float2 v[4];
+            if constexpr (kProducts) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = kept[i].v[k];
+            } else {
+                kept[i].values(v);
+                Walk::multiply(now, p.gamma, c, span, v);
+            }
+            write_values<MODE, FAST, VEC>(p, out, c, span, v, f);
+        }
+    }
 }
 // What differs between the kinds of output is decided once per row: `write(mode, fast)` is called with the kind as a constant,
 // and whether the row's codes can do without a test of the step.
-template <typename F>
+template <bool CODES, typename F>   // CODES: of the row's own step
 __device__ __forceinline__ void for_mode(const NormParams& p, const RowFactors& f, F&& write) {
-    switch (p.mode) {
-        case NORM_BF16: write(std::integral_constant<int, NORM_BF16>(), std::false_type()); break;
-        case NORM_F32: write(std::integral_constant<int, NORM_F32>(), std::false_type()); break;
-        case NORM_I8:
+    if constexpr (CODES) {
+        if (p.mode == NORM_I8) {
             if (fast_step(f.step, true)) write(std::integral_constant<int, NORM_I8>(), std::true_type());
             else write(std::integral_constant<int, NORM_I8>(), std::false_type());
-            break;
-        case NORM_F8:
+        } else {
             if (fast_step(f.step, p.fp8_direct)) write(std::integral_constant<int, NORM_F8>(), std::true_type());
             else write(std::integral_constant<int, NORM_F8>(), std::false_type());
-            break;
-        case NORM_I8_GIVEN: write(std::integral_constant<int, NORM_I8_GIVEN>(), std::false_type()); break;
-        default: write(std::integral_constant<int, NORM_F8_GIVEN>(), std::false_type()); break;
+        }
+    } else {
+        switch (p.mode) {
+            case NORM_BF16: write(std::integral_constant<int, NORM_BF16>(), std::false_type()); break;
+            case NORM_F32: write(std::integral_constant<int, NORM_F32>(), std::false_type()); break;
+            case NORM_I8_GIVEN: write(std::integral_constant<int, NORM_I8_GIVEN>(), std::false_type()); break;
+            default: write(std::integral_constant<int, NORM_F8_GIVEN>(), std::false_type()); break;
+        }
     }
 }
-__device__ __forceinline__ uint8_t* out_row(const NormParams& p, uint32_t row) {
-    return static_cast<uint8_t*>(p.out.ptr) + row_offset(p.out, row, p.dims, p.flat) * (p.mode == NORM_BF16 ? 2 : p.mode == NORM_F32 ? 4 : 1);
+__device__ __forceinline__ uint8_t* out_row(const NormParams& p, uint32_t row, uint32_t phase) {
+    return static_cast<uint8_t*>(p.out.ptr) + (row_offset(p.out, row, p.dims, p.flat) - phase) * (p.mode == NORM_BF16 ? 2 : p.mode == NORM_F32 ? 4 : 1);
 }
 
 // A row per warp (BLOCK = false: four rows per block) or per block, NV steps per warp, kept in registers between the row's one
 // read and its one write. Two blocks of 512 threads fit an SM where rows are kept in bf16.
 template <int XT, int RT, int VEC, int NV, bool BLOCK, int THREADS>
 __global__ void __launch_bounds__(THREADS, THREADS == 512 && RowKept<XT, RT>::kType == ROW_BF16 ? 2 : 1) norm_kernel(const __grid_constant__ NormParams p) {
-    constexpr int G = NV < 2 ? 1 : (VEC == 8 && XT != ROW_F32 && RT != ROW_F32) ? 4 : 2;   // steps loaded at a time
+    constexpr int G = NV < 2 ? 1 : (VEC != 1 && RT == ROW_NONE) ? NV : (VEC != 1 && XT != ROW_F32 && RT != ROW_F32) ? 4 : 2;   // steps loaded at a time
     __shared__ float2 scratch[32];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t row = BLOCK ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 5);
     if (row >= p.rows) return;   // whole warps, never part of a block that synchronises
     const uint32_t c0 = BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0;
-    RowKept<XT, RT> kept[NV];
-    float2 sum = both(0.0f);
-    float top = 0.0f;
-    const NormRows<XT, RT> rows(p, row);
-    auto read = [&](auto tops) {
+    const NormRows<XT, RT, VEC> rows(p, row);
+    auto whole_row = [&](auto codes, auto gamma) {
+        constexpr bool kCodes = decltype(codes)::value, kGamma = decltype(gamma)::value, kAhead = NV <= 4;
+        std::conditional_t<kCodes && NV <= 4, RowProducts, RowKept<XT, RT>> kept[NV];
+        float2 sum = both(0.0f);
+        float top = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i += G) read_steps<XT, RT, VEC, G>(p, rows, c0 + i * 256, decltype(tops)::value, kept + i, sum, top);
+        for (int i = 0; i < NV; i += G) read_steps<XT, RT, VEC, G, kCodes, kGamma, kAhead>(p, rows, c0 + i * 256, kept + i, sum, top);
+        const float2 s = reduce_row<BLOCK, true>(sum.x + sum.y, top, blockDim.x >> 5, scratch);
+        const RowFactors f = row_factors(p, s.x, s.y, row);
+        if (p.scale && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) p.scale[row] = f.scale;
+        uint8_t* out = out_row(p, row, rows.span.phase);
+        for_mode<kCodes>(p, f, [&](auto mode, auto fast) { write_steps<decltype(mode)::value, decltype(fast)::value, VEC, NV, kGamma, kAhead>(p, out, c0, rows.span, kept, f); });
     };
-    if (p.mode == NORM_I8 || p.mode == NORM_F8) read(std::true_type());
-    else read(std::false_type());
-    const float2 s = reduce_row<BLOCK, true>(sum.x + sum.y, top, blockDim.x >> 5, scratch);
-    const RowFactors f = row_factors(p, s.x, s.y, row);
-    if (p.scale && (BLOCK ? threadIdx.x : threadIdx.x & 31) == 0) p.scale[row] = f.scale;
-    uint8_t* out = out_row(p, row);
-    for_mode(p, f, [&](auto mode, auto fast) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-            if (in_row<VEC>(c0 + i * 256, p.cols)) write_step<decltype(mode)::value, decltype(fast)::value, VEC>(p, out, c0 + i * 256, kept[i], f);
-    });
+    if (p.mode == NORM_I8 || p.mode == NORM_F8) {
+        if (p.gamma.ptr) whole_row(std::true_type(), std::true_type());
+        else whole_row(std::true_type(), std::false_type());
+    } else {
+        if (p.gamma.ptr) whole_row(std::false_type(), std::true_type());
+        else whole_row(std::false_type(), std::false_type());
+    }
 }
 
 // Rows too long for registers: the row is read a second time (from L2, mostly) once its sums are known. The second read
@@ -432,36 +604,45 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t row = blockIdx.x, first = (threadIdx.x >> 5) * 256;
-    const bool tops = p.mode == NORM_I8 || p.mode == NORM_F8;
-    const NormRows<XT, RT> rows(p, row);
-    float2 sum = both(0.0f);
-    float top = 0.0f;
+    const NormRows<XT, RT, VEC> rows(p, row);
+    auto whole_row = [&](auto codes, auto gamma) {
+        constexpr bool kCodes = decltype(codes)::value, kGamma = decltype(gamma)::value;
+        float2 sum = both(0.0f);
+        float top = 0.0f;
 #pragma unroll 1
-    for (uint32_t c = first; in_row<VEC>(c, p.cols); c += 32 * 256) {
-        RowKept<XT, RT> kept;
-        read_steps<XT, RT, VEC, 1>(p, rows, c, tops, &kept, sum, top);
-    }
-    const float2 s = reduce_row<true, true>(sum.x + sum.y, top, 32, scratch);
-    const RowFactors f = row_factors(p, s.x, s.y, row);
-    if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
-    uint8_t* out = out_row(p, row);
-    for_mode(p, f, [&](auto mode, auto fast) {
-#pragma unroll 1
-        for (uint32_t c = first; in_row<VEC>(c, p.cols); c += 32 * 256) {
+        for (uint32_t c = first; in_row<VEC>(c, rows.span); c += 32 * 256) {
             RowKept<XT, RT> kept;
-            if constexpr (RT == ROW_NONE) {
-                load_piece<XT, VEC>(rows.x, c, p.cols, kept.w);
-            } else if (rows.sum) {
-                load_piece<KT, VEC>(rows.sum, c, p.cols, kept.w);
-            } else {
-                uint32_t x[2 * RowElem<XT>::kBytes], r[2 * RowElem<RT != ROW_NONE ? RT : XT>::kBytes];
-                load_piece<XT, VEC>(rows.x, c, p.cols, x);
-                load_piece<RT, VEC>(rows.residual, c, p.cols, r);
-                stream_values<XT, RT>(x, r, kept);
-            }
-            write_step<decltype(mode)::value, decltype(fast)::value, VEC>(p, out, c, kept, f);
+            read_steps<XT, RT, VEC, 1, kCodes, kGamma, true>(p, rows, c, &kept, sum, top);
         }
-    });
+        const float2 s = reduce_row<true, true>(sum.x + sum.y, top, 32, scratch);
+        const RowFactors f = row_factors(p, s.x, s.y, row);
+        if (p.scale && threadIdx.x == 0) p.scale[row] = f.scale;
+        uint8_t* out = out_row(p, row, rows.span.phase);
+        for_mode<kCodes>(p, f, [&](auto mode, auto fast) {
+#pragma unroll 1
+            for (uint32_t c = first; in_row<VEC>(c, rows.span); c += 32 * 256) {
+                RowKept<XT, RT> kept;
+                if constexpr (RT == ROW_NONE) {
+                    load_piece<XT, VEC>(rows.x, c, rows.span, kept.w);
+                } else if (rows.sum) {
+                    load_piece<KT, VEC>(rows.sum, c, rows.span, kept.w);
+                } else {
+                    uint32_t x[2 * RowElem<XT>::kBytes], r[2 * RowElem<RT != ROW_NONE ? RT : XT>::kBytes];
+                    load_piece<XT, VEC>(rows.x, c, rows.span, x);
+                    load_piece<RT, VEC>(rows.residual, c, rows.span, r);
+                    stream_values<XT, RT>(x, r, kept);
+                }
+                write_steps<decltype(mode)::value, decltype(fast)::value, VEC, 1, kGamma, true>(p, out, c, rows.span, &kept, f);
+            }
+        });
+    };
+    if (p.mode == NORM_I8 || p.mode == NORM_F8) {
+        if (p.gamma.ptr) whole_row(std::true_type(), std::true_type());
+        else whole_row(std::true_type(), std::false_type());
+    } else {
+        if (p.gamma.ptr) whole_row(std::false_type(), std::true_type());
+        else whole_row(std::false_type(), std::false_type());
+    }
 }
 
 // ------------------------------------------------------------------------------------------ gradient
@@ -482,9 +663,9 @@ __device__ __forceinline__ void grad_piece(const float2 (&x)[4], const float2 (&
     }
 }
 template <int VEC>
-__device__ __forceinline__ void grad_scale(const NormGradParams& p, const float2 (&y)[4], uint32_t c, float2 (&a)[4]) {
+__device__ __forceinline__ void grad_scale(const NormGradParams& p, const float2 (&y)[4], uint32_t c, const RowSpan<VEC>& span, float2 (&a)[4]) {
     if (p.gamma.ptr) {
-        load_gamma<VEC>(p.gamma, c, p.cols, a);
+        load_gamma<VEC>(p.gamma, c, span, a);
 #pragma unroll
         for (int k = 0; k < 4; ++k) a[k] = __fmul2_rn(a[k], y[k]);
     } else {
@@ -501,11 +682,14 @@ __device__ __forceinline__ void sum_grad(const float2 (&x)[4], const float2 (&a)
 }
 // A lane's eight sums of dgamma to the block's row of `partial`.
 template <int VEC>
-__device__ __forceinline__ void store_sums(float* mine, uint32_t c, uint32_t cols, const float2 (&acc)[4]) {
+__device__ __forceinline__ void store_sums(float* mine, uint32_t c, const RowSpan<VEC>& span, const float2 (&acc)[4]) {
     uint32_t w[8];
     pack<ROW_F32>(acc, w);
-    store_piece<ROW_F32, VEC>(mine, c, cols, w);
+    store_floats<VEC>(mine, c, span, w);
 }
+// The span of a block's (or warp's) rows: all of them have the first one's phase (launch_norm_grad).
+template <int XT, int VEC>
+__device__ __forceinline__ RowSpan<VEC> grad_span(const NormGradParams& p, uint32_t row) { return RowSpan<VEC>(row_of<XT>(p.x, row, p.dims, p.flat), RowElem<XT>::kBytes, p.cols); }
 // XT: type of x, dy, dsum and dx; DSUM: whether there is a gradient of the sum. A row per warp or per block, as in norm_kernel.
 template <int XT, bool DSUM, int VEC, int NV, bool BLOCK, int THREADS>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
@@ -520,27 +704,31 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[i][k] = both(0.0f);
+    const RowSpan<VEC> span = grad_span<XT, VEC>(p, blockIdx.x * kRowsPerBlock + sub);
+    const uint32_t shift = span.phase * RowElem<XT>::kBytes;
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x * kRowsPerBlock + sub; row < p.rows; row += gridDim.x * kRowsPerBlock, turn ^= 1) {
-        const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat), *yr = row_of<XT>(p.dy, row, p.dims, p.flat);
-        const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) : nullptr;
+        const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat) - shift, *yr = row_of<XT>(p.dy, row, p.dims, p.flat) - shift;
+        const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) - shift : nullptr;
         uint32_t xs[NV][W], ys[NV][W], ds[DSUM ? NV : 1][W];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, p.cols)) {
-                load_piece<XT, VEC>(xr, c0 + i * 256, p.cols, xs[i]);
-                load_piece<XT, VEC>(yr, c0 + i * 256, p.cols, ys[i]);
-                if constexpr (DSUM) load_piece<XT, VEC>(sr, c0 + i * 256, p.cols, ds[i]);
+            if (in_row<VEC>(c0 + i * 256, span)) {
+                load_piece<XT, VEC>(xr, c0 + i * 256, span, xs[i]);
+                load_piece<XT, VEC>(yr, c0 + i * 256, span, ys[i]);
+                if constexpr (DSUM) load_piece<XT, VEC>(sr, c0 + i * 256, span, ds[i]);
             }
         }
         float2 squares = both(0.0f), dot = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, p.cols)) {
+            if (in_row<VEC>(c0 + i * 256, span)) {
                 float2 x[4], y[4], a[4];
+                trim_piece<XT, VEC>(c0 + i * 256, span, xs[i]);
+                trim_piece<XT, VEC>(c0 + i * 256, span, ys[i]);
                 unpack<XT>(xs[i], x);
                 unpack<XT>(ys[i], y);
-                grad_scale<VEC>(p, y, c0 + i * 256, a);
+                grad_scale<VEC>(p, y, c0 + i * 256, span, a);
                 sum_grad(x, a, squares, dot);
             }
         }
@@ -548,19 +736,19 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const
         const float2 s = reduce_row<BLOCK, false>(squares.x + squares.y, dot.x + dot.y, blockDim.x >> 5, scratch[turn]);
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
-        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat);
+        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat) - shift;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, p.cols)) {
+            if (in_row<VEC>(c0 + i * 256, span)) {
                 float2 x[4], y[4], a[4], add[4];
                 unpack<XT>(xs[i], x);
                 unpack<XT>(ys[i], y);
                 if constexpr (DSUM) unpack<XT>(ds[i], add);
-                grad_scale<VEC>(p, y, c0 + i * 256, a);
+                grad_scale<VEC>(p, y, c0 + i * 256, span, a);
                 grad_piece<DSUM>(x, y, a, add, inv, mean_au, acc[i]);
                 uint32_t w[W];
                 pack<XT>(a, w);
-                store_piece<XT, VEC>(out, c0 + i * 256, p.cols, w);
+                store_piece<XT, VEC>(out, c0 + i * 256, span, w);
             }
         }
     }
@@ -574,7 +762,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const
                 for (int i = 0; i < NV; ++i)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const uint32_t c = i * 256 + lane_column<VEC>(e);
+                        const uint32_t c = i * 256 + lane_column<VEC>(e) - span.phase;   // (below the phase: past any column)
                         const float v = (e & 1) ? acc[i][e >> 1].y : acc[i][e >> 1].x;
                         if (c < p.cols) block_sums[c] = w ? block_sums[c] + v : v;
                     }
@@ -585,7 +773,7 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const
     } else {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (in_row<VEC>(c0 + i * 256, p.cols)) store_sums<VEC>(mine, c0 + i * 256, p.cols, acc[i]);
+            if (in_row<VEC>(c0 + i * 256, span)) store_sums<VEC>(mine, c0 + i * 256, span, acc[i]);
     }
 }
 // Longer rows, walked by a loop. KEEP: x and dy are kept in shared memory between the two passes, and so are the sums of dgamma,
@@ -601,10 +789,12 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
     uint4* keep = grad_smem + threadIdx.x;                                                       // [step][16-byte word of x, then dy][thread]
     float4* sums = reinterpret_cast<float4*>(grad_smem + steps * 2 * Q * threads) + threadIdx.x;   // [step][half of the eight][thread]
     float* mine = p.partial ? p.partial + uint64_t(blockIdx.x) * p.cols : nullptr;
+    const RowSpan<VEC> span = grad_span<XT, VEC>(p, blockIdx.x);
+    const uint32_t shift = span.phase * RowElem<XT>::kBytes;
     uint32_t turn = 0;
     for (uint32_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat), *yr = row_of<XT>(p.dy, row, p.dims, p.flat);
-        const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) : nullptr;
+        const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat) - shift, *yr = row_of<XT>(p.dy, row, p.dims, p.flat) - shift;
+        const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) - shift : nullptr;
         float2 squares = both(0.0f), dot = both(0.0f);
 #pragma unroll 1
         for (uint32_t i0 = 0; i0 < steps; i0 += 2) {
@@ -612,15 +802,17 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
 #pragma unroll
             for (uint32_t j = 0; j < 2; ++j) {
                 const uint32_t c = first + (i0 + j) * 256;
-                if (i0 + j < steps && in_row<VEC>(c, p.cols)) {
-                    load_piece<XT, VEC>(xr, c, p.cols, xw[j]);
-                    load_piece<XT, VEC>(yr, c, p.cols, yw[j]);
+                if (i0 + j < steps && in_row<VEC>(c, span)) {
+                    load_piece<XT, VEC>(xr, c, span, xw[j]);
+                    load_piece<XT, VEC>(yr, c, span, yw[j]);
                 }
             }
 #pragma unroll
             for (uint32_t j = 0; j < 2; ++j) {
                 const uint32_t i = i0 + j, c = first + i * 256;
-                if (i < steps && in_row<VEC>(c, p.cols)) {
+                if (i < steps && in_row<VEC>(c, span)) {
+                    trim_piece<XT, VEC>(c, span, xw[j]);
+                    trim_piece<XT, VEC>(c, span, yw[j]);
                     if constexpr (KEEP) {
 #pragma unroll
                         for (int k = 0; k < Q; ++k) {
@@ -631,7 +823,7 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
                     float2 x[4], y[4], a[4];
                     unpack<XT>(xw[j], x);
                     unpack<XT>(yw[j], y);
-                    grad_scale<VEC>(p, y, c, a);
+                    grad_scale<VEC>(p, y, c, span, a);
                     sum_grad(x, a, squares, dot);
                 }
             }
@@ -640,15 +832,15 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
         const bool begin = row == blockIdx.x;
-        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat);
+        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat) - shift;
 #pragma unroll 1
         for (uint32_t i = 0; i < steps; ++i) {
             const uint32_t c = first + i * 256;
-            if (!in_row<VEC>(c, p.cols)) break;
+            if (!in_row<VEC>(c, span)) break;
             uint32_t xw[W], yw[W], w[W];
             float2 x[4], y[4], a[4], add[4], acc[4];
             if constexpr (DSUM) {
-                load_piece<XT, VEC>(sr, c, p.cols, w);
+                load_piece<XT, VEC>(sr, c, span, w);
                 unpack<XT>(w, add);
             }
             if constexpr (KEEP) {
@@ -659,12 +851,12 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
                     yw[4 * k] = u.x; yw[4 * k + 1] = u.y; yw[4 * k + 2] = u.z; yw[4 * k + 3] = u.w;
                 }
             } else {
-                load_piece<XT, VEC>(xr, c, p.cols, xw);
-                load_piece<XT, VEC>(yr, c, p.cols, yw);
+                load_piece<XT, VEC>(xr, c, span, xw);
+                load_piece<XT, VEC>(yr, c, span, yw);
             }
             unpack<XT>(xw, x);
             unpack<XT>(yw, y);
-            grad_scale<VEC>(p, y, c, a);
+            grad_scale<VEC>(p, y, c, span, a);
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[k] = both(0.0f);
             if (mine && !begin) {
@@ -674,7 +866,7 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
                     acc[2] = make_float2(u.x, u.y); acc[3] = make_float2(u.z, u.w);
                 } else {
                     uint32_t t[8];
-                    load_piece<ROW_F32, VEC>(mine, c, p.cols, t);
+                    load_floats<VEC>(mine, c, span, t);
                     unpack<ROW_F32>(t, acc);
                 }
             }
@@ -684,20 +876,20 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
                     sums[(i * 2) * threads] = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
                     sums[(i * 2 + 1) * threads] = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
                 } else {
-                    store_sums<VEC>(mine, c, p.cols, acc);
+                    store_sums<VEC>(mine, c, span, acc);
                 }
             }
             pack<XT>(a, w);
-            store_piece<XT, VEC>(out, c, p.cols, w);
+            store_piece<XT, VEC>(out, c, span, w);
         }
     }
     if constexpr (KEEP) {
         if (mine) {
 #pragma unroll 1
-            for (uint32_t i = 0; i < steps && in_row<VEC>(first + i * 256, p.cols); ++i) {
+            for (uint32_t i = 0; i < steps && in_row<VEC>(first + i * 256, span); ++i) {
                 const float4 t = sums[(i * 2) * threads], u = sums[(i * 2 + 1) * threads];
                 const float2 acc[4] = {make_float2(t.x, t.y), make_float2(t.z, t.w), make_float2(u.x, u.y), make_float2(u.z, u.w)};
-                store_sums<VEC>(mine, first + i * 256, p.cols, acc);
+                store_sums<VEC>(mine, first + i * 256, span, acc);
             }
         }
     }
@@ -730,12 +922,7 @@ __device__ __forceinline__ void column_sums(const float* partial, float* out, ui
 template <int VEC>
 __device__ __forceinline__ uint32_t slot_column(uint32_t slot) {
     const uint32_t e = slot >> 5, lane = slot & 31;
-    return (e / VEC) * (32 * VEC) + lane * VEC + e % VEC;
-}
-template <int VEC>
-__device__ __forceinline__ uint32_t column_slot(uint32_t c) {
-    const uint32_t chunk = c / (32 * VEC), in = c % (32 * VEC);
-    return (chunk * VEC + in % VEC) * 32 + in / VEC;
+    return VEC == 1 ? e * 32 + lane : lane * 8 + e;
 }
 template <int XT>
 __device__ __forceinline__ const uint8_t* trans_row(const QuantTransParams& p, uint32_t row) {
@@ -752,13 +939,14 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
     float2 top[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) top[k] = both(0.0f);
-    const bool there = in_row<VEC>(c0, p.cols);
+    const RowSpan<VEC> span(nullptr, 1, p.cols);
+    const bool there = in_row<VEC>(c0, span);
 #pragma unroll 1
     for (uint32_t r = r0 + warp; r < r1; r += 32) {
         uint32_t x[4][W];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (there && r + 8 * j < r1) load_piece<XT, VEC>(trans_row<XT>(p, r + 8 * j), c0, p.cols, x[j]);
+            if (there && r + 8 * j < r1) load_piece<XT, VEC>(trans_row<XT>(p, r + 8 * j), c0, span, x[j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (there && r + 8 * j < r1) {
@@ -801,6 +989,7 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
         steps[threadIdx.x] = make_code_step(s);
     }
     __syncthreads();
+    const RowSpan<VEC> span(nullptr, 1, p.cols);
 #pragma unroll 1
     for (uint32_t g = 0; g < kTransRows / 32; ++g) {
         const uint32_t r = r0 + g * 32 + warp * 4;
@@ -808,7 +997,7 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
         float2 v[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (in_row<VEC>(c0, p.cols) && r + j < p.rows) load_piece<XT, VEC>(trans_row<XT>(p, p.row0 + r + j), c0, p.cols, x[j]);
+            if (in_row<VEC>(c0, span) && r + j < p.rows) load_piece<XT, VEC>(trans_row<XT>(p, p.row0 + r + j), c0, span, x[j]);
             else {
 #pragma unroll
                 for (int k = 0; k < W; ++k) x[j][k] = 0;
@@ -825,14 +1014,18 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
     }
     __syncthreads();
     const uint32_t rows = min(kTransRows, p.rows - r0), cols = min(256u, p.cols - c0);
-    // nine 16-byte words cover a column's 128 bytes at any alignment
-    for (uint32_t i = threadIdx.x; i < cols * 9; i += 256) {
-        const uint32_t col = i / 9, k = i % 9;
+    // nine 16-byte words cover a column's 128 bytes at any alignment, eight where they are aligned; neighbouring lanes take
+    // neighbouring slots, whose words lie in different banks
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.out) + p.row0 + r0) | p.out_ld) % 16 == 0;
+    const uint32_t words = aligned ? 8 : 9;
+    for (uint32_t i = threadIdx.x; i < 256 * words; i += 256) {
+        const uint32_t slot = aligned ? i / 8 : i / 9, k = i - slot * words, col = slot_column<VEC>(slot);
+        if (col >= cols) continue;
         uint8_t* a = static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0;
         const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u;
         const int begin = int(16 * k) - int(off);   // first row of the word
         if (begin >= int(rows)) continue;
-        const uint32_t* column = tile + column_slot<VEC>(col) * kPitch;
+        const uint32_t* column = tile + slot * kPitch;
         if (begin >= 0 && begin + 16 <= int(rows)) {
             const uint32_t w0 = uint32_t(begin) >> 2, sh = (uint32_t(begin) & 3u) * 8;
             uint32_t w[5], o[4];

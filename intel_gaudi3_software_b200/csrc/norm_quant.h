@@ -71,10 +71,14 @@ struct RowLaunch {
     bool dependent_launch;
 };
 
-// `vec` (8, 2 or 1): the length, start and pitch of every row of every tensor, gamma included, allow accesses of so many elements.
+// How the rows of a call's tensors lie (`vec`): 8, every row of every tensor, and its end, on eight elements; kPhased, a row of
+// every tensor equally far past eight elements (gamma on 16 bytes); 1, anything.
+constexpr int kPhased = 0;
 cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec);
 // Blocks the gradient kernel runs with, i.e. rows of `partial`.
 uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32);
+// Of those, the blocks that phased rows can use (0: none).
+uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols, bool fp32);
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks);
 cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols);
 // Number of kernels launched is returned in *launches.

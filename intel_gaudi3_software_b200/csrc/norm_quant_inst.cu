@@ -1,6 +1,6 @@
 // Instantiations of the row kernels and their launchers. The Makefile compiles this file once per variant with -DINST_XT=<1|2>
-// -DINST_VEC=<8|2|1> (element type of x, elements moved at once) and one of -DINST_NORM=<0|1|2> (element type of the residual),
-// -DINST_GRAD=<0|1> (with a gradient of the sum) and -DINST_TRANS.
+// -DINST_VEC=<8|0|1> (element type of x, how rows lie: 0 is kPhased) and one of -DINST_NORM=<0|1|2> (element type of the residual),
+// -DINST_GRAD=<0|1> (with a gradient of the sum) and -DINST_TRANS (not for kPhased).
 #include <algorithm>
 
 #include "norm_quant.cuh"
@@ -14,11 +14,12 @@ namespace mmeb200 {
 // the loads in flight to cover the latency of HBM and for the row's reduction to be a small part of the work.
 template <int XT, int RT, int VEC>
 cudaError_t norm_of(const RowLaunch& env, const NormParams& p) {
+    const uint32_t cols = p.cols + (VEC == kPhased ? 7 : 0);   // as far as a row may reach
     const dim3 warps((p.rows + 3) / 4), blocks(p.rows);
-    if (p.cols <= 256) return launch_rows(env, norm_kernel<XT, RT, VEC, 1, false, 128>, p, warps, 128, 0);
-    if (p.cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, VEC, 4, false, 128>, p, warps, 128, 0);
-    if (p.cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, VEC, 4, true, 512>, p, blocks, 32 * ((p.cols + 1023) / 1024), 0);
-    if (p.cols <= 32768) return launch_rows(env, norm_kernel<XT, RT, VEC, 8, true, 512>, p, blocks, 32 * ((p.cols + 2047) / 2048), 0);
+    if (cols <= 256) return launch_rows(env, norm_kernel<XT, RT, VEC, 1, false, 128>, p, warps, 128, 0);
+    if (cols <= 1024) return launch_rows(env, norm_kernel<XT, RT, VEC, 4, false, 128>, p, warps, 128, 0);
+    if (cols <= 16384) return launch_rows(env, norm_kernel<XT, RT, VEC, 4, true, 512>, p, blocks, 32 * ((cols + 1023) / 1024), 0);
+    if (cols <= 32768) return launch_rows(env, norm_kernel<XT, RT, VEC, 8, true, 512>, p, blocks, 32 * ((cols + 2047) / 2048), 0);
     return launch_rows(env, norm_long_kernel<XT, RT, VEC>, p, blocks, 1024, 0);
 }
 template cudaError_t norm_of<INST_XT, INST_NORM, INST_VEC>(const RowLaunch&, const NormParams&);

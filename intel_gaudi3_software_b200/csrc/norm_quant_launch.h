@@ -33,8 +33,9 @@ struct GradShape {
     size_t smem;
 };
 constexpr int kGradSmem = 220 * 1024;
-inline GradShape grad_shape(uint32_t cols, bool fp32) {
-    if (cols <= 1024) return {GRAD_WARP, 128, cols <= 256 ? 1u : 4u, 4, 4, cols * sizeof(float)};
+inline GradShape grad_shape(uint32_t row_cols, bool fp32) {
+    const uint32_t cols = row_cols % 8 ? row_cols + 7 : row_cols;   // with room for a phase
+    if (cols <= 1024) return {GRAD_WARP, 128, cols <= 256 ? 1u : 4u, 4, 4, row_cols * sizeof(float)};
     if (cols <= 8192) {
         const uint32_t threads = 32 * ((cols + 1023) / 1024);
         return {GRAD_BLOCK, threads, 4, 1, std::max(1u, 512u / threads), 0};
