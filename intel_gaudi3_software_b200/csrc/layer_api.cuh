@@ -341,7 +341,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         TRY(layer_check_vector(c, dgamma, "dgamma", cols));
     }
     if (!(eps >= 0.0f) || eps > 3.4e38f) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
-    uint32_t blocks = norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), x->dtype == DT_FP32);
+    uint32_t blocks = norm_grad_blocks(c->device, c->sm_count, uint32_t(rows), uint32_t(cols));
     const uint64_t need = uint64_t(blocks) * cols;
     if (workspace) {
         TRY(layer_check(c, workspace, "workspace", true, false));
@@ -390,7 +390,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
             p.partial = static_cast<float*>(scratch);
         }
     }
-    const uint32_t phased = norm_grad_phased_blocks(blocks, p.rows, p.cols, x->dtype == DT_FP32);
+    const uint32_t phased = norm_grad_phased_blocks(blocks, p.rows, p.cols);
     const int vec = layer_vector(p.cols, p.dims, {&p.x, &p.dy, &p.dsum, &p.dx}, p.gamma.ptr, p.partial, p.flat && p.cols % 8 != 0 && phased > 0);
     if (vec == kPhased) blocks = phased;
     CUDA_OK(c, launch_norm_grad(layer_launch(c), p, vec, blocks));
@@ -678,7 +678,8 @@ extern "C" int mmeb200_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200
 }
 extern "C" size_t mmeb200_rms_norm_grad_workspace(const mmeb200_ctx* c, uint64_t rows, uint64_t cols) {
     if (!c || rows >= (uint64_t(1) << 31) || cols >= (uint64_t(1) << 31)) return 0;
-    return size_t(std::max(norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), false), norm_grad_blocks(c->sm_count, uint32_t(rows), uint32_t(cols), true))) * cols * sizeof(float);
+    DeviceGuard guard(c->device);
+    return size_t(norm_grad_blocks(c->device, c->sm_count, uint32_t(rows), uint32_t(cols))) * cols * sizeof(float);
 }
 extern "C" int mmeb200_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, const mmeb200_tensor* x, int op, int scale_mode) {
     return layer_entry(c, [&] { return run_quantize(c, out, scale, x, op, scale_mode); });

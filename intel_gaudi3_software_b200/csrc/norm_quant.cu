@@ -1,5 +1,6 @@
 // Launchers of the row kernels: the instantiation for a call's element types and alignment, and the small kernels beside them.
 #include <algorithm>
+#include <atomic>
 
 #include "norm_quant.cuh"
 #include "norm_quant_launch.h"
@@ -17,10 +18,22 @@ cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec) {
     return rt == ROW_NONE ? norm_with<ROW_F32, ROW_NONE>(env, p, vec) : rt == ROW_BF16 ? norm_with<ROW_F32, ROW_BF16>(env, p, vec) : norm_with<ROW_F32, ROW_F32>(env, p, vec);
 }
 
-uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32) {
-    const GradShape g = grad_shape(cols, fp32);
-    // as many blocks as the SMs hold at once: a block walks its rows to the end
-    return uint32_t(std::min<uint64_t>((uint64_t(rows) + g.rows_per_block - 1) / g.rows_per_block, uint64_t(sm_count) * g.blocks_per_sm));
+// As many blocks as the SMs hold at once: a block walks its rows to the end.
+uint32_t norm_grad_blocks(int device, int sm_count, uint32_t rows, uint32_t cols) {
+    const GradShape g = grad_shape(cols);
+    uint64_t held = uint64_t(sm_count) * g.blocks_per_sm;
+    if (g.form == GRAD_CLUSTER) {
+        static std::atomic<int> known[64][9][9] = {};   // by device, ranks and warps
+        std::atomic<int>& entry = known[device & 63][g.ranks][g.threads / 32];
+        int n = entry;
+        if (n == 0) {
+            n = norm_grad_clusters(g.ranks, g.threads);
+            if (n <= 0) n = std::max(1, sm_count / int(g.ranks));
+            entry = n;
+        }
+        held = uint64_t(n);
+    }
+    return uint32_t(std::min<uint64_t>((uint64_t(rows) + g.rows_per_block - 1) / g.rows_per_block, held));
 }
 template <int XT, bool DSUM>
 static cudaError_t norm_grad_with(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
@@ -28,8 +41,8 @@ static cudaError_t norm_grad_with(const RowLaunch& env, const NormGradParams& p,
 }
 // A block walks rows that are `blocks` blocks apart and keeps the sums of its columns: phased rows need a multiple of eight blocks,
 // so that a block's rows have one phase.
-uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols, bool fp32) {
-    return uint64_t(blocks) * grad_shape(cols, fp32).rows_per_block >= rows ? blocks : blocks & ~7u;
+uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols) {
+    return uint64_t(blocks) * grad_shape(cols).rows_per_block >= rows ? blocks : blocks & ~7u;
 }
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks) {
     if (p.x.type == ROW_BF16) return p.dsum.ptr ? norm_grad_with<ROW_BF16, true>(env, p, vec, blocks) : norm_grad_with<ROW_BF16, false>(env, p, vec, blocks);

@@ -690,72 +690,160 @@ __device__ __forceinline__ void store_sums(float* mine, uint32_t c, const RowSpa
 // The span of a block's (or warp's) rows: all of them have the first one's phase (launch_norm_grad).
 template <int XT, int VEC>
 __device__ __forceinline__ RowSpan<VEC> grad_span(const NormGradParams& p, uint32_t row) { return RowSpan<VEC>(row_of<XT>(p.x, row, p.dims, p.flat), RowElem<XT>::kBytes, p.cols); }
-// XT: type of x, dy, dsum and dx; DSUM: whether there is a gradient of the sum. A row per warp or per block, as in norm_kernel.
-template <int XT, bool DSUM, int VEC, int NV, bool BLOCK, int THREADS>
+// How a row is shared: by a warp (four rows per block), a block, or the blocks of a cluster (`ranks` of them, which add their sums
+// through each other's shared memory).
+enum : int { GRAD_WARP, GRAD_BLOCK, GRAD_CLUSTER, GRAD_REREAD };
+
+// The pieces of a row's tensors (x, dy, dsum), which every thread keeps for itself. FETCHED (bf16 rows that move by 16 bytes): in
+// shared memory, copied there a row ahead. Else in registers, loaded when the row begins.
+// (16384 x 4096 bf16 with gamma in registers: 67 us, and 91 us with dsum; pieces in registers and gamma read twice per row: 90 and
+// 101 us. fp32 pieces would leave an SM half its threads.)
+template <int XT, bool DSUM, int VEC, int NV>
+struct GradPieces {
+    static constexpr bool kFetched = XT == ROW_BF16 && VEC != 1;
+    static constexpr int W = 2 * RowElem<XT>::kBytes, kTensors = DSUM ? 3 : 2;
+    uint32_t w[kFetched ? 1 : kTensors * NV][W];
+    uint4* mine;         // [stage][tensor][step][thread]
+    uint32_t stage = 0;
+    __device__ __forceinline__ explicit GradPieces(uint4* smem) : mine(smem + threadIdx.x) {}
+    __device__ __forceinline__ uint4* slot(uint32_t at, int tensor, int i) const { return mine + ((at * kTensors + tensor) * NV + i) * blockDim.x; }
+    // Row `row` into the stage that is not in use; done counts with wait().
+    __device__ __forceinline__ void fetch(const NormGradParams& p, uint32_t row, uint32_t c0, const RowSpan<VEC>& span) const {
+        if constexpr (kFetched) {
+            if (row < p.rows) {
+                const RowTensor* t[3] = {&p.x, &p.dy, &p.dsum};
+#pragma unroll
+                for (int k = 0; k < kTensors; ++k) {
+                    const uint8_t* a = row_of<XT>(*t[k], row, p.dims, p.flat) + (int64_t(c0 + lane_column<VEC>(0)) - span.phase) * RowElem<XT>::kBytes;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i)
+                        if (in_row<VEC>(c0 + i * 256, span)) cp_async16(slot(stage ^ 1, k, i), a + i * 256 * RowElem<XT>::kBytes);
+                }
+            }
+            cp_async_commit();
+        }
+    }
+    // The row that is to be worked on.
+    __device__ __forceinline__ void begin(const NormGradParams& p, uint32_t row, uint32_t next, uint32_t c0, const RowSpan<VEC>& span) {
+        if constexpr (kFetched) {
+            stage ^= 1;
+            fetch(p, next, c0, span);   // into the stage that the row before left: its values were used up by what was stored
+            cp_async_wait<1>();
+        } else {
+            const RowTensor* t[3] = {&p.x, &p.dy, &p.dsum};
+#pragma unroll
+            for (int k = 0; k < kTensors; ++k) {
+                const uint8_t* a = row_of<XT>(*t[k], row, p.dims, p.flat) - span.phase * RowElem<XT>::kBytes;
+#pragma unroll
+                for (int i = 0; i < NV; ++i)
+                    if (in_row<VEC>(c0 + i * 256, span)) load_piece<XT, VEC>(a, c0 + i * 256, span, w[k * NV + i]);
+            }
+        }
+    }
+    __device__ __forceinline__ void values(int tensor, int i, uint32_t c, const RowSpan<VEC>& span, float2 (&v)[4]) const {
+        uint32_t q[W];
+        if constexpr (kFetched) {
+            const uint4 u = *slot(stage, tensor, i);
+            q[0] = u.x; q[1] = u.y; q[2] = u.z; q[3] = u.w;
+        } else {
+#pragma unroll
+            for (int k = 0; k < W; ++k) q[k] = w[tensor * NV + i][k];
+        }
+        trim_piece<XT, VEC>(c, span, q);
+        unpack<XT>(q, v);
+    }
+};
+// XT: type of x, dy, dsum and dx; DSUM: whether there is a gradient of the sum.
+template <int XT, bool DSUM, int VEC, int NV, int FORM, int THREADS>
 __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const __grid_constant__ NormGradParams p) {
+    constexpr bool BLOCK = FORM != GRAD_WARP;
     constexpr int kRowsPerBlock = BLOCK ? 1 : 4, W = 2 * RowElem<XT>::kBytes;
     __shared__ float2 scratch[2][32];
-    extern __shared__ uint4 grad_smem[];   // a row per warp: [cols] floats, the four warps' sums of dgamma
+    __shared__ float2 shares[2][8];        // GRAD_CLUSTER: the sums of every block of the cluster
+    extern __shared__ uint4 grad_smem[];   // the pieces; GRAD_WARP: then [cols] floats, the four warps' sums of dgamma
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t sub = BLOCK ? 0 : (threadIdx.x >> 5), c0 = BLOCK ? (threadIdx.x >> 5) * 256 * NV : 0;
+    uint32_t rank = 0, unit = blockIdx.x, units = gridDim.x;
+    if constexpr (FORM == GRAD_CLUSTER) {
+        rank = cluster_ctarank();
+        unit /= p.ranks;
+        units /= p.ranks;
+        cluster_sync_all();   // all blocks run before the first writes to another's memory
+    }
+    const uint32_t warp = threadIdx.x >> 5, sub = BLOCK ? 0 : warp, c0 = BLOCK ? (rank * (blockDim.x >> 5) + warp) * 256 * NV : 0;
     float2 acc[NV][4];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) acc[i][k] = both(0.0f);
-    const RowSpan<VEC> span = grad_span<XT, VEC>(p, blockIdx.x * kRowsPerBlock + sub);
-    const uint32_t shift = span.phase * RowElem<XT>::kBytes;
-    uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x * kRowsPerBlock + sub; row < p.rows; row += gridDim.x * kRowsPerBlock, turn ^= 1) {
-        const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat) - shift, *yr = row_of<XT>(p.dy, row, p.dims, p.flat) - shift;
-        const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) - shift : nullptr;
-        uint32_t xs[NV][W], ys[NV][W], ds[DSUM ? NV : 1][W];
+    // a thread's columns are the same in all rows: where its registers do not hold the pieces too, they hold gamma
+    constexpr bool kHold = GradPieces<XT, DSUM, VEC, NV>::kFetched;
+    float2 gamma[kHold ? NV : 1][4];
+    const uint32_t first = unit * kRowsPerBlock + sub, stride = units * kRowsPerBlock;
+    const RowSpan<VEC> span = grad_span<XT, VEC>(p, first);
+    GradPieces<XT, DSUM, VEC, NV> pieces(grad_smem);
+    pieces.fetch(p, first, c0, span);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, span)) {
-                load_piece<XT, VEC>(xr, c0 + i * 256, span, xs[i]);
-                load_piece<XT, VEC>(yr, c0 + i * 256, span, ys[i]);
-                if constexpr (DSUM) load_piece<XT, VEC>(sr, c0 + i * 256, span, ds[i]);
-            }
+    for (int i = 0; i < (kHold ? NV : 0); ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) gamma[i][k] = both(1.0f);
+        if (p.gamma.ptr && in_row<VEC>(c0 + i * 256, span)) load_gamma<VEC>(p.gamma, c0 + i * 256, span, gamma[i]);
+    }
+    const auto scale = [&](const float2(&y)[4], int i, float2(&a)[4]) {
+        if constexpr (kHold) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] = __fmul2_rn(y[k], gamma[i][k]);
+        } else {
+            grad_scale<VEC>(p, y, c0 + i * 256, span, a);
         }
+    };
+    uint32_t turn = 0;
+    for (uint32_t row = first; row < p.rows; row += stride, turn ^= 1) {
+        pieces.begin(p, row, row + stride, c0, span);
         float2 squares = both(0.0f), dot = both(0.0f);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, span)) {
+            const uint32_t c = c0 + i * 256;
+            if (in_row<VEC>(c, span)) {
                 float2 x[4], y[4], a[4];
-                trim_piece<XT, VEC>(c0 + i * 256, span, xs[i]);
-                trim_piece<XT, VEC>(c0 + i * 256, span, ys[i]);
-                unpack<XT>(xs[i], x);
-                unpack<XT>(ys[i], y);
-                grad_scale<VEC>(p, y, c0 + i * 256, span, a);
+                pieces.values(0, i, c, span, x);
+                pieces.values(1, i, c, span, y);
+                scale(y, i, a);
                 sum_grad(x, a, squares, dot);
             }
         }
         // two buffers: the next row's sums may start before all have read
-        const float2 s = reduce_row<BLOCK, false>(squares.x + squares.y, dot.x + dot.y, blockDim.x >> 5, scratch[turn]);
+        float2 s = reduce_row<BLOCK, false>(squares.x + squares.y, dot.x + dot.y, blockDim.x >> 5, scratch[turn]);
+        if constexpr (FORM == GRAD_CLUSTER) {
+            if (threadIdx.x < p.ranks) st_shared_cluster_f2(mapa_shared(smem_u32(&shares[turn][rank]), threadIdx.x), s);
+            __syncwarp();
+            cluster_sync_all();
+            s = shares[turn][0];
+            for (uint32_t r = 1; r < p.ranks; ++r) s = __fadd2_rn(s, shares[turn][r]);
+        }
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
-        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat) - shift;
+        uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat) - span.phase * RowElem<XT>::kBytes;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (in_row<VEC>(c0 + i * 256, span)) {
+            const uint32_t c = c0 + i * 256;
+            if (in_row<VEC>(c, span)) {
                 float2 x[4], y[4], a[4], add[4];
-                unpack<XT>(xs[i], x);
-                unpack<XT>(ys[i], y);
-                if constexpr (DSUM) unpack<XT>(ds[i], add);
-                grad_scale<VEC>(p, y, c0 + i * 256, span, a);
+                pieces.values(0, i, c, span, x);
+                pieces.values(1, i, c, span, y);
+                if constexpr (DSUM) pieces.values(2, i, c, span, add);
+                scale(y, i, a);
                 grad_piece<DSUM>(x, y, a, add, inv, mean_au, acc[i]);
                 uint32_t w[W];
                 pack<XT>(a, w);
-                store_piece<XT, VEC>(out, c0 + i * 256, span, w);
+                store_piece<XT, VEC>(out, c, span, w);
             }
         }
     }
     if (!p.partial) return;
-    float* mine = p.partial + uint64_t(blockIdx.x) * p.cols;
+    float* mine = p.partial + uint64_t(unit) * p.cols;
     if constexpr (!BLOCK) {
-        float* block_sums = reinterpret_cast<float*>(grad_smem);
+        float* block_sums = reinterpret_cast<float*>(grad_smem + (GradPieces<XT, DSUM, VEC, NV>::kFetched ? 2 * GradPieces<XT, DSUM, VEC, NV>::kTensors * NV * THREADS : 0));
         for (uint32_t w = 0; w < 4; ++w) {   // the warps add their sums in turn: the order is fixed
             if (sub == w) {
 #pragma unroll
@@ -776,18 +864,14 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) norm_grad_kernel(const
             if (in_row<VEC>(c0 + i * 256, span)) store_sums<VEC>(mine, c0 + i * 256, span, acc[i]);
     }
 }
-// Longer rows, walked by a loop. KEEP: x and dy are kept in shared memory between the two passes, and so are the sums of dgamma,
-// every thread its own; else both passes read from memory and the sums live in the block's row of `partial`.
-template <int XT, bool DSUM, int VEC, bool KEEP>
+// Rows too long even for a cluster: both passes read from memory and the sums of dgamma live in the block's row of `partial`.
+template <int XT, bool DSUM, int VEC>
 __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_constant__ NormGradParams p) {
-    constexpr int W = 2 * RowElem<XT>::kBytes, Q = W / 4;
+    constexpr int W = 2 * RowElem<XT>::kBytes;
     __shared__ float2 scratch[2][32];
-    extern __shared__ uint4 grad_smem[];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t threads = blockDim.x, steps = p.steps, first = (threadIdx.x >> 5) * 256 * steps;
-    uint4* keep = grad_smem + threadIdx.x;                                                       // [step][16-byte word of x, then dy][thread]
-    float4* sums = reinterpret_cast<float4*>(grad_smem + steps * 2 * Q * threads) + threadIdx.x;   // [step][half of the eight][thread]
+    const uint32_t first = (threadIdx.x >> 5) * 256, stride = (blockDim.x >> 5) * 256;
     float* mine = p.partial ? p.partial + uint64_t(blockIdx.x) * p.cols : nullptr;
     const RowSpan<VEC> span = grad_span<XT, VEC>(p, blockIdx.x);
     const uint32_t shift = span.phase * RowElem<XT>::kBytes;
@@ -796,63 +880,33 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
         const uint8_t *xr = row_of<XT>(p.x, row, p.dims, p.flat) - shift, *yr = row_of<XT>(p.dy, row, p.dims, p.flat) - shift;
         const uint8_t* sr = DSUM ? row_of<XT>(p.dsum, row, p.dims, p.flat) - shift : nullptr;
         float2 squares = both(0.0f), dot = both(0.0f);
-#pragma unroll 1
-        for (uint32_t i0 = 0; i0 < steps; i0 += 2) {
-            uint32_t xw[2][W], yw[2][W];
-#pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                const uint32_t c = first + (i0 + j) * 256;
-                if (i0 + j < steps && in_row<VEC>(c, span)) {
-                    load_piece<XT, VEC>(xr, c, span, xw[j]);
-                    load_piece<XT, VEC>(yr, c, span, yw[j]);
-                }
-            }
-#pragma unroll
-            for (uint32_t j = 0; j < 2; ++j) {
-                const uint32_t i = i0 + j, c = first + i * 256;
-                if (i < steps && in_row<VEC>(c, span)) {
-                    trim_piece<XT, VEC>(c, span, xw[j]);
-                    trim_piece<XT, VEC>(c, span, yw[j]);
-                    if constexpr (KEEP) {
-#pragma unroll
-                        for (int k = 0; k < Q; ++k) {
-                            keep[(i * 2 * Q + k) * threads] = make_uint4(xw[j][4 * k], xw[j][4 * k + 1], xw[j][4 * k + 2], xw[j][4 * k + 3]);
-                            keep[(i * 2 * Q + Q + k) * threads] = make_uint4(yw[j][4 * k], yw[j][4 * k + 1], yw[j][4 * k + 2], yw[j][4 * k + 3]);
-                        }
-                    }
-                    float2 x[4], y[4], a[4];
-                    unpack<XT>(xw[j], x);
-                    unpack<XT>(yw[j], y);
-                    grad_scale<VEC>(p, y, c, span, a);
-                    sum_grad(x, a, squares, dot);
-                }
-            }
+#pragma unroll 2
+        for (uint32_t c = first; in_row<VEC>(c, span); c += stride) {
+            uint32_t xw[W], yw[W];
+            float2 x[4], y[4], a[4];
+            load_piece<XT, VEC>(xr, c, span, xw);
+            load_piece<XT, VEC>(yr, c, span, yw);
+            trim_piece<XT, VEC>(c, span, xw);
+            trim_piece<XT, VEC>(c, span, yw);
+            unpack<XT>(xw, x);
+            unpack<XT>(yw, y);
+            grad_scale<VEC>(p, y, c, span, a);
+            sum_grad(x, a, squares, dot);
         }
-        const float2 s = reduce_row<true, false>(squares.x + squares.y, dot.x + dot.y, threads >> 5, scratch[turn]);
+        const float2 s = reduce_row<true, false>(squares.x + squares.y, dot.x + dot.y, blockDim.x >> 5, scratch[turn]);
         const float inv = inverse_rms(s.x, p.per_col, p.eps);
         const float mean_au = s.y * p.per_col * inv;
         const bool begin = row == blockIdx.x;
         uint8_t* out = row_of<XT>(p.dx, row, p.dims, p.flat) - shift;
 #pragma unroll 1
-        for (uint32_t i = 0; i < steps; ++i) {
-            const uint32_t c = first + i * 256;
-            if (!in_row<VEC>(c, span)) break;
+        for (uint32_t c = first; in_row<VEC>(c, span); c += stride) {
             uint32_t xw[W], yw[W], w[W];
             float2 x[4], y[4], a[4], add[4], acc[4];
+            load_piece<XT, VEC>(xr, c, span, xw);
+            load_piece<XT, VEC>(yr, c, span, yw);
             if constexpr (DSUM) {
                 load_piece<XT, VEC>(sr, c, span, w);
                 unpack<XT>(w, add);
-            }
-            if constexpr (KEEP) {
-#pragma unroll
-                for (int k = 0; k < Q; ++k) {
-                    const uint4 t = keep[(i * 2 * Q + k) * threads], u = keep[(i * 2 * Q + Q + k) * threads];
-                    xw[4 * k] = t.x; xw[4 * k + 1] = t.y; xw[4 * k + 2] = t.z; xw[4 * k + 3] = t.w;
-                    yw[4 * k] = u.x; yw[4 * k + 1] = u.y; yw[4 * k + 2] = u.z; yw[4 * k + 3] = u.w;
-                }
-            } else {
-                load_piece<XT, VEC>(xr, c, span, xw);
-                load_piece<XT, VEC>(yr, c, span, yw);
             }
             unpack<XT>(xw, x);
             unpack<XT>(yw, y);
@@ -860,37 +914,14 @@ __global__ void __launch_bounds__(512, 2) norm_grad_loop_kernel(const __grid_con
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[k] = both(0.0f);
             if (mine && !begin) {
-                if constexpr (KEEP) {
-                    const float4 t = sums[(i * 2) * threads], u = sums[(i * 2 + 1) * threads];
-                    acc[0] = make_float2(t.x, t.y); acc[1] = make_float2(t.z, t.w);
-                    acc[2] = make_float2(u.x, u.y); acc[3] = make_float2(u.z, u.w);
-                } else {
-                    uint32_t t[8];
-                    load_floats<VEC>(mine, c, span, t);
-                    unpack<ROW_F32>(t, acc);
-                }
+                uint32_t t[8];
+                load_floats<VEC>(mine, c, span, t);
+                unpack<ROW_F32>(t, acc);
             }
             grad_piece<DSUM>(x, y, a, add, inv, mean_au, acc);
-            if (mine) {
-                if constexpr (KEEP) {
-                    sums[(i * 2) * threads] = make_float4(acc[0].x, acc[0].y, acc[1].x, acc[1].y);
-                    sums[(i * 2 + 1) * threads] = make_float4(acc[2].x, acc[2].y, acc[3].x, acc[3].y);
-                } else {
-                    store_sums<VEC>(mine, c, span, acc);
-                }
-            }
+            if (mine) store_sums<VEC>(mine, c, span, acc);
             pack<XT>(a, w);
             store_piece<XT, VEC>(out, c, span, w);
-        }
-    }
-    if constexpr (KEEP) {
-        if (mine) {
-#pragma unroll 1
-            for (uint32_t i = 0; i < steps && in_row<VEC>(first + i * 256, span); ++i) {
-                const float4 t = sums[(i * 2) * threads], u = sums[(i * 2 + 1) * threads];
-                const float2 acc[4] = {make_float2(t.x, t.y), make_float2(t.z, t.w), make_float2(u.x, u.y), make_float2(u.z, u.w)};
-                store_sums<VEC>(mine, first + i * 256, span, acc);
-            }
         }
     }
 }

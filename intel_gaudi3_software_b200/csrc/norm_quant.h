@@ -45,7 +45,7 @@ struct NormGradParams {
     uint32_t rows, cols;
     uint32_t dims[4];
     uint32_t flat;
-    uint32_t steps;        // set by the launcher
+    uint32_t ranks;        // blocks of a row's cluster; set by the launcher
     float eps, per_col;
 };
 
@@ -75,10 +75,10 @@ struct RowLaunch {
 // every tensor equally far past eight elements (gamma on 16 bytes); 1, anything.
 constexpr int kPhased = 0;
 cudaError_t launch_norm(const RowLaunch& env, const NormParams& p, int vec);
-// Blocks the gradient kernel runs with, i.e. rows of `partial`.
-uint32_t norm_grad_blocks(int sm_count, uint32_t rows, uint32_t cols, bool fp32);
+// Blocks (or clusters of blocks) the gradient kernel runs with, i.e. rows of `partial`.
+uint32_t norm_grad_blocks(int device, int sm_count, uint32_t rows, uint32_t cols);
 // Of those, the blocks that phased rows can use (0: none).
-uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols, bool fp32);
+uint32_t norm_grad_phased_blocks(uint32_t blocks, uint32_t rows, uint32_t cols);
 cudaError_t launch_norm_grad(const RowLaunch& env, const NormGradParams& p, int vec, uint32_t blocks);
 cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float* out, uint32_t blocks, uint32_t cols);
 // Number of kernels launched is returned in *launches.

@@ -26,25 +26,57 @@ template cudaError_t norm_of<INST_XT, INST_NORM, INST_VEC>(const RowLaunch&, con
 
 #elif defined(INST_GRAD)
 
-template <int XT, bool DSUM, int VEC>
-cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& given, uint32_t blocks) {
-    NormGradParams p = given;
-    const dim3 g(blocks);
-    const GradShape shape = grad_shape(p.cols, XT == ROW_F32);
-    p.steps = shape.steps;
-    if (shape.form == GRAD_WARP && shape.steps == 1) return launch_rows(env, norm_grad_kernel<XT, DSUM, VEC, 1, false, 128>, p, g, 128, shape.smem);
-    if (shape.form == GRAD_WARP) return launch_rows(env, norm_grad_kernel<XT, DSUM, VEC, 4, false, 128>, p, g, 128, shape.smem);
-    if (shape.form == GRAD_BLOCK) return launch_rows(env, norm_grad_kernel<XT, DSUM, VEC, 4, true, 256>, p, g, shape.threads, 0);
-    if (shape.form == GRAD_REREAD) return launch_rows(env, norm_grad_loop_kernel<XT, DSUM, VEC, false>, p, g, shape.threads, 0);
+template <int XT, bool DSUM, int VEC, int NV>
+size_t grad_smem_bytes(const GradShape& shape, uint32_t cols) {
+    using Pieces = GradPieces<XT, DSUM, VEC, NV>;
+    return (Pieces::kFetched ? size_t(2) * Pieces::kTensors * NV * 16 * shape.threads : 0) + (shape.form == GRAD_WARP ? size_t(cols) * sizeof(float) : 0);
+}
+template <int XT, bool DSUM, int VEC, int NV, int FORM, int THREADS>
+cudaError_t launch_grad(const RowLaunch& env, const NormGradParams& p, uint32_t blocks, const GradShape& shape) {
+    const auto kern = norm_grad_kernel<XT, DSUM, VEC, NV, FORM, THREADS>;
+    const size_t smem = grad_smem_bytes<XT, DSUM, VEC, NV>(shape, p.cols);
     static bool done[64] = {};
-    if (!done[env.device & 63]) {
-        const cudaError_t e = cudaFuncSetAttribute(norm_grad_loop_kernel<XT, DSUM, VEC, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kGradSmem);
+    if (smem > 40 * 1024 && !done[env.device & 63]) {   // (48 KB with the static shared memory need no leave)
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
         if (e != cudaSuccess) return e;
         done[env.device & 63] = true;
     }
-    return launch_rows(env, norm_grad_loop_kernel<XT, DSUM, VEC, true>, p, g, shape.threads, shape.smem);
+    return launch_rows(env, kern, p, dim3(blocks * shape.ranks), shape.threads, smem, shape.ranks);
+}
+template <int XT, bool DSUM, int VEC>
+cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& given, uint32_t blocks) {
+    NormGradParams p = given;
+    const GradShape shape = grad_shape(p.cols);
+    p.ranks = shape.ranks;
+    if (shape.form == GRAD_WARP && p.cols + (p.cols % 8 ? 7 : 0) <= 256) return launch_grad<XT, DSUM, VEC, 1, GRAD_WARP, 128>(env, p, blocks, shape);
+    if (shape.form == GRAD_WARP) return launch_grad<XT, DSUM, VEC, 4, GRAD_WARP, 128>(env, p, blocks, shape);
+    if (shape.form == GRAD_BLOCK) return launch_grad<XT, DSUM, VEC, 4, GRAD_BLOCK, 256>(env, p, blocks, shape);
+    if (shape.form == GRAD_CLUSTER) return launch_grad<XT, DSUM, VEC, 4, GRAD_CLUSTER, 256>(env, p, blocks, shape);
+    return launch_rows(env, norm_grad_loop_kernel<XT, DSUM, VEC>, p, dim3(blocks), shape.threads, 0);
 }
 template cudaError_t norm_grad_of<INST_XT, INST_GRAD != 0, INST_VEC>(const RowLaunch&, const NormGradParams&, uint32_t);
+
+#if INST_XT == 1 && INST_GRAD == 1 && INST_VEC == 8
+// Of the form that needs most shared memory; all have the same registers.
+int norm_grad_clusters(uint32_t ranks, uint32_t threads) {
+    const auto kern = norm_grad_kernel<ROW_BF16, true, 8, 4, GRAD_CLUSTER, 256>;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) != cudaSuccess) return 0;
+    GradShape shape{GRAD_CLUSTER, threads, 1, 1, ranks};
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ranks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(ranks * 64);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = grad_smem_bytes<ROW_BF16, true, 8, 4>(shape, 0);
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
+}
+#endif
 
 #elif defined(INST_TRANS)
 

@@ -4,52 +4,53 @@
 #include <algorithm>
 #include <cstring>
 
-#include "norm_quant.h"
+#include "norm_quant.cuh"
 
 namespace mmeb200 {
 
 template <typename P>
-inline cudaError_t launch_rows(const RowLaunch& env, void (*kern)(P), const P& p, dim3 grid, unsigned threads, size_t smem) {
+inline cudaError_t launch_rows(const RowLaunch& env, void (*kern)(P), const P& p, dim3 grid, unsigned threads, size_t smem, unsigned cluster = 1) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = env.stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = env.dependent_launch ? 1 : 0;
+    cudaLaunchAttribute attrs[2];
+    cfg.attrs = attrs;
+    if (env.dependent_launch) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attrs[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[cfg.numAttrs].val.clusterDim.x = cluster;
+        attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
 
-// The gradient's form and shape: a function of the columns and the type, so that its workspace can be asked for.
-enum : int { GRAD_WARP, GRAD_BLOCK, GRAD_LOOP, GRAD_REREAD };
+// The gradient's form and shape: a function of the columns, so that its workspace can be asked for. A thread takes at most 32
+// columns, a block 256 threads; up to eight blocks share a row.
 struct GradShape {
     int form;
-    uint32_t threads, steps, rows_per_block, blocks_per_sm;   // steps: of 256 columns per warp
-    size_t smem;
+    uint32_t threads, rows_per_block, blocks_per_sm, ranks;
 };
-constexpr int kGradSmem = 220 * 1024;
-inline GradShape grad_shape(uint32_t row_cols, bool fp32) {
+inline GradShape grad_shape(uint32_t row_cols) {
     const uint32_t cols = row_cols % 8 ? row_cols + 7 : row_cols;   // with room for a phase
-    if (cols <= 1024) return {GRAD_WARP, 128, cols <= 256 ? 1u : 4u, 4, 4, row_cols * sizeof(float)};
-    if (cols <= 8192) {
-        const uint32_t threads = 32 * ((cols + 1023) / 1024);
-        return {GRAD_BLOCK, threads, 4, 1, std::max(1u, 512u / threads), 0};
-    }
-    const uint32_t steps = (cols + 16 * 256 - 1) / (16 * 256);
-    const uint64_t smem = uint64_t(512) * steps * 8 * ((fp32 ? 8 : 4) + 4);   // x and dy, the sums of dgamma
-    if (smem <= kGradSmem) return {GRAD_LOOP, 512, steps, 1, smem <= kGradSmem / 2 ? 2u : 1u, size_t(smem)};
-    return {GRAD_REREAD, 512, steps, 1, 2, 0};
+    if (cols <= 1024) return {GRAD_WARP, 128, 4, 4, 1};
+    const uint32_t ranks = (cols + 8191) / 8192, threads = 32 * (((cols + ranks - 1) / ranks + 1023) / 1024);
+    if (ranks <= 8) return {ranks == 1 ? GRAD_BLOCK : GRAD_CLUSTER, threads, 1, std::max(1u, 512u / threads), ranks};
+    return {GRAD_REREAD, 512, 1, 2, 1};
 }
 
 template <int XT, int RT, int VEC>
 cudaError_t norm_of(const RowLaunch& env, const NormParams& p);
 template <int XT, bool DSUM, int VEC>
 cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& p, uint32_t blocks);
+int norm_grad_clusters(uint32_t ranks, uint32_t threads);   // of so many blocks of so many threads that the current device holds at once
 template <int XT, int VEC>
 cudaError_t quant_trans_of(const RowLaunch& env, const QuantTransParams& p, int* launches);
 
