@@ -440,7 +440,7 @@ int run_quantize(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, con
     p.rows = uint32_t(rows); p.cols = uint32_t(cols);
     int launches = 0;
     const uint32_t dims[4] = {p.rows, 1, 1, 1};
-    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, layer_vector(p.cols, dims, {&p.x}, nullptr, nullptr, false), &launches));
+    CUDA_OK(c, launch_quant_trans(layer_launch(c), p, layer_vector(p.cols, dims, {&p.x}, nullptr, nullptr, true), &launches));
     c->launches += uint64_t(launches);
     return st.finish();
 }

@@ -58,7 +58,7 @@ cudaError_t launch_column_sums(const RowLaunch& env, const float* partial, float
 
 template <int XT>
 static cudaError_t quant_trans_with(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
-    return vec == 8 ? quant_trans_of<XT, 8>(env, p, launches) : quant_trans_of<XT, 1>(env, p, launches);
+    return vec == 8 ? quant_trans_of<XT, 8>(env, p, launches) : vec == kPhased ? quant_trans_of<XT, kPhased>(env, p, launches) : quant_trans_of<XT, 1>(env, p, launches);
 }
 cudaError_t launch_quant_trans(const RowLaunch& env, const QuantTransParams& p, int vec, int* launches) {
     *launches = 0;

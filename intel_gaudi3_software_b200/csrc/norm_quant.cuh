@@ -949,11 +949,24 @@ __device__ __forceinline__ void column_sums(const float* partial, float* out, ui
 // One step per column of x, result transposed. First the columns' maxima (as bit patterns, whose order is the values'; a NaN's
 // is above infinity's, so it stays), then the codes through a tile in shared memory, then the steps in place of the maxima.
 // x is read twice; the second pass walks the rows from the end, so that it begins with what the first left in L2. In both a
-// warp reads 256 consecutive columns of a row; slot e * 32 + lane stands for the column of that lane's element e.
+// warp reads 256 consecutive columns of a row; slot e * 32 + lane stands for the column of that lane's element e. Phased rows: every
+// eighth row has the same phase, so a warp takes rows that are a multiple of eight apart, and of its 256 columns it can be sure of
+// 248 whatever its phase.
 template <int VEC>
 __device__ __forceinline__ uint32_t slot_column(uint32_t slot) {
     const uint32_t e = slot >> 5, lane = slot & 31;
     return VEC == 1 ? e * 32 + lane : lane * 8 + e;
+}
+template <int VEC>
+constexpr uint32_t kTransCols = VEC == kPhased ? 248 : 256;   // columns of a tile
+// Offset of a lane's element e from the tile's first column (negative below it) in rows of this phase.
+template <int VEC>
+__device__ __forceinline__ int element_column(int e, uint32_t phase) { return int(lane_column<VEC>(e)) - int(phase); }
+template <int VEC>
+__device__ __forceinline__ uint32_t element_slot(int e, uint32_t phase) {
+    const uint32_t lane = threadIdx.x & 31;
+    if constexpr (VEC != kPhased) return e * 32 + lane;
+    return ((uint32_t(e) - phase) & 7) * 32 + lane - (uint32_t(e) < phase);
 }
 template <int XT>
 __device__ __forceinline__ const uint8_t* trans_row(const QuantTransParams& p, uint32_t row) {
@@ -962,22 +975,24 @@ __device__ __forceinline__ const uint8_t* trans_row(const QuantTransParams& p, u
 template <int XT, int VEC>
 __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__ QuantTransParams p) {
     constexpr int W = 2 * RowElem<XT>::kBytes;
+    constexpr uint32_t kCols = kTransCols<VEC>;
     __shared__ float part[8][257];
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * 256;
-    const uint32_t rows_per = (p.rows + gridDim.y - 1) / gridDim.y, r0 = blockIdx.y * rows_per, r1 = min(p.rows, r0 + rows_per);
+    const uint32_t warp = threadIdx.x >> 5, c0 = blockIdx.x * kCols;
+    const uint32_t rows_per = ((p.rows + gridDim.y - 1) / gridDim.y + 7) & ~7u, r0 = min(p.rows, blockIdx.y * rows_per), r1 = min(p.rows, r0 + rows_per);
     float2 top[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) top[k] = both(0.0f);
-    const RowSpan<VEC> span(nullptr, 1, p.cols);
+    const RowSpan<VEC> span(trans_row<XT>(p, r0 + warp), RowElem<XT>::kBytes, p.cols);
+    const uint32_t shift = span.phase * RowElem<XT>::kBytes;
     const bool there = in_row<VEC>(c0, span);
 #pragma unroll 1
     for (uint32_t r = r0 + warp; r < r1; r += 32) {
         uint32_t x[4][W];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (there && r + 8 * j < r1) load_piece<XT, VEC>(trans_row<XT>(p, r + 8 * j), c0, span, x[j]);
+            if (there && r + 8 * j < r1) load_piece<XT, VEC>(trans_row<XT>(p, r + 8 * j) - shift, c0, span, x[j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (there && r + 8 * j < r1) {
@@ -988,47 +1003,56 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
             }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) part[warp][e * 32 + lane] = (e & 1) ? top[e >> 1].y : top[e >> 1].x;
+    for (int e = 0; e < 8; ++e)
+        if (VEC != kPhased || element_column<VEC>(e, span.phase) >= 0) part[warp][element_slot<VEC>(e, span.phase)] = (e & 1) ? top[e >> 1].y : top[e >> 1].x;
     __syncthreads();
-    const uint32_t mine = c0 + slot_column<VEC>(threadIdx.x);
+    const uint32_t column = slot_column<VEC>(threadIdx.x), mine = c0 + column;
+    if (column >= kCols || mine >= p.cols) return;
     float t = part[0][threadIdx.x];
 #pragma unroll
     for (int i = 1; i < 8; ++i) t = max_nan(t, part[i][threadIdx.x]);
-    if (mine < p.cols) atomicMax(reinterpret_cast<uint32_t*>(p.scale) + mine, __float_as_uint(t) & 0x7FFFFFFFu);
+    atomicMax(reinterpret_cast<uint32_t*>(p.scale) + mine, __float_as_uint(t) & 0x7FFFFFFFu);
 }
-// Tiles of 128 rows x 256 columns: a warp takes four rows at a time, a lane eight of their columns, whose codes make one word per
-// column. The tile's columns leave as aligned 16-byte words (byte by byte at their ends).
+// Tiles of 128 rows x 256 columns (248 phased): a warp takes four rows at a time, a lane eight of their columns, whose codes make one
+// word per column. The tile's columns leave as aligned 16-byte words (byte by byte at their ends). Four blocks per SM hide one's
+// loads behind another's stores: 8192 x 8192 bf16 64 us, with three and rows read a step ahead 68 us.
 constexpr uint32_t kTransRows = 128;
-template <bool I8, bool GIVEN>
-__device__ __forceinline__ uint32_t column_codes(const QuantTransParams& p, float2 v0, float2 v1, const CodeStep& s) {
-    if (!GIVEN && fast_step(s, I8 || p.fp8_direct)) return make_codes<I8, true>(v0, v1, s, p.hw);
-    return make_codes<I8, false>(v0, v1, s, p.hw);
-}
 template <int XT, int VEC, bool I8, bool GIVEN>
-__global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_constant__ QuantTransParams p) {
+__global__ void __launch_bounds__(256, XT == ROW_BF16 ? 4 : 3) quant_trans_kernel(const __grid_constant__ QuantTransParams p) {
     constexpr int W = 2 * RowElem<XT>::kBytes;
     constexpr uint32_t kPitch = 33;               // words: 128 rows and one word that keeps the banks apart
     __shared__ uint32_t tile[256 * kPitch + 4];   // by slot: neighbouring lanes, neighbouring banks
     __shared__ CodeStep steps[256];               // by slot
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c0 = blockIdx.x * 256, r0 = (gridDim.y - 1 - blockIdx.y) * kTransRows;
+    const uint32_t warp = threadIdx.x >> 5, c0 = blockIdx.x * kTransCols<VEC>, r0 = (gridDim.y - 1 - blockIdx.y) * kTransRows;
     {
         const uint32_t c = c0 + slot_column<VEC>(threadIdx.x);
-        float s = 0.0f;
+        float s = 1.0f;
         if (c < p.cols) s = GIVEN ? p.given[uint64_t(c) * p.given_stride] : __fdiv_rn(p.scale[c], p.top);
         steps[threadIdx.x] = make_code_step(s);
     }
+    // a step is 32 rows, four of them a warp's: neighbours, or (phased) eight apart
+    constexpr uint32_t kApart = VEC == kPhased ? 8 : 1;
+    const uint32_t first = VEC == kPhased ? warp : warp * 4;
+    const RowSpan<VEC> span(trans_row<XT>(p, p.row0 + r0 + first), RowElem<XT>::kBytes, p.cols);
+    const uint32_t shift = span.phase * RowElem<XT>::kBytes;
     __syncthreads();
-    const RowSpan<VEC> span(nullptr, 1, p.cols);
+    CodeStep mine[8];   // of this lane's columns
+    bool all_fast = !GIVEN;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        mine[e] = VEC != kPhased || element_column<VEC>(e, span.phase) >= 0 ? steps[element_slot<VEC>(e, span.phase)] : CodeStep{1.0f, -1.0f};
+        all_fast = all_fast && fast_step(mine[e], I8 || p.fp8_direct);
+    }
 #pragma unroll 1
     for (uint32_t g = 0; g < kTransRows / 32; ++g) {
-        const uint32_t r = r0 + g * 32 + warp * 4;
+        const uint32_t r = r0 + g * 32 + first;
         uint32_t x[4][W];
         float2 v[4][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (in_row<VEC>(c0, span) && r + j < p.rows) load_piece<XT, VEC>(trans_row<XT>(p, p.row0 + r + j), c0, span, x[j]);
+            if (in_row<VEC>(c0, span) && r + j * kApart < p.rows) load_piece<XT, VEC>(trans_row<XT>(p, p.row0 + r + j * kApart) - shift, c0, span, x[j]);
             else {
 #pragma unroll
                 for (int k = 0; k < W; ++k) x[j][k] = 0;
@@ -1036,15 +1060,38 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) unpack<XT>(x[j], v[j]);
+        const auto put = [&](int e, uint32_t word) {
+            if (VEC != kPhased || element_column<VEC>(e, span.phase) >= 0) tile[element_slot<VEC>(e, span.phase) * kPitch + g * 8 + warp] = word;
+        };
+        const auto codes = [&](auto fast) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint32_t even = 2 * k * 32 + lane, odd = even + 32;
-            tile[even * kPitch + g * 8 + warp] = column_codes<I8, GIVEN>(p, make_float2(v[0][k].x, v[1][k].x), make_float2(v[2][k].x, v[3][k].x), steps[even]);
-            tile[odd * kPitch + g * 8 + warp] = column_codes<I8, GIVEN>(p, make_float2(v[0][k].y, v[1][k].y), make_float2(v[2][k].y, v[3][k].y), steps[odd]);
-        }
+            for (int k = 0; k < 4; ++k) {
+                put(2 * k, make_codes<I8, decltype(fast)::value>(make_float2(v[0][k].x, v[1][k].x), make_float2(v[2][k].x, v[3][k].x), mine[2 * k], p.hw));
+                put(2 * k + 1, make_codes<I8, decltype(fast)::value>(make_float2(v[0][k].y, v[1][k].y), make_float2(v[2][k].y, v[3][k].y), mine[2 * k + 1], p.hw));
+            }
+        };
+        if (all_fast) codes(std::true_type());
+        else codes(std::false_type());
     }
     __syncthreads();
-    const uint32_t rows = min(kTransRows, p.rows - r0), cols = min(256u, p.cols - c0);
+    if constexpr (VEC == kPhased) {
+        // word w of a step holds rows w, w + 8, w + 16, w + 24: put the bytes in the rows' order
+        for (uint32_t i = threadIdx.x; i < 256 * (kTransRows / 32); i += 256) {
+            uint32_t* w = tile + (i & 255) * kPitch + (i >> 8) * 8;
+            uint32_t o[8];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t a = w[4 * half], b = w[4 * half + 1], c = w[4 * half + 2], d = w[4 * half + 3];
+                const uint32_t ab = __byte_perm(a, b, 0x5140), cd = __byte_perm(c, d, 0x5140), ab2 = __byte_perm(a, b, 0x7362), cd2 = __byte_perm(c, d, 0x7362);
+                o[half] = __byte_perm(ab, cd, 0x5410); o[2 + half] = __byte_perm(ab, cd, 0x7632);
+                o[4 + half] = __byte_perm(ab2, cd2, 0x5410); o[6 + half] = __byte_perm(ab2, cd2, 0x7632);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k] = o[k];
+        }
+        __syncthreads();
+    }
+    const uint32_t rows = min(kTransRows, p.rows - r0), cols = min(kTransCols<VEC>, p.cols - c0);
     // nine 16-byte words cover a column's 128 bytes at any alignment, eight where they are aligned; neighbouring lanes take
     // neighbouring slots, whose words lie in different banks
     const bool aligned = ((reinterpret_cast<uintptr_t>(p.out) + p.row0 + r0) | p.out_ld) % 16 == 0;
@@ -1052,6 +1099,11 @@ __global__ void __launch_bounds__(256, 3) quant_trans_kernel(const __grid_consta
     for (uint32_t i = threadIdx.x; i < 256 * words; i += 256) {
         const uint32_t slot = aligned ? i / 8 : i / 9, k = i - slot * words, col = slot_column<VEC>(slot);
         if (col >= cols) continue;
+        if (aligned && 16 * k + 16 <= rows) {
+            const uint32_t* w = tile + slot * kPitch + 4 * k;
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0 + 16 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+            continue;
+        }
         uint8_t* a = static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0;
         const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u;
         const int begin = int(16 * k) - int(off);   // first row of the word

@@ -1,6 +1,6 @@
 // Instantiations of the row kernels and their launchers. The Makefile compiles this file once per variant with -DINST_XT=<1|2>
 // -DINST_VEC=<8|0|1> (element type of x, how rows lie: 0 is kPhased) and one of -DINST_NORM=<0|1|2> (element type of the residual),
-// -DINST_GRAD=<0|1> (with a gradient of the sum) and -DINST_TRANS (not for kPhased).
+// -DINST_GRAD=<0|1> (with a gradient of the sum) and -DINST_TRANS.
 #include <algorithm>
 
 #include "norm_quant.cuh"
@@ -89,9 +89,9 @@ cudaError_t quant_trans_of(const RowLaunch& env, const QuantTransParams& p, int*
     if (!p.given) {
         e = cudaMemsetAsync(p.scale, 0, size_t(p.cols) * sizeof(float), env.stream);
         if (e != cudaSuccess) return e;
-        // strips of 256 columns, cut along the rows into about eight blocks per SM, of at least 32 rows
-        const uint32_t strips = (p.cols + 255) / 256, want = (uint32_t(env.sm_count) * 8 + strips - 1) / strips;
-        const uint32_t cuts = std::max(1u, std::min((p.rows + 31) / 32, std::min(want, 65535u)));
+        // strips of 256 columns, cut along the rows into as many blocks as the SMs hold at once, of at least 32 rows
+        const uint32_t strips = (p.cols + kTransCols<VEC> - 1) / kTransCols<VEC>, held = uint32_t(env.sm_count) * (XT == ROW_BF16 ? 6 : 4);
+        const uint32_t cuts = std::max(1u, std::min((p.rows + 31) / 32, held / strips));
         e = launch_rows(env, column_max_kernel<XT, VEC>, p, dim3(strips, cuts), 256, 0);
         if (e != cudaSuccess) return e;
         ++*launches;
@@ -104,7 +104,7 @@ cudaError_t quant_trans_of(const RowLaunch& env, const QuantTransParams& p, int*
         QuantTransParams q = p;
         q.row0 = uint32_t(r);
         q.rows = uint32_t(std::min<uint64_t>(p.rows - r, uint64_t(65535) * kRows));
-        e = launch_rows(env, kern, q, dim3((p.cols + 255) / 256, (q.rows + kRows - 1) / kRows), 256, 0);
+        e = launch_rows(env, kern, q, dim3((p.cols + kTransCols<VEC> - 1) / kTransCols<VEC>, (q.rows + kRows - 1) / kRows), 256, 0);
         if (e != cudaSuccess) return e;
         ++*launches;
     }
