@@ -1092,36 +1092,34 @@ __global__ void __launch_bounds__(256, XT == ROW_BF16 ? 4 : 3) quant_trans_kerne
         __syncthreads();
     }
     const uint32_t rows = min(kTransRows, p.rows - r0), cols = min(kTransCols<VEC>, p.cols - c0);
-    // The aligned 16-byte words of every column (at most eight), then the bytes at its two ends, so that no warp does both. Neighbouring
-    // lanes take neighbouring slots, whose words lie in different banks.
-    uint8_t* const out = static_cast<uint8_t*>(p.out) + p.row0 + r0;
-    const auto column_of = [&](uint32_t slot, uint8_t** a) {
-        const uint32_t col = slot_column<VEC>(slot);
-        *a = out + uint64_t(c0 + col) * p.out_ld;
-        return col < cols;
-    };
-    for (uint32_t i = threadIdx.x; i < 256 * 8; i += 256) {
-        const uint32_t slot = i >> 3;
-        uint8_t* a;
-        if (!column_of(slot, &a)) continue;
-        const uint32_t begin = (0u - uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u) + 16 * (i & 7);
-        if (begin + 16 > rows) continue;
-        const uint32_t *w = tile + slot * kPitch + (begin >> 2), sh = (begin & 3u) * 8;
-        uint32_t o[4];
+    // nine 16-byte words cover a column's 128 bytes at any alignment, eight where they are aligned; neighbouring lanes take
+    // neighbouring slots, whose words lie in different banks
+    const bool aligned = ((reinterpret_cast<uintptr_t>(p.out) + p.row0 + r0) | p.out_ld) % 16 == 0;
+    const uint32_t words = aligned ? 8 : 9;
+    for (uint32_t i = threadIdx.x; i < 256 * words; i += 256) {
+        const uint32_t slot = aligned ? i / 8 : i / 9, k = i - slot * words, col = slot_column<VEC>(slot);
+        if (col >= cols) continue;
+        if (aligned && 16 * k + 16 <= rows) {
+            const uint32_t* w = tile + slot * kPitch + 4 * k;
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0 + 16 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+            continue;
+        }
+        uint8_t* a = static_cast<uint8_t*>(p.out) + uint64_t(c0 + col) * p.out_ld + p.row0 + r0;
+        const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u;
+        const int begin = int(16 * k) - int(off);   // first row of the word
+        if (begin >= int(rows)) continue;
+        const uint32_t* column = tile + slot * kPitch;
+        if (begin >= 0 && begin + 16 <= int(rows)) {
+            const uint32_t w0 = uint32_t(begin) >> 2, sh = (uint32_t(begin) & 3u) * 8;
+            uint32_t w[5], o[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], sh);   // the last word (the padding, at the end) counts only when sh != 0
-        *reinterpret_cast<uint4*>(a + begin) = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-    for (uint32_t i = threadIdx.x; i < 256 * 2; i += 256) {
-        const uint32_t slot = i & 255;
-        uint8_t* a;
-        if (!column_of(slot, &a)) continue;
-        const uint32_t off = uint32_t(reinterpret_cast<uintptr_t>(a)) & 15u, head = min(rows, (16 - off) & 15u), tail = (off + rows) & 15u;
-        const uint32_t begin = i < 256 ? 0 : rows - tail, count = i < 256 ? head : (head + tail <= rows ? tail : 0);
-        const uint8_t* bytes = reinterpret_cast<const uint8_t*>(tile + slot * kPitch);
+            for (int j = 0; j < 5; ++j) w[j] = column[w0 + j];   // the fifth word (the padding, at the end) counts only when sh != 0
 #pragma unroll
-        for (uint32_t k = 0; k < 15; ++k)
-            if (k < count) a[begin + k] = bytes[begin + k];
+            for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], sh);
+            *reinterpret_cast<uint4*>(a + begin) = make_uint4(o[0], o[1], o[2], o[3]);
+        } else {
+            for (int r = max(begin, 0); r < min(begin + 16, int(rows)); ++r) a[r] = uint8_t(column[r >> 2] >> (8 * (r & 3)));
+        }
     }
 }
 __device__ __forceinline__ void column_steps(float* scale, uint32_t cols, float top) {
