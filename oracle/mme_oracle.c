@@ -18,7 +18,7 @@
 
 enum { RM_NE = 0, RM_Z = 1, RM_UP = 2, RM_DOWN = 3, RM_SR = 4, RM_HAZ = 6, RM_SR_NE_DNORM = 7 };
 enum { T_FP8_143 = 9, T_FP8_152 = 10, T_BF16 = 12, T_FP32 = 13 };
-enum { OP_FWD = 0, OP_DEDX = 1, OP_DEDW = 2, OP_DET_DEDW = 3, OP_AB = 5, OP_ABT = 6, OP_ATB = 7, OP_ATBT = 8 };
+enum { OP_FWD = 0, OP_DEDX = 1, OP_DEDW = 2, OP_DET_DEDW = 3, OP_TRANSPOSED_DEDX = 4, OP_AB = 5, OP_ABT = 6, OP_ATB = 7, OP_ATBT = 8 };
 
 #define F32_NAN 0x7FFFFFFFu
 
@@ -520,6 +520,28 @@ int mo_conv(int threads, mo_tensor* out, const mo_tensor* x, const mo_tensor* w,
             const mo_conv_params* p, int op, int rm)
 {
     if (op == OP_DET_DEDW) op = OP_DEDW;
+    if (op == OP_TRANSPOSED_DEDX) {
+        /* impl:625-647: dedx on the weights with their two fastest dims swapped and S mirrored */
+        if (!supported_in(w->dtype)) return -2;
+        const size_t elem = (size_t) elem_size(w->dtype);
+        mo_tensor v = *w;
+        v.sizes[0] = w->sizes[1];
+        v.sizes[1] = w->sizes[0];
+        size_t n = 1;
+        for (int d = 0; d < 5; d++) { v.strides[d] = (uint32_t) n; n *= v.sizes[d]; }
+        v.data = malloc(n * elem + 1);
+        size_t at[5];
+        for (size_t i = 0; i < n; i++) {
+            size_t rest = i, off = 0;
+            for (int d = 0; d < 5; d++) { at[d] = rest % v.sizes[d]; rest /= v.sizes[d]; }
+            const size_t from[5] = {at[1], at[0], w->sizes[2] - 1 - at[2], at[3], at[4]};
+            for (int d = 0; d < 5; d++) off += from[d] * w->strides[d];
+            memcpy((char*) v.data + i * elem, (const char*) w->data + off * elem, elem);
+        }
+        const int rc = mo_conv(threads, out, x, &v, y, p, OP_DEDX, rm);
+        free(v.data);
+        return rc;
+    }
     if (op != OP_FWD && op != OP_DEDX && op != OP_DEDW) return -2;
     if (out->dtype != T_FP32) return -2;
     const size_t C = x->sizes[0], Kout = w->sizes[0];
