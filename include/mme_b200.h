@@ -184,7 +184,9 @@ int mmeb200_set_accumulation(mmeb200_ctx* ctx, int mode);
  * (CTA-pair kernel: 1 = the tiles of a ragged last wave are cut along K among the CTA pairs wherever a cut exists; off by
  * default, it did not pay on the shapes measured), "dependent_launch" (0 = the tcgen05 GEMM kernels are launched without programmatic
  * stream serialisation; with it, the kernel's set-up overlaps the tail of the kernel before it in the stream and it touches
- * memory only after that kernel has completed). The same knobs take their defaults from environment variables read once in
+ * memory only after that kernel has completed), and for the scaled products of few tokens "token_tile" (tokens per tile, rounded up
+ * to a multiple of 16), "token_split" (1..8 CTAs that share a tile's common dimension) and "token_ctas" (1 or 2 CTAs per SM), each
+ * followed where the sizes have that form; "pair" chooses between the two kernels of scaled products as well. The older knobs take their defaults from environment variables read once in
  * mmeb200_create (MME_B200_PAIR, MME_B200_BLOCK_N, MME_B200_SPLIT_K, MME_B200_EPI_GROUPS, MME_B200_GM,
  * MME_B200_NO_TMA_STORE, MME_B200_NO_HOST_PIPELINE, MME_B200_TILE_N, MME_B200_STREAM_K, MME_B200_DEPENDENT_LAUNCH); no launch
  * reads the environment. Results do not depend on the knobs beyond the accumulation tolerance (summation order). */

@@ -7,6 +7,13 @@
 // 8-bit output: with a = max |v|, step = a / top, every code is the nearest representable value to the 32-bit quotient
 // v / step (ties to even), and the row's scale is step * inv. inv does not enter the codes, so sum and maximum are taken in
 // one pass, and the codes do not depend on the order of any sum: they are fixed by the definition, bit for bit.
+//
+// A row takes a warp (up to 1024 columns), a block (32 columns a thread, 64 past 16384), or a loop that reads it twice. Blocks are
+// not kept over rows: the next row's loads come from the block beside it, two of 512 threads per SM. Measured against what has to
+// be read and written at 6549 GB/s: 8192 x 8192 bf16 with residual to int8 70.9 us (101 %), 16384 x 4096 with an fp32 residual to
+// bf16 119 us (103 %), quantisation of 2048 x 28672 bf16 33.4 us (81 %) and 8192 x 8192 fp32 54.8 us (94 %), 8192 x 4999 (odd
+// rows) 61 us (72 %: gamma's words are shifted for every row). 200000 rows of 128 columns take 54 us (22 %): a block lives for
+// four short rows and what bounds it is the rate at which blocks start.
 #pragma once
 #include <type_traits>
 
@@ -649,7 +656,9 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
 // With a = dy * gamma, u = x * inv:  dx = inv * (a - u * mean(a * u)) + dsum,  dgamma = sum over rows of dy * u.
 // mean(a * u) = inv * mean(a * x), so both sums of a row (x^2 and a * x) are taken in one pass. A block walks rows b, b +
 // blocks, ...; every thread keeps the sums of its own columns of dgamma, and the block's partial sums (one row of `partial`)
-// are added in a fixed order by column_sums: results do not depend on timing.
+// are added in a fixed order by column_sums: results do not depend on timing. HBM bounds it: 16384 x 4096 bf16 67.6 us (91 % of the
+// copy rate), 91 us with the sum's gradient (90 %), 2048 x 16384 54 us (76 %, two blocks of a cluster per row); 8000 rows of 1000
+// columns 19.5 us (38 %), where the block's first row and the second launch weigh most.
 //
 // a (dy * gamma) becomes dx; acc += dy * u.
 template <bool DSUM>
@@ -1013,6 +1022,8 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
     for (int i = 1; i < 8; ++i) t = max_nan(t, part[i][threadIdx.x]);
     atomicMax(reinterpret_cast<uint32_t*>(p.scale) + mine, __float_as_uint(t) & 0x7FFFFFFFu);
 }
+// Both passes together: 8192 x 8192 bf16 64 us, where reading x twice and writing once is 51 us; 8191 x 8193 112 us (the ends of the
+// result's rows are written byte by byte; in a pass of their own that was 121 us).
 // Tiles of 128 rows x 256 columns (248 phased): a warp takes four rows at a time, a lane eight of their columns, whose codes make one
 // word per column. The tile's columns leave as aligned 16-byte words (byte by byte at their ends). Four blocks per SM hide one's
 // loads behind another's stores: 8192 x 8192 bf16 64 us, with three and rows read a step ahead 68 us.

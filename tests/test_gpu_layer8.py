@@ -196,6 +196,28 @@ def test_norm_zero_rows_and_rows_that_hold_no_number(calc, dev, port, cols, ot):
     check_norm(calc, dev, port, 8, cols, abi.FP32, None, None, ot, values=v)
 
 
+@pytest.mark.parametrize("cols", [5, 41, 249, 257, 1019, 4999, 16381, 33001])
+@pytest.mark.parametrize("ot", [abi.INT8, abi.FP8_143, abi.BF16])
+def test_rows_of_odd_length_do_not_see_their_neighbours(calc, dev, port, cols, ot):
+    """Rows one behind the other: the words at a row's ends hold its neighbours' values too, here numbers and no numbers in turn."""
+    rng = np.random.default_rng([21, cols])
+    v = rows_like(rng, 17, cols)
+    v[1::2] = np.nan
+    v[3::4] = -np.inf
+    if ot != abi.BF16:
+        check_norm(calc, dev, port, 17, cols, abi.BF16, None, abi.FP32, ot, values=v)
+        check_norm(calc, dev, port, 17, cols, abi.FP32, None, abi.BF16, ot, values=v)
+        return
+    tx, to = dev.put(encode(v, abi.BF16)[0], abi.BF16), dev.put(np.zeros((17, cols), np.uint16), abi.BF16)
+    calc.rms_norm(to, tx, None, EPS)
+    calc.sync()
+    out, x = decode(dev.get(to), abi.BF16), encode(v, abi.BF16)[1]
+    want = layer8.norm(x[::2], np.ones(cols), EPS)[0]
+    # (one rounding to bf16, and the reciprocal root's error, far below it)
+    assert (np.abs(out[::2] - want) <= np.abs(want) * (2.0 ** -8 + 2 * layer8.inverse_bound(cols))).all()
+    assert np.isnan(out[1::2]).all()
+
+
 def test_norm_float_rows_that_hold_no_number(calc, dev):
     v = np.ones((3, 300), np.float32)
     v[0, 7] = np.nan
@@ -296,7 +318,7 @@ def test_quantize_given_scale_values(calc, dev, port):
 
 
 # ------------------------------------------------------------------------------------------ quantisation
-@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 300), (300, 1), (63, 65), (64, 64), (65, 63), (130, 1000), (1000, 130), (2049, 40), (17, 4100)])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 300), (300, 1), (63, 65), (64, 64), (65, 63), (130, 1000), (1000, 130), (2049, 40), (17, 4100), (137, 249), (128, 248), (9, 497), (265, 1001)])
 @pytest.mark.parametrize("xt", [abi.BF16, abi.FP32])
 def test_quantize_transposed(calc, dev, port, rows, cols, xt):
     rng = np.random.default_rng([9, rows, cols])
@@ -362,6 +384,20 @@ def test_grad_over_lengths(calc, dev, cols, xt):
 def test_grad_rows(calc, dev, rows):
     grad_case(calc, dev, rows, 48, abi.BF16, None, True, seed=2)
     grad_case(calc, dev, rows, 1032, abi.FP32, abi.FP32, False, seed=2, workspace=True)
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 8193), (40, 8200), (700, 8209), (9, 16384), (3, 20001), (2, 40000), (2, 65529), (3, 65536), (3, 65543), (2, 70001)])
+def test_grad_of_rows_that_blocks_share(calc, dev, rows, cols):
+    grad_case(calc, dev, rows, cols, abi.BF16, abi.FP32, True, seed=4)
+    grad_case(calc, dev, rows, cols, abi.FP32, abi.BF16, False, seed=4, workspace=True)
+
+
+@pytest.mark.parametrize("rows,cols", [(2601, 9), (2601, 249), (2501, 257), (1499, 1019), (1400, 1021), (613, 4099)])
+def test_grad_of_odd_rows_in_many_turns(calc, dev, rows, cols):
+    """A block walks several rows; all of them lie equally far past eight elements."""
+    grad_case(calc, dev, rows, cols, abi.BF16, abi.BF16, True, seed=5)
+    grad_case(calc, dev, rows, cols, abi.BF16, abi.FP32, False, seed=5, pitch=1, offset=3)
+    grad_case(calc, dev, rows, cols, abi.FP32, None, False, seed=5)
 
 
 @pytest.mark.parametrize("pitch,offset", [(0, 1), (3, 0), (8, 0), (24, 5)])
@@ -492,6 +528,21 @@ def test_product_pair_kernel(calc, dev, port, m, n, k, groups):
     finally:
         calc.set_option("pair", -1)
         calc.set_option("epi_groups", -1)
+
+
+@pytest.mark.parametrize("ctas", [1, 2])
+@pytest.mark.parametrize("tile,split", [(16, 1), (16, 2), (16, 3), (32, 4), (48, 5), (64, 6), (80, 7), (128, 8), (256, 1), (256, 8), (7, 8)])
+def test_product_forms_of_the_token_kernel(calc, dev, port, tile, split, ctas):
+    knobs = {"pair": 0, "token_tile": tile, "token_split": split, "token_ctas": ctas}
+    for name, value in knobs.items():
+        calc.set_option(name, value)
+    try:
+        check_product(calc, dev, port, 37, 200, 1296, bias_t=abi.FP32)
+        check_product(calc, dev, port, 130, 140, 2000, xt=abi.FP8_143, ot=abi.FP32)
+        check_product(calc, dev, port, 5, 300, 100)   # fewer k blocks than the split asks for
+    finally:
+        for name in knobs:
+            calc.set_option(name, -1)
 
 
 def test_product_token_kernel_on_many_tiles(calc, dev, port):
@@ -746,7 +797,6 @@ def test_streams_graphs_and_two_contexts(port):
     for _ in range(10):
         calc.set_stream(stream.cuda_stream)
         go(0, False)
-        first = dg.clone() if False else None
         calc.set_stream(other.cuda_stream)
         other.wait_stream(stream)
         go(0, False)
