@@ -190,6 +190,7 @@ void layer_flatten(uint32_t (&dims)[4], uint32_t* flat, std::initializer_list<Ro
 // How the rows of these tensors and gamma lie: 8, kPhased (where `phases` allows it) or 1 (norm_quant.h).
 int layer_vector(uint32_t cols, const uint32_t (&dims)[4], std::initializer_list<const RowTensor*> all, const void* gamma, const void* partial, bool phases) {
     bool eight = cols % 8 == 0 && reinterpret_cast<uintptr_t>(partial) % 16 == 0;
+    phases = phases && cols < (1u << 30);   // (phased columns are counted in 32 bits with a sign)
     const RowTensor* first = *all.begin();
     const auto elements = [](const RowTensor* t) { return reinterpret_cast<uintptr_t>(t->ptr) / (t->type >= ROW_I8 ? 1 : t->type == ROW_BF16 ? 2 : 4); };
     for (const RowTensor* t : all) {

@@ -1,6 +1,9 @@
 """The 8-bit layer operators on the GPU: RMS norm with the residual's addition and 8-bit rows, its gradient, quantisation,
 scaled products, and a run of them together. Bounds: tests/layer8.py."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -809,6 +812,52 @@ def test_streams_graphs_and_two_contexts(port):
     check(0)
     for st in state:
         st[0].close()
+
+
+FIRST_CALLS_CAPTURED = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from intel_gaudi3_software_b200 import Calculator, abi
+kinds = {torch.bfloat16: abi.BF16, torch.float32: abi.FP32, torch.int8: abi.INT8}
+def t(a):
+    return abi.make_tensor(a.data_ptr(), kinds[a.dtype], list(reversed(a.shape)), list(reversed(a.stride())), mem_space=abi.MEM_DEVICE)
+stream = torch.cuda.Stream()
+calc = Calculator(device=0)
+calc.set_stream(stream.cuda_stream)
+rows, cols, n = 12, 9104, 136
+x, dy = (torch.randn(rows, cols, device="cuda").bfloat16() for _ in range(2))
+w, gamma = torch.randn(cols, n, device="cuda").bfloat16(), torch.rand(cols, device="cuda")
+outs = [torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros(n, cols, dtype=torch.int8, device="cuda"),
+        torch.zeros(n, device="cuda"), torch.zeros(rows, n, device="cuda"), torch.zeros_like(x), torch.zeros(cols, device="cuda")]
+work = torch.zeros(calc.rms_norm_grad_workspace(rows, cols) // 4, device="cuda")
+q, s, wq, ws, y, dx, dg = (t(o) for o in outs)
+def run():
+    calc.rms_norm(q, t(x), t(gamma), 1e-5, scale=s)
+    calc.quantize(wq, ws, t(w), abi.OP_TRANS)
+    calc.scaled_gemm(y, q, s, wq, ws)
+    calc.rms_norm_grad(dx, dg, t(dy), t(x), t(gamma), 1e-5, workspace=t(work))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=stream):
+    run()
+graph.replay()
+torch.cuda.synchronize()
+replayed = [o.clone() for o in outs]
+for o in outs:
+    o.zero_()
+torch.cuda.synchronize()
+run()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(replayed, outs)) and all(o.any() for o in outs)
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    """Nothing that a call sets up once keeps it from being captured."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_CAPTURED, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
 
 
 # ------------------------------------------------------------------------------------------ refusals
