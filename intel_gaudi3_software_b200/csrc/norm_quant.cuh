@@ -74,7 +74,8 @@ __device__ __forceinline__ void store_element(uint8_t* a, const uint32_t (&w)[W]
 }
 // The eight elements of a lane, packed. Columns from `c0` on (in_row); those outside the span read as zeros, of a phased row once
 // trim_piece has cleared them: there the aligned 16 bytes around a row's ends are read whole (none without a byte of the row), so
-// that no lane goes another way while loads are issued. `row` is where column 0 would be.
+// that no lane goes another way while loads are issued (a branch for the ends: 79 us where this takes 71, 8192 x 4999). Such a word
+// lies in the page of the byte it shares with the row. `row` is where column 0 would be.
 template <int TYPE, int VEC, int W>
 __device__ __forceinline__ void load_piece(const void* row, uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[W]) {
     constexpr int kBytes = RowElem<TYPE>::kBytes;
