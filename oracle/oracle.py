@@ -83,7 +83,7 @@ class _Base:
 
 
 class Port(_Base):
-    """The plain-C restatement (Gaudi3 model, bf16/fp8 operands)."""
+    """The plain-C restatement (Gaudi3 model; bf16 / fp8 operands, fp32 and tf32 ones in GEMMs)."""
     prefix = "mo_"
     kind = "port"
 
