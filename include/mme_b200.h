@@ -414,7 +414,10 @@ size_t mmeb200_rms_norm_grad_workspace(const mmeb200_ctx* ctx, uint64_t rows, ui
 int mmeb200_quantize(mmeb200_ctx* ctx, mmeb200_tensor* out, mmeb200_tensor* scale, const mmeb200_tensor* x, int op, int scale_mode);
 
 /* Product of 8-bit operands with a scale for each token and channel, both [K, rows] with K contiguous (op MMEB200_OP_ABT):
- *   out[n, m] = (sum_k x[k, m] * w[k, n]) * x_scale[m] * w_scale[n] + bias[n],  rounded once.
+ *   out[n, m] = (sum_k x[k, m] * w[k, n]) * x_scale[m] * w_scale[n] + bias[n].
+ * Roundings: the sum to 32 bits, its product with x_scale[m] to 32 bits, that times w_scale[n] plus bias[n] to 32 bits (one fused
+ * operation), the result to out's type. int8 sums are exact before their rounding, so an int8 product's row has the same bits
+ * whatever the other rows, the kernel and the knobs; fp8 sums may differ in their order.
  *   x, w: both int8 (any code, -128 included; the sum is exact, K <= 131071), or both fp8 (1-4-3 'minimal' or 1-5-2 'full', any
  *   exponent bias; fp32 sum on the tensor cores). x_scale, w_scale: dense fp32, one element per row or one for all.
  *   bias: bf16 or fp32, dense, may be NULL. out: bf16 or fp32, any row pitch. K = 0 gives the bias, or zeros.

@@ -614,8 +614,9 @@ __device__ __forceinline__ void stage_columns(const GemmParams& p, float* cols, 
         cols[kScaledCols + i] = there && p.scaled.col_bias ? scaled_bias(p.scaled, n) : 0.0f;
     }
 }
-// 32 accumulator columns of a row whose scale is xs -> packed bf16 or fp32 outputs, rounded once. cols: the staged scales of
-// these columns.
+// 32 accumulator columns of a row whose scale is xs -> packed bf16 or fp32 outputs: acc * xs is rounded, then its product with
+// the column's scale, together with the bias where there is one, as in the few-token kernel: equal sums give equal outputs.
+// cols: the staged scales of these columns.
 template <int KIND>
 __device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const float* cols, bool has_bias, float xs, uint32_t out_elem) {
 #pragma unroll
@@ -623,12 +624,15 @@ __device__ __forceinline__ void epilogue_scaled(uint32_t (&v)[32], const float* 
         const float4 w = reinterpret_cast<const float4*>(cols)[q];
         float2 y0 = make_float2(scaled_acc<KIND>(v[4 * q]), scaled_acc<KIND>(v[4 * q + 1]));
         float2 y1 = make_float2(scaled_acc<KIND>(v[4 * q + 2]), scaled_acc<KIND>(v[4 * q + 3]));
-        y0 = __fmul2_rn(__fmul2_rn(y0, make_float2(xs, xs)), make_float2(w.x, w.y));
-        y1 = __fmul2_rn(__fmul2_rn(y1, make_float2(xs, xs)), make_float2(w.z, w.w));
+        y0 = __fmul2_rn(y0, make_float2(xs, xs));
+        y1 = __fmul2_rn(y1, make_float2(xs, xs));
         if (has_bias) {
             const float4 b = reinterpret_cast<const float4*>(cols + kScaledCols)[q];
-            y0 = __fadd2_rn(y0, make_float2(b.x, b.y));
-            y1 = __fadd2_rn(y1, make_float2(b.z, b.w));
+            y0 = __ffma2_rn(y0, make_float2(w.x, w.y), make_float2(b.x, b.y));
+            y1 = __ffma2_rn(y1, make_float2(w.z, w.w), make_float2(b.z, b.w));
+        } else {
+            y0 = __fmul2_rn(y0, make_float2(w.x, w.y));
+            y1 = __fmul2_rn(y1, make_float2(w.z, w.w));
         }
         if (out_elem == 2) {   // words 2q, 2q + 1 lie below every value still to be read
             asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v[2 * q]) : "f"(y0.y), "f"(y0.x));

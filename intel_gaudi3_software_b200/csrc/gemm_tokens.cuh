@@ -40,8 +40,8 @@ __device__ __forceinline__ void token_put(const TokenGemmParams& p, uint32_t m, 
         static_cast<float*>(p.out)[uint64_t(m) * p.out_ld + n] = y;
     }
 }
-// COUNT consecutive tokens of this lane's channel: acc * (the token's scale, held by lane `place` + j) * ws + bias. `exist` of
-// them exist. All values first, then all stores: nothing waits between two of them.
+// COUNT consecutive tokens of this lane's channel: acc * (the token's scale, held by lane `place` + j), rounded, then * ws + bias in
+// one operation, as in the CTA-pair kernel (epilogue_scaled). `exist` of them exist. All values first, then all stores: nothing waits between two of them.
 template <int KIND, bool BF16, int COUNT>
 __device__ __forceinline__ void token_put_all(const TokenGemmParams& p, const uint32_t* v, uint32_t m, uint32_t exist, uint32_t n, float scales, uint32_t place, float ws,
                                               float bias) {
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) gemm_tokens_kernel(const __g
     griddep_wait();
 
     const uint32_t sub = warp & 3, grp = (warp - 2) >> 2, n = n0 + sub * 32 + lane;   // epilogue: this lane's channel
-    float ws = 0.0f, bias = 0.0f;
+    float ws = 0.0f, bias = -0.0f;   // (no bias: minus zero, which leaves every sum as it is)
     bool ready = true;
     if (warp == 0) {
         if (elect_one()) {

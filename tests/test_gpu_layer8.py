@@ -629,6 +629,42 @@ def test_product_scales_that_are_no_number(calc, dev):
         assert np.isnan(out[2]).all() and (np.delete(out, 2, axis=0) == 0).all()
 
 
+@pytest.mark.parametrize("ot", [abi.FP32, abi.BF16])
+@pytest.mark.parametrize("bias_t", [None, abi.FP32, abi.BF16])
+def test_product_int8_rows_do_not_depend_on_the_kernel(calc, dev, ot, bias_t):
+    """Integer sums are exact, so both kernels round the same numbers in the same way; so does a row alone. Signs of zeros too."""
+    rng = np.random.default_rng(17)
+    m, n, k = 300, 1112, 1040
+    x, w = rng.integers(-128, 128, (m, k)).astype(np.int8), rng.integers(-128, 128, (n, k)).astype(np.int8)
+    x[::7] = 0
+    xs, ws = rng.standard_normal(m).astype(np.float32), rng.standard_normal(n).astype(np.float32)
+    bias = None if bias_t is None else encode(rng.standard_normal(n) * 50, bias_t)[0]
+    tx, tw, txs, tws = dev.put(x, abi.INT8), dev.put(w, abi.INT8), dev.put(xs, abi.FP32), dev.put(ws, abi.FP32)
+    tb = None if bias is None else dev.put(bias, bias_t)
+    rows = {}
+    for form, knobs in {"pair": {"pair": 1}, "pair, no tensor map": {"pair": 1, "tma_store": 0}, "few tokens": {"pair": 0, "token_split": 1}, "few tokens, split": {"pair": 0, "token_split": 5}}.items():
+        to = dev.put(np.ones((m, n), abi.NP_DTYPE[ot]), ot)
+        for name, value in knobs.items():
+            calc.set_option(name, value)
+        try:
+            calc.scaled_gemm(to, tx, txs, tw, tws, bias=tb)
+        finally:
+            for name in knobs:
+                calc.set_option(name, -1)
+        calc.sync()
+        rows[form] = dev.get(to).view(np.uint8)
+    alone = dev.put(np.ones((2, n), abi.NP_DTYPE[ot]), ot)
+    calc.scaled_gemm(alone, dev.put(x[40:42], abi.INT8), dev.put(xs[40:42], abi.FP32), tw, tws, bias=tb)
+    calc.sync()
+    for form, got in rows.items():
+        assert (got == rows["pair"]).all(), form
+    assert (dev.get(alone).view(np.uint8) == rows["pair"][40:42]).all()
+    if bias is None:   # the definition's two products, bit for bit
+        with np.errstate(all="ignore"):
+            y = ((x.astype(np.int64) @ w.astype(np.int64).T).astype(np.float32) * xs[:, None]) * ws
+        assert (rows["pair"] == np.ascontiguousarray(encode(y, ot)[0]).view(np.uint8)).all()
+
+
 # ------------------------------------------------------------------------------------------ together, host tensors, streams, graphs
 def test_layer_run(calc, dev, port):
     """norm with the residual's addition -> 8-bit product -> norm of the sum -> 8-bit product, as a layer uses them, against 64 bits."""
