@@ -18,6 +18,7 @@
 #include "gemm_tokens.h"
 #include "gaudi3_exact.cuh"
 #include "kernels.cuh"
+#include "layer_host.h"
 #include "mme_b200.h"
 #include "norm_quant.h"
 

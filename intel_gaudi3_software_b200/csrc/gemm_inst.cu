@@ -72,7 +72,7 @@ LaunchResult INST_NAME(const LaunchEnv& env, const GemmParams& p, uint64_t tiles
     cfg.attrs = &attr;
     cfg.numAttrs = env.dependent_launch ? 1 : 0;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, gemm_tcgen05_pair_kernel<INST_KIND, INST_PAIR_EPI, INST_PAIR_CUT != 0, INST_PAIR_SCALED != 0>, p);
-    return {e != cudaSuccess ? e : cudaGetLastError(), LAUNCH_OK, "pair kernel launch"};
+    return {e, LAUNCH_OK, "pair kernel launch"};
 }
 
 #else

@@ -46,7 +46,7 @@ static LaunchResult launch(const LaunchEnv& env, TokenGemmParams& p) {
     while (p.tmem_cols < p.tok) p.tmem_cols *= 2;
     cfg.gridDim = dim3(p.splits * ((p.N + kBlockM - 1) / kBlockM), (p.M + p.tok - 1) / p.tok);
     e = cudaLaunchKernelEx(&cfg, gemm_tokens_kernel<KIND>, p);
-    return {e != cudaSuccess ? e : cudaGetLastError(), LAUNCH_OK, "few-token kernel launch"};
+    return {e, LAUNCH_OK, "few-token kernel launch"};   // (not the thread's last error, which may be an older one of the caller's)
 }
 
 LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmParams p) {
@@ -54,25 +54,29 @@ LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmPa
 }
 
 template <int KIND>
-static int capacity(const LaunchEnv& env, uint32_t tok, uint32_t splits, uint32_t ctas) {
+static bool capacity(const LaunchEnv& env, uint32_t tok, uint32_t splits, uint32_t ctas, int* n) {
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attrs[2];
-    if (configure<KIND>(env, tok, splits, ctas, &cfg, attrs) != cudaSuccess) return 0;
+    if (configure<KIND>(env, tok, splits, ctas, &cfg, attrs) != cudaSuccess) return false;
     cfg.gridDim = dim3(splits * unsigned(env.sm_count));
     cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, gemm_tokens_kernel<KIND>, &cfg) != cudaSuccess) return 0;
-    return n * int(splits);
+    if (cudaOccupancyMaxActiveClusters(n, gemm_tokens_kernel<KIND>, &cfg) != cudaSuccess) return false;
+    *n *= int(splits);
+    return true;
 }
 
 LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p) {
     const uint64_t blocks = (uint64_t(p.M) * p.N + 255) / 256, most = uint64_t(env.sm_count) * 8;
-    gemm_empty_sum_kernel<<<unsigned(blocks < most ? blocks : most), 256, 0, env.stream>>>(p);
-    return {cudaGetLastError(), LAUNCH_OK, "empty-sum kernel launch"};
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(unsigned(blocks < most ? blocks : most));
+    cfg.blockDim = dim3(256);
+    cfg.stream = env.stream;
+    return {cudaLaunchKernelEx(&cfg, gemm_empty_sum_kernel, p), LAUNCH_OK, "empty-sum kernel launch"};
 }
 
-int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
-    return kind == KIND_I8 ? capacity<KIND_I8>(env, tok, splits, ctas) : capacity<KIND_F8>(env, tok, splits, ctas);
+bool gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas, int* n) {
+    return kind == KIND_I8 ? capacity<KIND_I8>(env, tok, splits, ctas, n) : capacity<KIND_F8>(env, tok, splits, ctas, n);
 }
 
 }  // namespace mmeb200

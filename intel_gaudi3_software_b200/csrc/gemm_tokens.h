@@ -31,8 +31,8 @@ struct TokenGemmParams {
 LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmParams p);
 // out = bias (or zero) for operands without a common dimension.
 LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p);
-// Most CTAs the device runs at once in clusters of `splits` with tiles of `tok` tokens (0 on failure).
-int gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas);
+// Most CTAs the device runs at once in clusters of `splits` with tiles of `tok` tokens; false where the question fails.
+bool gemm_tokens_capacity(const LaunchEnv& env, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas, int* n);
 // Stages of the ring of a CTA, one of `ctas` on its SM; fewer than three do not keep the tensor cores fed.
 uint32_t gemm_tokens_stages(uint32_t tok, uint32_t ctas);
 

@@ -147,7 +147,7 @@ struct LayerStage {
     int finish() {
         for (int i = 0; i < n; ++i)
             if (is_out[i]) TRY(stage_out(c, &staged[i]));
-        return finish_call(c, any_host);
+        return any_host ? collect_status(c) : 0;   // (every CUDA call's own status was looked at)
     }
 };
 
@@ -464,13 +464,9 @@ int layer_pad_operand(mmeb200_ctx* c, TmaOperand* o, uint8_t* dst) {
 }
 
 int layer_token_capacity(mmeb200_ctx* c, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
-    static int caps[64][2][4][9] = {};   // of the full ring, which all tiles nearly have
-    int& cap = caps[c->device & 63][kind == KIND_I8][ctas][splits];
-    if (cap == 0) {
-        cap = gemm_tokens_capacity(launch_env(c), kind, tok, splits, ctas);
-        if (cap == 0) cap = -1;
-    }
-    return cap;
+    static std::atomic<int> known[64][2][4][9] = {};   // of the full ring, which all tiles nearly have
+    return device_holds(known[c->device & 63][kind == KIND_I8][ctas][splits], [&](int* n) { return gemm_tokens_capacity(launch_env(c), kind, tok, splits, ctas, n); },
+                        [] { cudaGetLastError(); });
 }
 // Which kernel a product takes, and with what tile and split: the choice with the least estimated time, a function of the
 // sizes alone. The estimates (microseconds) are sums of a few measured rates, which reproduce the measured times of some

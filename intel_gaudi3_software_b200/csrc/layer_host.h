@@ -1,0 +1,25 @@
+// Host-side bookkeeping of the 8-bit layer operators, without a CUDA call of its own (the tests compile it without a GPU).
+#pragma once
+#include <atomic>
+
+namespace mmeb200 {
+
+// How much of a kernel the device holds at once: `ask(&n)` puts the question when it first comes up (and is false where it fails),
+// `known` keeps the answer. A failed question only rules out what needs the answer: `forget` clears the error that it left, and
+// the result is `instead`, which is kept where it is a usable number (not negative: also for the answer "none"), else asked again.
+template <typename Ask, typename Forget>
+int device_holds(std::atomic<int>& known, Ask&& ask, Forget&& forget, int instead = -1) {
+    int n = known.load(std::memory_order_relaxed);   // the answer + 1
+    if (n) return n - 1;
+    if (!ask(&n)) {
+        forget();
+        n = instead;
+        if (n < 0) return n;
+    } else if (n <= 0) {
+        n = instead > 0 ? instead : 0;
+    }
+    known.store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+
+}  // namespace mmeb200

@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <atomic>
 
+#include "layer_host.h"
 #include "norm_quant.cuh"
 #include "norm_quant_launch.h"
 
@@ -24,14 +25,9 @@ uint32_t norm_grad_blocks(int device, int sm_count, uint32_t rows, uint32_t cols
     uint64_t held = uint64_t(sm_count) * g.blocks_per_sm;
     if (g.form == GRAD_CLUSTER) {
         static std::atomic<int> known[64][9][9] = {};   // by device, ranks and warps
-        std::atomic<int>& entry = known[device & 63][g.ranks][g.threads / 32];
-        int n = entry;
-        if (n == 0) {
-            n = norm_grad_clusters(g.ranks, g.threads);
-            if (n <= 0) n = std::max(1, sm_count / int(g.ranks));
-            entry = n;
-        }
-        held = uint64_t(n);
+        // (any number is right; it is kept, so that the workspace asked for is the one the call wants)
+        held = uint64_t(device_holds(known[device & 63][g.ranks][g.threads / 32], [&](int* n) { return norm_grad_clusters(g.ranks, g.threads, n); }, [] { cudaGetLastError(); },
+                                     std::max(1, sm_count / int(g.ranks))));
     }
     return uint32_t(std::min<uint64_t>((uint64_t(rows) + g.rows_per_block - 1) / g.rows_per_block, held));
 }

@@ -58,9 +58,9 @@ template cudaError_t norm_grad_of<INST_XT, INST_GRAD != 0, INST_VEC>(const RowLa
 
 #if INST_XT == 1 && INST_GRAD == 1 && INST_VEC == 8
 // Of the form that needs most shared memory; all have the same registers.
-int norm_grad_clusters(uint32_t ranks, uint32_t threads) {
+bool norm_grad_clusters(uint32_t ranks, uint32_t threads, int* n) {
     const auto kern = norm_grad_kernel<ROW_BF16, true, 8, 4, GRAD_CLUSTER, 256>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) != cudaSuccess) return false;
     GradShape shape{GRAD_CLUSTER, threads, 1, 1, ranks};
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
@@ -73,8 +73,7 @@ int norm_grad_clusters(uint32_t ranks, uint32_t threads) {
     cfg.dynamicSmemBytes = grad_smem_bytes<ROW_BF16, true, 8, 4>(shape, 0);
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    int n = 0;
-    return cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess ? n : 0;
+    return cudaOccupancyMaxActiveClusters(n, kern, &cfg) == cudaSuccess;
 }
 #endif
 

@@ -28,8 +28,7 @@ inline cudaError_t launch_rows(const RowLaunch& env, void (*kern)(P), const P& p
         attrs[cfg.numAttrs].val.clusterDim.y = attrs[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    return cudaLaunchKernelEx(&cfg, kern, p);   // (not the thread's last error, which may be an older one of the caller's)
 }
 
 // The gradient's form and shape: a function of the columns, so that its workspace can be asked for. A thread takes at most 32
@@ -50,7 +49,7 @@ template <int XT, int RT, int VEC>
 cudaError_t norm_of(const RowLaunch& env, const NormParams& p);
 template <int XT, bool DSUM, int VEC>
 cudaError_t norm_grad_of(const RowLaunch& env, const NormGradParams& p, uint32_t blocks);
-int norm_grad_clusters(uint32_t ranks, uint32_t threads);   // of so many blocks of so many threads that the current device holds at once
+bool norm_grad_clusters(uint32_t ranks, uint32_t threads, int* n);   // of so many blocks of so many threads that the current device holds at once
 template <int XT, int VEC>
 cudaError_t quant_trans_of(const RowLaunch& env, const QuantTransParams& p, int* launches);
 

@@ -1,0 +1,19 @@
+// TEST INFRASTRUCTURE: the layer operators' host-side bookkeeping (csrc/layer_host.h) with fakes of the CUDA calls behind it.
+// Nothing in the product links or calls this file.
+#include "layer_host.h"
+
+using namespace mmeb200;
+
+extern "C" {
+// Asks `times` times; the first `failures` questions fail, the others answer `answer`. results[i]: what came back; returns the
+// number of questions put, and in *forgotten the number of errors cleared.
+int hc_device_holds(int times, int failures, int answer, int instead, int* results, int* forgotten)
+{
+    std::atomic<int> known{0};
+    int asked = 0;
+    *forgotten = 0;
+    for (int i = 0; i < times; i++)
+        results[i] = device_holds(known, [&](int* n) { *n = answer; return ++asked > failures; }, [&] { ++*forgotten; }, instead);
+    return asked;
+}
+}

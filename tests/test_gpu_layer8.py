@@ -850,6 +850,44 @@ def test_streams_graphs_and_two_contexts(port):
         st[0].close()
 
 
+def test_an_earlier_error_of_the_callers_is_not_the_call_s(calc, dev, port):
+    """The thread's last CUDA error, left by a call of the program's own, neither fails a call nor is taken away by it."""
+    runtime = C.CDLL("libcudart.so.12")
+    rng = np.random.default_rng(18)
+    m, k, n = 300, 1104, 264
+    v, g = rows_like(rng, m, k), dev.put(np.ones(k, np.float32), abi.FP32)
+    x, q, s = dev.put(v, abi.FP32), dev.put(np.zeros((m, k), np.int8), abi.INT8), dev.put(np.zeros(m, np.float32), abi.FP32)
+    qt, st = dev.put(np.zeros((k, m), np.int8), abi.INT8), dev.put(np.zeros(k, np.float32), abi.FP32)
+    w, one = dev.put(np.ones((n, k), np.int8), abi.INT8), dev.put(np.ones(1, np.float32), abi.FP32)
+    odd = dev.put(np.ones((n, k), np.int8), abi.INT8, offset=1)
+    y, dx, dg = dev.put(np.zeros((m, n), np.float32), abi.FP32), dev.put(np.zeros((m, k), np.float32), abi.FP32), dev.put(np.zeros(k, np.float32), abi.FP32)
+    few, none = dev.put(np.zeros((3, n), np.float32), abi.FP32), T(None, abi.INT8, [0, 3], mem_space=abi.MEM_DEVICE)
+    q3 = T(q.data, abi.INT8, [k, 3], mem_space=abi.MEM_DEVICE)
+    host_q, host_s = np.zeros((m, k), np.int8), np.zeros(m, np.float32)
+    calls = {
+        "norm": lambda: calc.rms_norm(q, x, g, EPS, scale=s),
+        "gradient": lambda: calc.rms_norm_grad(dx, dg, x, x, g, EPS),
+        "rows": lambda: calc.quantize(q, s, x),
+        "columns": lambda: calc.quantize(qt, st, x, abi.OP_TRANS),
+        "product": lambda: calc.scaled_gemm(y, q, s, w, one),
+        "product of few tokens": lambda: calc.scaled_gemm(few, q3, one, w, one),
+        "product of unaligned rows": lambda: calc.scaled_gemm(few, q3, one, odd, one),
+        "product of nothing": lambda: calc.scaled_gemm(few, none, one, T(None, abi.INT8, [0, n], mem_space=abi.MEM_DEVICE), one),
+        "host rows": lambda: calc.quantize(T(host_q, abi.INT8, [k, m]), T(host_s, abi.FP32, [m]), T(v, abi.FP32, [k, m])),
+    }
+    for name, call in calls.items():
+        error = runtime.cudaSetDevice(9999)
+        assert error != 0
+        try:
+            call()
+            assert runtime.cudaPeekAtLastError() == error, name
+        finally:
+            runtime.cudaGetLastError()
+    calc.sync()
+    codes, step = layer8.codes_of(v, abi.INT8, port)
+    assert (dev.get(q) == codes).all() and (dev.get(s)[0] == step).all() and (host_q == codes).all() and (dev.get(few) == 0).all()
+
+
 FIRST_CALLS_CAPTURED = """
 import sys, torch
 sys.path.insert(0, sys.argv[1])
