@@ -112,10 +112,15 @@ int layer_scratch(mmeb200_ctx* c, size_t bytes, const char* remedy, void** out) 
     *out = c->layer_ws;
     return 0;
 }
-int layer_scratch_used(mmeb200_ctx* c) {
-    CUDA_OK(c, cudaEventRecord(c->layer_ws_used, c->stream));
-    return 0;
-}
+// Records the event when the call that took scratch memory is through, or returns early.
+struct LayerScratchMark {
+    mmeb200_ctx* c;
+    int operator()() const {
+        CUDA_OK(c, cudaEventRecord(c->layer_ws_used, c->stream));
+        return 0;
+    }
+};
+using LayerScratchUse = UseMark<LayerScratchMark>;
 
 // Host tensors are staged as everywhere else in this library; device tensors are used where they lie.
 struct LayerStage {
@@ -383,11 +388,13 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
     for (int d = 0; d < 4; ++d) p.dims[d] = x->sizes[d + 1];
     layer_flatten(p.dims, &p.flat, {&p.x, &p.dy, &p.dsum, &p.dx});
     p.eps = eps; p.per_col = 1.0f / float(cols);
-    void* scratch = nullptr;
+    LayerScratchUse use(LayerScratchMark{c});
     if (dgamma) {
         if (workspace) p.partial = static_cast<float*>(workspace->data);
         else {
+            void* scratch = nullptr;
             TRY(layer_scratch(c, need * sizeof(float), "pass a workspace", &scratch));
+            use.begin();
             p.partial = static_cast<float*>(scratch);
         }
     }
@@ -400,7 +407,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         CUDA_OK(c, launch_column_sums(layer_launch(c), p.partial, static_cast<float*>(tdg->data), blocks, uint32_t(cols)));
         c->launches++;
     }
-    if (scratch) TRY(layer_scratch_used(c));
+    TRY(use.end());
     return st.finish();
 }
 
@@ -454,14 +461,27 @@ bool layer_operand(const mmeb200_tensor* t, TmaOperand* o) {
     // rows that share memory (a stride below their length) are read like any others
     return tma_compatible(*o) && (o->rows == 1 || o->row_stride != 0);
 }
-int layer_pad_operand(mmeb200_ctx* c, TmaOperand* o, uint8_t* dst) {
-    const uint64_t ld = (o->inner + 15) & ~uint64_t(15);
-    CUDA_OK(c, launch_pad_rows(layer_launch(c), o->ptr, dst, o->rows, o->inner, o->row_stride, ld));
-    c->launches++;
-    o->ptr = dst;
-    o->row_stride = ld;
-    return 0;
-}
+// Copies of a product's operands that have to be made before it. They are launched when nothing else of the call can fail but
+// the product's own launch.
+struct LayerPads {
+    TmaOperand from[2], to[2];
+    int n = 0;
+    static uint64_t bytes(const TmaOperand& o) { return o.rows * ((o.inner + 15) & ~uint64_t(15)); }
+    // *o lies at dst from now on
+    void add(TmaOperand* o, uint8_t* dst) {
+        from[n] = *o;
+        o->ptr = dst;
+        o->row_stride = (o->inner + 15) & ~uint64_t(15);
+        to[n++] = *o;
+    }
+    int launch(mmeb200_ctx* c) const {
+        for (int i = 0; i < n; ++i) {
+            CUDA_OK(c, launch_pad_rows(layer_launch(c), from[i].ptr, const_cast<void*>(to[i].ptr), from[i].rows, from[i].inner, from[i].row_stride, to[i].row_stride));
+            c->launches++;
+        }
+        return 0;
+    }
+};
 
 int layer_token_capacity(mmeb200_ctx* c, uint32_t kind, uint32_t tok, uint32_t splits, uint32_t ctas) {
     static std::atomic<int> known[64][2][4][9] = {};   // of the full ring, which all tiles nearly have
@@ -532,7 +552,7 @@ ProductPlan layer_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t N, ui
 }
 
 // Few tokens or few tiles: the cluster kernel (gemm_tokens.cuh).
-int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, const ProductPlan& plan, TokenGemmParams& p) {
+int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, const LayerPads& pads, const ProductPlan& plan, TokenGemmParams& p) {
     p.num_k_blocks = uint32_t((ox.inner + kRowBytes - 1) / kRowBytes);
     p.tok = plan.tok;
     p.splits = plan.splits;
@@ -541,6 +561,7 @@ int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, con
     p.status = c->d_status;
     TRY(encode_tiled(c, &p.tm_w, ow, kRowBytes, kBlockM));
     TRY(encode_tiled(c, &p.tm_x, ox, kRowBytes, p.tok));
+    TRY(pads.launch(c));
     return launch_status(c, launch_gemm_tokens(launch_env(c), kind, p));
 }
 
@@ -553,7 +574,7 @@ bool layer_tma_output(const TokenGemmParams& t, const mmeb200_ctx* c, TmaOperand
 }
 
 // Many tiles: the CTA-pair kernel of the other GEMMs, with the scaling epilogue.
-int layer_pair_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, const TokenGemmParams& t, const mmeb200_tensor* out) {
+int layer_pair_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, const TmaOperand& ow, const LayerPads& pads, const TokenGemmParams& t) {
     GemmParams p;
     memset(&p, 0, sizeof p);
     p.M = t.M; p.N = t.N; p.K = uint32_t(ox.inner);
@@ -573,6 +594,7 @@ int layer_pair_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, cons
     if (layer_tma_output(t, c, &od) && encode_tiled(c, &p.tm_out, od, kRowBytes / od.elem, 32, od.elem == 2 ? 2 : 0) == 0) p.tma_store = 1;
     bool two_groups = p.num_k_blocks <= 12;
     if (c->tune.epi_groups > 0) two_groups = c->tune.epi_groups == 2;
+    TRY(pads.launch(c));
     return launch_status(c, launch_gemm_pair_scaled(launch_env(c), kind, two_groups ? 2 : 1, p, uint64_t(p.m_tiles) * p.n_tiles));
 }
 
@@ -636,18 +658,20 @@ int run_scaled_gemm(mmeb200_ctx* c, mmeb200_tensor* out, const mmeb200_tensor* x
     const uint32_t kind = i8 ? KIND_I8 : KIND_F8;
     TmaOperand ox, ow;
     const bool x_fits = layer_operand(tx, &ox), w_fits = layer_operand(tw, &ow);
-    void* scratch = nullptr;
-    if (!x_fits || !w_fits) {
-        const size_t xb = x_fits ? 0 : M * ((K + 15) & ~uint64_t(15)), wb = w_fits ? 0 : N * ((K + 15) & ~uint64_t(15));
-        TRY(layer_scratch(c, xb + wb, "operands need 16-byte aligned rows", &scratch));
-        if (!x_fits) TRY(layer_pad_operand(c, &ox, static_cast<uint8_t*>(scratch)));
-        if (!w_fits) TRY(layer_pad_operand(c, &ow, static_cast<uint8_t*>(scratch) + xb));
-    }
     const ProductPlan plan = layer_plan(c, kind, p.M, p.N, uint32_t((K + kRowBytes - 1) / kRowBytes), p.out_bf16 ? 2 : 4, layer_tma_output(p, c));
-    if (plan.pair) TRY(layer_pair_product(c, kind, ox, ow, p, to));
-    else if (plan.tok) TRY(layer_token_product(c, kind, ox, ow, plan, p));
-    else return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");
-    if (scratch) TRY(layer_scratch_used(c));
+    if (!plan.pair && !plan.tok) return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");
+    LayerScratchUse use(LayerScratchMark{c});
+    LayerPads pads;
+    if (!x_fits || !w_fits) {
+        const size_t xb = x_fits ? 0 : LayerPads::bytes(ox), wb = w_fits ? 0 : LayerPads::bytes(ow);
+        void* scratch = nullptr;
+        TRY(layer_scratch(c, xb + wb, "operands need 16-byte aligned rows", &scratch));
+        use.begin();
+        if (!x_fits) pads.add(&ox, static_cast<uint8_t*>(scratch));
+        if (!w_fits) pads.add(&ow, static_cast<uint8_t*>(scratch) + xb);
+    }
+    TRY(plan.pair ? layer_pair_product(c, kind, ox, ow, pads, p) : layer_token_product(c, kind, ox, ow, pads, plan, p));
+    TRY(use.end());
     return st.finish();
 }
 

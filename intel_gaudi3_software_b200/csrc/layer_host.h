@@ -22,4 +22,24 @@ int device_holds(std::atomic<int>& known, Ask&& ask, Forget&& forget, int instea
     return n;
 }
 
+// Marks the end of a call's use of shared memory on every way out of the call, errors in its middle included: work that was
+// launched before them is still in flight. `mark()` returns a status.
+template <typename Mark>
+class UseMark {
+    Mark mark;
+    bool open = false;
+
+public:
+    explicit UseMark(Mark m) : mark(m) {}
+    UseMark(const UseMark&) = delete;
+    UseMark& operator=(const UseMark&) = delete;
+    void begin() { open = true; }
+    int end() {
+        if (!open) return 0;
+        open = false;
+        return mark();
+    }
+    ~UseMark() { end(); }
+};
+
 }  // namespace mmeb200

@@ -16,4 +16,21 @@ int hc_device_holds(int times, int failures, int answer, int instead, int* resul
         results[i] = device_holds(known, [&](int* n) { *n = answer; return ++asked > failures; }, [&] { ++*forgotten; }, instead);
     return asked;
 }
+
+// A call that takes shared memory (or not), fails after its first launch (or not) and ends its use itself otherwise: how often
+// the use was marked, and in *status what the call returned.
+int hc_use_mark(int takes, int fails, int mark_status, int* status)
+{
+    int marks = 0;
+    const auto mark = [&] { ++marks; return mark_status; };
+    const auto call = [&]() -> int {
+        UseMark<decltype(mark)> use(mark);
+        if (takes) use.begin();
+        if (fails) return -3;
+        if (const int rc = use.end()) return rc;
+        return 0;
+    };
+    *status = call();
+    return marks;
+}
 }

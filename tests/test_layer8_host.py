@@ -36,3 +36,9 @@ def test_a_failed_question_is_asked_again_and_its_error_cleared(host):
 def test_a_number_instead_of_a_failed_answer_stays(host):
     """The gradient's workspace is asked for and used by two calls: both have to see the same number."""
     assert holds(host, 3, 1, 74, 18) == ([18, 18, 18], 1, 1)
+
+
+@pytest.mark.parametrize("takes,fails,mark_status,marks,status", [(0, 0, 0, 0, 0), (0, 1, 0, 0, -3), (1, 0, 0, 1, 0), (1, 1, 0, 1, -3), (1, 0, -7, 1, -7)])
+def test_the_use_of_scratch_memory_is_marked_once_on_every_way_out(host, takes, fails, mark_status, marks, status):
+    got = C.c_int()
+    assert host.hc_use_mark(takes, fails, mark_status, C.byref(got)) == marks and got.value == status
