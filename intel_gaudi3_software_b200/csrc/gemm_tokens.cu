@@ -44,7 +44,8 @@ static LaunchResult launch(const LaunchEnv& env, TokenGemmParams& p) {
     p.stages = gemm_tokens_stages(p.tok, p.ctas);
     p.tmem_cols = 32;
     while (p.tmem_cols < p.tok) p.tmem_cols *= 2;
-    cfg.gridDim = dim3(p.splits * ((p.N + kBlockM - 1) / kBlockM), (p.M + p.tok - 1) / p.tok);
+    const uint32_t m_tiles = (p.M + p.tok - 1) / p.tok - p.m_tile0;
+    cfg.gridDim = dim3(p.splits * ((p.N + kBlockM - 1) / kBlockM), m_tiles < kTokenTilesY ? m_tiles : kTokenTilesY);
     e = cudaLaunchKernelEx(&cfg, gemm_tokens_kernel<KIND>, p);
     return {e, LAUNCH_OK, "few-token kernel launch"};   // (not the thread's last error, which may be an older one of the caller's)
 }

@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kTokenThreads, 2) gemm_tokens_kernel(const __g
     uint64_t* done_bar = empty_bar + kTokenMaxStages;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(done_bar + 1);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = blockIdx.x % p.splits, n0 = (blockIdx.x / p.splits) * kBlockM, m0 = blockIdx.y * p.tok;
+    const uint32_t rank = blockIdx.x % p.splits, n0 = (blockIdx.x / p.splits) * kBlockM, m0 = (p.m_tile0 + blockIdx.y) * p.tok;
     const uint32_t per = (p.num_k_blocks + p.splits - 1) / p.splits;
     const uint32_t kb0 = rank * per, kb1 = min(p.num_k_blocks, kb0 + per);   // the planner leaves no share empty
 

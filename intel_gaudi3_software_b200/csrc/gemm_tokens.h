@@ -16,6 +16,7 @@ struct TokenGemmParams {
     uint32_t tok;               // tokens of a tile (a multiple of 16, at most 256)
     uint32_t splits;            // CTAs of a cluster, each with its share of the k blocks
     uint32_t ctas;              // CTAs that share an SM (1 or 2): sets how much shared memory each has for its ring
+    uint32_t m_tile0;           // first token tile of this launch: a grid has at most kTokenTilesY of them
     uint32_t stages, stage_bytes;
     uint32_t tmem_cols;
     uint32_t idesc;
@@ -27,7 +28,9 @@ struct TokenGemmParams {
     uint32_t* status;
 };
 
-// Fills stages, stage_bytes and tmem_cols for p.tok and launches on a grid of splits x channel tiles x token tiles.
+constexpr uint32_t kTokenTilesY = 65535;
+// Fills stages, stage_bytes and tmem_cols for p.tok and launches on a grid of splits x channel tiles x token tiles (from m_tile0 on,
+// kTokenTilesY at most).
 LaunchResult launch_gemm_tokens(const LaunchEnv& env, uint32_t kind, TokenGemmParams p);
 // out = bias (or zero) for operands without a common dimension.
 LaunchResult launch_gemm_empty_sum(const LaunchEnv& env, const TokenGemmParams& p);

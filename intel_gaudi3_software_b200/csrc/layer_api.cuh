@@ -512,7 +512,7 @@ ProductPlan layer_make_plan(mmeb200_ctx* c, uint32_t kind, uint32_t M, uint32_t 
         const uint32_t m_tiles = (M + want - 1) / want, tok = c->tune.token_tile > 0 ? want : ((M + m_tiles - 1) / m_tiles + 15) & ~15u;
         const double stage = kBlockM * kRowBytes + tok * kRowBytes, tiles = channels * m_tiles;
         const double memory = hbm + 0.25 * (m_tiles - 1) * 128.0 * kb * N / 6.05e6;   // a quarter of the weights' further reads misses L2
-        if (tok == before || m_tiles > 65535 || tiles * 8 >= 2147483648.0) continue;
+        if (tok == before) continue;
         before = tok;
         for (uint32_t s = 1; s <= 8 && s <= kb; ++s) {
             const uint32_t per = (kb + s - 1) / s;
@@ -562,7 +562,8 @@ int layer_token_product(mmeb200_ctx* c, uint32_t kind, const TmaOperand& ox, con
     TRY(encode_tiled(c, &p.tm_w, ow, kRowBytes, kBlockM));
     TRY(encode_tiled(c, &p.tm_x, ox, kRowBytes, p.tok));
     TRY(pads.launch(c));
-    return launch_status(c, launch_gemm_tokens(launch_env(c), kind, p));
+    for (; uint64_t(p.m_tile0) * p.tok < p.M; p.m_tile0 += kTokenTilesY) TRY(launch_status(c, launch_gemm_tokens(launch_env(c), kind, p)));
+    return 0;
 }
 
 // Whether a tensor map can describe the output.
@@ -659,7 +660,6 @@ int run_scaled_gemm(mmeb200_ctx* c, mmeb200_tensor* out, const mmeb200_tensor* x
     TmaOperand ox, ow;
     const bool x_fits = layer_operand(tx, &ox), w_fits = layer_operand(tw, &ow);
     const ProductPlan plan = layer_plan(c, kind, p.M, p.N, uint32_t((K + kRowBytes - 1) / kRowBytes), p.out_bf16 ? 2 : 4, layer_tma_output(p, c));
-    if (!plan.pair && !plan.tok) return c->fail(MMEB200_ERR_UNSUPPORTED, "the product has too many tiles");
     LayerScratchUse use(LayerScratchMark{c});
     LayerPads pads;
     if (!x_fits || !w_fits) {

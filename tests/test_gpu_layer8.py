@@ -557,6 +557,28 @@ def test_product_token_kernel_on_many_tiles(calc, dev, port):
         calc.set_option("pair", -1)
 
 
+@pytest.mark.parametrize("m,n,tile", [(65535 * 16 + 40, 5, 16), (65535 * 256 + 300, 1, -1)])
+def test_product_of_more_token_tiles_than_a_grid_has(calc, m, n, tile):
+    """More than 65535 tiles along the tokens take a second launch. Sums of 16 small integers: exact in fp32."""
+    rng = np.random.default_rng(19)
+    x, w = rng.integers(-128, 128, (m, 16)).astype(np.int8), rng.integers(-128, 128, (n, 16)).astype(np.int8)
+    bufs = [calc.to_device(a) for a in (x, w, np.float32([1]), np.full((m + 1) * n, -1.0, np.float32))]
+    tx, tw = T(bufs[0].ptr, abi.INT8, [16, m], mem_space=abi.MEM_DEVICE), T(bufs[1].ptr, abi.INT8, [16, n], mem_space=abi.MEM_DEVICE)
+    one, to = T(bufs[2].ptr, abi.FP32, [1], mem_space=abi.MEM_DEVICE), T(bufs[3].ptr, abi.FP32, [n, m], mem_space=abi.MEM_DEVICE)
+    calc.set_option("token_tile", tile)
+    launches = calc.launch_count()
+    try:
+        calc.scaled_gemm(to, tx, one, tw, one)
+    finally:
+        calc.set_option("token_tile", -1)
+    calc.sync()
+    assert calc.launch_count() >= launches + 2   # (the plan chooses the tile where no knob does: smaller ones, more launches)
+    got = bufs[3].download(np.float32).reshape(-1)[: (m + 1) * n].reshape(m + 1, n)
+    assert (got[:m] == x.astype(np.float32) @ w.astype(np.float32).T).all() and (got[m] == -1).all()
+    for b in bufs:
+        b.free()
+
+
 def test_product_int8_is_exact_at_the_range_s_ends(calc, dev, port):
     """Sums near +-2^31: the accumulator is a whole number up to the conversion."""
     check_product(calc, dev, port, 5, 140, 131071 // 16 * 16, extreme=True, ot=abi.FP32)
@@ -574,6 +596,25 @@ def test_product_int8_is_exact_at_the_range_s_ends(calc, dev, port):
 def test_product_operands_at_any_pitch_and_offset(calc, dev, port, xpitch, wpitch, xoff, woff):
     check_product(calc, dev, port, 33, 200, 1013, xpitch=xpitch, wpitch=wpitch, xoff=xoff, woff=woff)
     check_product(calc, dev, port, 300, 700, 85, xt=abi.FP8_143, xpitch=xpitch, wpitch=wpitch, xoff=xoff, woff=woff, ot=abi.FP32)
+
+
+@pytest.mark.parametrize("m", [5, 300])
+@pytest.mark.parametrize("step,k", [(16, 64), (16, 272), (3, 100), (0, 48)])
+def test_product_operands_whose_rows_share_memory(calc, dev, m, step, k):
+    """Rows `step` bytes apart and longer than that: windows over one sequence."""
+    rng = np.random.default_rng([20, m, step, k])
+    n = 270
+
+    def windows(rows):
+        flat = rng.integers(-128, 128, step * (rows - 1) + k).astype(np.int8)
+        t = dev.put(flat, abi.INT8)
+        return T(t.data, abi.INT8, [k, rows], [1, step], mem_space=abi.MEM_DEVICE), np.stack([flat[step * r:step * r + k] for r in range(rows)]).astype(np.float64)
+
+    (tx, x), (tw, w) = windows(m), windows(n)
+    to, one = dev.put(np.zeros((m, n), np.float32), abi.FP32), dev.put(np.float32([1]), abi.FP32)
+    calc.scaled_gemm(to, tx, one, tw, one)
+    calc.sync()
+    assert (dev.get(to) == x @ w.T).all()
 
 
 @pytest.mark.parametrize("m", [7, 600])
