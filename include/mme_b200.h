@@ -383,7 +383,8 @@ int mmeb200_conv_dedw_allreduce(mmeb200_ctx* ctx, mmeb200_tensor* out, const mme
  * Streams and memory: device-tensor calls are asynchronous on the context's stream and can be captured into a CUDA graph
  * once each entry point (with these types) has run before; calls that need scratch memory are refused while capturing, see
  * the entries. The caller's current device is left as it was. An output may be the same tensor as an input (same address,
- * type and strides) where the entry says so; any other overlap is refused. Host tensors are staged as everywhere else. */
+ * type and strides) where the entry says so; any other overlap is refused. Device tensors may lie between each other's rows
+ * (column ranges of one matrix); host tensors, which are staged whole as everywhere else, must not where one is an output. */
 enum { MMEB200_SCALE_ROW = 0, MMEB200_SCALE_GIVEN = 1 };
 
 /* RMS norm of every row, with the residual's addition: h = x + residual, rounded to the residual's type and written to

@@ -62,12 +62,21 @@ bool layer_same_place(const mmeb200_tensor* a, const mmeb200_tensor* b) {
         if (a->sizes[d] != b->sizes[d] || (a->sizes[d] > 1 && a->strides[d] != b->strides[d])) return false;
     return true;
 }
-// An output may share memory with an input only element by element (in_place), with another output never.
+// An output may share memory with an input only element by element (in_place), with another output never. Device tensors may lie
+// between each other's rows; a host output is copied back with what lies between its rows, so there ranges count.
 int layer_check_overlap(mmeb200_ctx* c, const mmeb200_tensor* out, const char* out_name, const mmeb200_tensor* other, const char* other_name, bool in_place) {
     if (!out || !other || out->mem_space != other->mem_space || num_elems(out) == 0 || num_elems(other) == 0) return 0;
     const uintptr_t a = reinterpret_cast<uintptr_t>(out->data), b = reinterpret_cast<uintptr_t>(other->data);
     if (a + span_elems(out) * layer_elem_size(out) <= b || b + span_elems(other) * layer_elem_size(other) <= a) return 0;
     if (in_place && layer_same_place(out, other)) return 0;
+    if (out->mem_space == MMEB200_MEM_DEVICE) {
+        uint64_t strides[8];
+        for (int d = 1; d < 5; ++d) {
+            strides[d - 1] = out->sizes[d] > 1 ? uint64_t(out->strides[d]) * layer_elem_size(out) : 0;
+            strides[d + 3] = other->sizes[d] > 1 ? uint64_t(other->strides[d]) * layer_elem_size(other) : 0;
+        }
+        if (rows_lie_apart(a, uint64_t(out->sizes[0]) * layer_elem_size(out), b, uint64_t(other->sizes[0]) * layer_elem_size(other), strides)) return 0;
+    }
     return c->fail(MMEB200_ERR_INVALID_ARG, "%s and %s overlap in memory", out_name, other_name);
 }
 int layer_same_sizes(mmeb200_ctx* c, const mmeb200_tensor* a, const mmeb200_tensor* b, const char* name) {

@@ -1,5 +1,7 @@
 // TEST INFRASTRUCTURE: the layer operators' host-side bookkeeping (csrc/layer_host.h) with fakes of the CUDA calls behind it.
 // Nothing in the product links or calls this file.
+#include <vector>
+
 #include "layer_host.h"
 
 using namespace mmeb200;
@@ -15,6 +17,11 @@ int hc_device_holds(int times, int failures, int answer, int instead, int* resul
     for (int i = 0; i < times; i++)
         results[i] = device_holds(known, [&](int* n) { *n = answer; return ++asked > failures; }, [&] { ++*forgotten; }, instead);
     return asked;
+}
+
+int hc_rows_lie_apart(uint64_t a, uint64_t a_bytes, uint64_t b, uint64_t b_bytes, const uint64_t* strides, int n)
+{
+    return rows_lie_apart(uintptr_t(a), a_bytes, uintptr_t(b), b_bytes, std::vector<uint64_t>(strides, strides + n));
 }
 
 // A call that takes shared memory (or not), fails after its first launch (or not) and ends its use itself otherwise: how often

@@ -254,6 +254,42 @@ def test_norm_in_place(calc, dev, cols):
         assert (dev.get(o) == out).all() and (dev.get(s) == total).all()
 
 
+@pytest.mark.parametrize("cols", [71, 72, 1504, 20001])
+def test_tensors_between_each_other_s_rows(calc, dev, cols):
+    """x, residual, sum and out (then x, dy, dsum and dx) as column ranges of one matrix, against 64 bits, and nothing else of the
+    matrix touched. Ranges that share a column are refused, host ranges that cross too."""
+    rng = np.random.default_rng([21, cols])
+    rows, pitch = 9, 4 * cols + 3
+    (ab, a), (bb, b), (cb, c) = (encode(rows_like(rng, rows, cols), abi.BF16) for _ in range(3))
+    gb, g = encode(1 + 0.1 * rng.standard_normal(cols), abi.FP32)
+    tg, z, rest = dev.put(gb, abi.FP32), np.zeros_like(ab), np.full((rows, 3), 7, np.uint16)
+
+    def ranges(parts):
+        whole = dev.put(np.hstack(parts + [rest]), abi.BF16)
+        return whole, [T(whole.data + 2 * i * cols, abi.BF16, [cols, rows], [1, pitch], mem_space=abi.MEM_DEVICE) for i in range(4)]
+
+    whole, (x, res, s, o) = ranges([ab, bb, z, z])
+    calc.rms_norm(o, x, tg, EPS, residual=res, sum=s)
+    calc.sync()
+    got, (sb, h) = dev.get(whole), encode((a + b).astype(np.float32), abi.BF16)
+    assert (np.delete(got, np.s_[3 * cols:4 * cols], axis=1) == np.hstack([ab, bb, sb, rest])).all()
+    ref, _ = layer8.norm(h, g, EPS)
+    bound = np.abs(ref) * (layer8.inverse_bound(cols) + 2 * layer8.U)
+    assert (np.abs(decode(got[:, 3 * cols:4 * cols], abi.BF16) - ref) <= bound + layer8.HALF[abi.BF16] * (np.abs(ref) + bound) + 1e-38).all()
+    whole, (x, dy, ds, d) = ranges([ab, bb, cb, z])
+    calc.rms_norm_grad(d, None, dy, x, tg, EPS, dsum=ds)
+    calc.sync()
+    got = dev.get(whole)
+    assert (np.delete(got, np.s_[3 * cols:4 * cols], axis=1) == np.hstack([ab, bb, cb, rest])).all()
+    dx, _ = layer8.norm_grad(a, g, b, c, EPS)
+    assert (np.abs(decode(got[:, 3 * cols:4 * cols], abi.BF16) - dx) <= layer8.norm_grad_bounds(a, g, b, c, EPS, abi.BF16)[0]).all()
+    with pytest.raises(MmeError, match="overlap"):
+        calc.rms_norm(T(d.data - 2, abi.BF16, [cols, rows], [1, pitch], mem_space=abi.MEM_DEVICE), x, tg, EPS, residual=dy, sum=ds)
+    h = np.zeros((rows, 2 * cols), np.uint16)
+    with pytest.raises(MmeError, match="overlap"):
+        calc.rms_norm(T(h[:, cols:], abi.BF16, [cols, rows], [1, 2 * cols]), T(h, abi.BF16, [cols, rows], [1, 2 * cols]), None, EPS)
+
+
 def test_norm_in_five_dimensions(calc, dev, port):
     """Rows spread over four outer dimensions whose strides do not merge, in another order than the sizes."""
     rng = np.random.default_rng(7)
