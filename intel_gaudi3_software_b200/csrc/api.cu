@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cstdarg>
 #include <cstdio>
@@ -252,8 +253,8 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 typedef CUresult (*EncodeIm2colFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                    const int*, const int*, cuuint32_t, cuuint32_t, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn g_encode_tiled = nullptr;
-static EncodeIm2colFn g_encode_im2col = nullptr;
+static std::atomic<EncodeTiledFn> g_encode_tiled{nullptr};   // (two contexts may meet here on two threads)
+static std::atomic<EncodeIm2colFn> g_encode_im2col{nullptr};
 static int load_driver_entry_points(mmeb200_ctx* c) {
     if (g_encode_tiled && g_encode_im2col) return 0;
     cudaDriverEntryPointQueryResult q;
@@ -307,7 +308,7 @@ static int encode_tiled(mmeb200_ctx* c, CUtensorMap* tm, const TmaOperand& o, ui
     cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     // 16-bit outputs are raw bit patterns: describe them as integers so the copy engine cannot touch them
     const CUtensorMapDataType dt = (u16_type == 2) ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : tma_dtype(o.elem);
-    CUresult r = g_encode_tiled(tm, dt, 5, const_cast<void*>(o.ptr), dims, strides, box, estr,
+    CUresult r = g_encode_tiled.load()(tm, dt, 5, const_cast<void*>(o.ptr), dims, strides, box, estr,
                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
@@ -1532,7 +1533,7 @@ static int conv_fast_path(mmeb200_ctx* c, const mmeb200_tensor* x, const mmeb200
     cuuint64_t strides[3] = {uint64_t(act->strides[1]) * elem, uint64_t(act->strides[2]) * elem, uint64_t(act->strides[3]) * elem};
     for (int i = 0; i < 3; ++i)
         if (strides[i] % 16) return 0;
-    CUresult r = g_encode_im2col(&job->a_map, tma_dtype(elem), 4, act->data, dims, strides, lower, upper, chan_box, pix_box, trav,
+    CUresult r = g_encode_im2col.load()(&job->a_map, tma_dtype(elem), 4, act->data, dims, strides, lower, upper, chan_box, pix_box, trav,
                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return 0;  // geometry outside what the copy engine takes: general path

@@ -1,6 +1,7 @@
 // One instantiation of a tcgen05 GEMM kernel and its host launcher. The Makefile compiles this file once per
 // variant with  -DINST_NAME=<launcher name> -DINST_KIND=<KIND_*> and either -DINST_PAIR_EPI=<1|2> -DINST_PAIR_CUT=<0|1>
 // [-DINST_PAIR_SCALED=1] (CTA-pair kernel) or -DINST_BLOCK_N=<128|256> -DINST_STAGES=<n> (single-CTA kernel).
+#include <atomic>
 #include <cstring>
 
 #include "gemm_launch.h"
@@ -16,13 +17,13 @@ namespace mmeb200 {
 #ifndef INST_PAIR_SCALED
 #define INST_PAIR_SCALED 0
 #endif
-static int g_max_pairs[64] = {};
+static std::atomic<int> g_max_pairs[64] = {};
 
 static LaunchResult configure(const LaunchEnv& env, int* pairs) {
     auto kern = gemm_tcgen05_pair_kernel<INST_KIND, INST_PAIR_EPI, INST_PAIR_CUT != 0, INST_PAIR_SCALED != 0>;
     constexpr int smem = PairSmem<INST_PAIR_EPI>::kTotal + (INST_PAIR_SCALED ? int(kScaledSmemBytes) : 0);
     constexpr int threads = PairSmem<INST_PAIR_EPI>::kThreads;
-    int& cached = g_max_pairs[env.device & 63];
+    std::atomic<int>& cached = g_max_pairs[env.device & 63];
     if (cached == 0) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return {e, LAUNCH_OK, "cudaFuncSetAttribute(pair kernel)"};
@@ -77,7 +78,7 @@ LaunchResult INST_NAME(const LaunchEnv& env, const GemmParams& p, uint64_t tiles
 
 #else
 
-static bool g_configured[64] = {};
+static std::atomic<bool> g_configured[64] = {};
 
 LaunchResult INST_NAME(const LaunchEnv& env, const GemmParams& p, unsigned grid) {
     auto kern = gemm_tcgen05_kernel<INST_KIND, INST_BLOCK_N, INST_STAGES>;

@@ -1,6 +1,7 @@
 // Launcher of the few-token product kernel; see gemm_tokens.h.
 #include "gemm_tokens.cuh"
 
+#include <atomic>
 #include <cstring>
 
 namespace mmeb200 {
@@ -15,7 +16,7 @@ uint32_t gemm_tokens_stages(uint32_t tok, uint32_t ctas) {
 
 template <int KIND>
 static cudaError_t configure(const LaunchEnv& env, uint32_t tok, uint32_t splits, uint32_t ctas, cudaLaunchConfig_t* cfg, cudaLaunchAttribute* attrs) {
-    static bool done[64] = {};
+    static std::atomic<bool> done[64] = {};   // (two contexts may meet here on two threads)
     if (!done[env.device & 63]) {
         const cudaError_t e = cudaFuncSetAttribute(gemm_tokens_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTokenSmem);
         if (e != cudaSuccess) return e;

@@ -2,6 +2,7 @@
 // -DINST_VEC=<8|0|1> (element type of x, how rows lie: 0 is kPhased) and one of -DINST_NORM=<0|1|2> (element type of the residual),
 // -DINST_GRAD=<0|1> (with a gradient of the sum) and -DINST_TRANS.
 #include <algorithm>
+#include <atomic>
 
 #include "norm_quant.cuh"
 #include "norm_quant_launch.h"
@@ -35,7 +36,7 @@ template <int XT, bool DSUM, int VEC, int NV, int FORM, int THREADS>
 cudaError_t launch_grad(const RowLaunch& env, const NormGradParams& p, uint32_t blocks, const GradShape& shape) {
     const auto kern = norm_grad_kernel<XT, DSUM, VEC, NV, FORM, THREADS>;
     const size_t smem = grad_smem_bytes<XT, DSUM, VEC, NV>(shape, p.cols);
-    static bool done[64] = {};
+    static std::atomic<bool> done[64] = {};   // (two contexts may meet here on two threads)
     if (smem > 40 * 1024 && !done[env.device & 63]) {   // (48 KB with the static shared memory need no leave)
         const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
         if (e != cudaSuccess) return e;

@@ -1011,6 +1011,50 @@ def test_first_calls_of_a_process_inside_a_capture():
     assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
 
 
+FIRST_CALLS_ON_TWO_THREADS = """
+import sys, threading, torch
+sys.path.insert(0, sys.argv[1])
+from intel_gaudi3_software_b200 import Calculator, abi
+kinds = {torch.bfloat16: abi.BF16, torch.float32: abi.FP32, torch.int8: abi.INT8}
+def t(a):
+    return abi.make_tensor(a.data_ptr(), kinds[a.dtype], list(reversed(a.shape)), list(reversed(a.stride())), mem_space=abi.MEM_DEVICE)
+rows, cols, n = 520, 9104, 264
+gen = torch.Generator(device="cuda").manual_seed(1)
+x, dy = (torch.randn(rows, cols, device="cuda", generator=gen).bfloat16() for _ in range(2))
+w, gamma = torch.randn(cols, n, device="cuda", generator=gen).bfloat16(), torch.rand(cols, device="cuda", generator=gen)
+torch.cuda.synchronize()
+start, results = threading.Barrier(2), [None, None]
+def work(i):
+    calc = Calculator(device=0)
+    outs = [torch.zeros(rows, cols, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda"), torch.zeros(n, cols, dtype=torch.int8, device="cuda"),
+            torch.zeros(n, device="cuda"), torch.zeros(rows, n, device="cuda"), torch.zeros(9, n, device="cuda"), torch.zeros_like(x), torch.zeros(cols, device="cuda")]
+    torch.cuda.synchronize()
+    q, s, wq, ws, y, few, dx, dg = (t(o) for o in outs)
+    start.wait()
+    for _ in range(20):
+        calc.rms_norm(q, t(x), t(gamma), 1e-5, scale=s)
+        calc.quantize(wq, ws, t(w), abi.OP_TRANS)
+        calc.scaled_gemm(y, q, s, wq, ws)
+        calc.scaled_gemm(few, t(outs[0][:9]), t(outs[1][:9]), wq, ws)
+        calc.rms_norm_grad(dx, dg, t(dy), t(x), t(gamma), 1e-5)
+    calc.sync()
+    results[i] = outs
+    calc.close()
+threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+for th in threads: th.start()
+for th in threads: th.join()
+assert all(torch.equal(a, b) and a.any() for a, b in zip(*results))
+print("same")
+"""
+
+
+def test_first_calls_of_two_threads_at_once():
+    """Two contexts, each on a thread of its own, whose first calls of every kind meet."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS_ON_TWO_THREADS, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
 # ------------------------------------------------------------------------------------------ refusals
 def test_refusals(calc, dev):
     rng = np.random.default_rng(16)
