@@ -381,6 +381,28 @@ def test_quantize_transposed(calc, dev, port, rows, cols, xt):
         assert (dev.get(to) == layer8.codes_of(x.T, ot, port, given=[0.03])[0]).all()
 
 
+@pytest.mark.parametrize("pitch", [0, 3])
+def test_quantize_transposed_in_several_launches(calc, pitch):
+    """More rows than 65535 tiles of 128: the codes come from a second launch, the steps are of all rows. Columns whose largest
+    element lies in the first launch's rows, in the second's, and in the last row."""
+    rows, cols = 65535 * 128 + 131, 4
+    rng = np.random.default_rng(22)
+    v = rng.standard_normal((rows, cols), np.float32)
+    v[5, 0], v[65535 * 128 + 3, 1], v[rows - 1, 2] = 40, -50, 60
+    store = np.zeros((rows, cols + pitch), np.float32)
+    store[:, :cols] = v
+    bx, bo, bs = calc.to_device(store), calc.to_device(np.full((cols, rows + 5), 0x33, np.int8)), calc.to_device(np.zeros(cols, np.float32))
+    calc.quantize(T(bo.ptr, abi.INT8, [rows, cols], [1, rows + 5], mem_space=abi.MEM_DEVICE), T(bs.ptr, abi.FP32, [cols], mem_space=abi.MEM_DEVICE),
+                  T(bx.ptr, abi.FP32, [cols, rows], [1, cols + pitch], mem_space=abi.MEM_DEVICE), abi.OP_TRANS)
+    calc.sync()
+    step = (np.abs(v).max(axis=0) / np.float32(127)).astype(np.float32)
+    got = bo.download(np.int8)[: cols * (rows + 5)].reshape(cols, rows + 5)
+    assert (bs.download(np.float32)[:cols] == step).all()
+    assert (got[:, :rows] == np.rint(v.T / step[:, None])).all() and (got[:, rows:] == 0x33).all()
+    for b in (bx, bo, bs):
+        b.free()
+
+
 # ------------------------------------------------------------------------------------------ gradient
 def grad_case(calc, dev, rows, cols, xt, gt, with_dsum, seed=0, pitch=0, offset=0, dgamma=True, workspace=False):
     rng = np.random.default_rng([seed, rows, cols])
@@ -665,6 +687,13 @@ def test_product_fp8_types_and_biases(calc, dev, port, m):
     check_product(calc, dev, port, m, 520, 400, xt=abi.FP8_152, wt=abi.FP8_143, xbias=15, wbias=7)
     check_product(calc, dev, port, m, 520, 400, xt=abi.FP8_143, wt=abi.FP8_143, xbias=11, wbias=3, ot=abi.FP32)
     check_product(calc, dev, port, m, 520, 400, xt=abi.FP8_152, wt=abi.FP8_152, xbias=20, wbias=15)
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 4096, 2048), (4097, 2048, 1024)])
+def test_product_fp8_of_a_prompt(calc, dev, port, m, n, k):
+    """Many tiles and several waves of them. Sums are within the library's fp8 tolerance."""
+    check_product(calc, dev, port, m, n, k, xt=abi.FP8_143, bias_t=abi.BF16)
+    check_product(calc, dev, port, m, n, k, xt=abi.FP8_152, wt=abi.FP8_143, xbias=15, wbias=11, ot=abi.FP32)
 
 
 @pytest.mark.parametrize("xt", [abi.INT8, abi.FP8_143])
