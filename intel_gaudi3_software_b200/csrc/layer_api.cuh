@@ -278,7 +278,7 @@ int run_rms_norm(mmeb200_ctx* c, mmeb200_tensor* out, mmeb200_tensor* scale, mme
         TRY(layer_check(c, gamma, "gamma", true, false));
         TRY(layer_check_vector(c, gamma, "gamma", cols));
     }
-    if (!(eps >= 0.0f) || eps > 3.4e38f) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
+    if (!(eps >= 0.0f) || std::isinf(eps)) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
     TRY(layer_check_out_scale(c, out, scale, scale_mode, rows));
     const bool eight = layer_is_eight(out->dtype), given = eight && scale_mode == MMEB200_SCALE_GIVEN;
     float top = 0.0f;
@@ -355,7 +355,7 @@ int run_rms_norm_grad(mmeb200_ctx* c, mmeb200_tensor* dx, mmeb200_tensor* dgamma
         if (dgamma->dtype != DT_FP32) return c->fail(MMEB200_ERR_UNSUPPORTED, "dgamma: the sum over rows is fp32");
         TRY(layer_check_vector(c, dgamma, "dgamma", cols));
     }
-    if (!(eps >= 0.0f) || eps > 3.4e38f) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
+    if (!(eps >= 0.0f) || std::isinf(eps)) return c->fail(MMEB200_ERR_INVALID_ARG, "eps must be finite and not negative");
     uint32_t blocks = norm_grad_blocks(c->device, c->sm_count, uint32_t(rows), uint32_t(cols));
     const uint64_t need = uint64_t(blocks) * cols;
     if (workspace) {

@@ -234,6 +234,22 @@ def test_norm_float_rows_that_hold_no_number(calc, dev):
     assert np.abs(out[2] - 1).max() < 1e-5
 
 
+def test_eps_of_every_finite_size(calc, dev):
+    """eps = 0 and the largest float are finite and not negative. With the largest, mean(h^2) is below its last place: the root is
+    eps's own, up to its rounding, the reciprocal's and the product's."""
+    most = np.finfo(np.float32).max
+    v = np.float32([[3, -4, 0, 5], [1, 1, -1, 1]])
+    tx, to, td = dev.put(v, abi.FP32), dev.put(np.zeros_like(v), abi.FP32), dev.put(np.zeros_like(v), abi.FP32)
+    for eps in (0.0, float(most)):
+        calc.rms_norm(to, tx, None, eps)
+        calc.rms_norm_grad(td, None, tx, tx, None, eps)
+        calc.sync()
+        ref, _ = layer8.norm(v, np.ones(4), eps)
+        assert (np.abs(dev.get(to) - ref) <= np.abs(ref) * (layer8.inverse_bound(4) + 2 * layer8.U)).all()
+        dx, _ = layer8.norm_grad(v, np.ones(4), v, None, eps)
+        assert (np.abs(dev.get(td) - dx) <= layer8.norm_grad_bounds(v, np.ones(4), v, None, eps, abi.FP32)[0]).all()
+
+
 @pytest.mark.parametrize("cols", [64, 2056, 9001, 40000])
 def test_norm_in_place(calc, dev, cols):
     """sum over residual, out over x: the same values as with tensors of their own."""
