@@ -186,7 +186,8 @@ int mmeb200_set_accumulation(mmeb200_ctx* ctx, int mode);
  * stream serialisation; with it, the kernel's set-up overlaps the tail of the kernel before it in the stream and it touches
  * memory only after that kernel has completed), and for the scaled products of few tokens "token_tile" (tokens per tile, rounded up
  * to a multiple of 16), "token_split" (1..8 CTAs that share a tile's common dimension) and "token_ctas" (1 or 2 CTAs per SM), each
- * followed where the sizes have that form; "pair" chooses between the two kernels of scaled products as well. The older knobs take their defaults from environment variables read once in
+ * followed where the sizes have that form; "pair" chooses between the two kernels of scaled products as well, which follow
+ * "epi_groups", "raster_gm", "tma_store" and "dependent_launch" too and none of the others ("tile_n", "stream_k", ...). The older knobs take their defaults from environment variables read once in
  * mmeb200_create (MME_B200_PAIR, MME_B200_BLOCK_N, MME_B200_SPLIT_K, MME_B200_EPI_GROUPS, MME_B200_GM,
  * MME_B200_NO_TMA_STORE, MME_B200_NO_HOST_PIPELINE, MME_B200_TILE_N, MME_B200_STREAM_K, MME_B200_DEPENDENT_LAUNCH); no launch
  * reads the environment. Results do not depend on the knobs beyond the accumulation tolerance (summation order). */
@@ -380,9 +381,9 @@ int mmeb200_conv_dedw_allreduce(mmeb200_ctx* ctx, mmeb200_tensor* out, const mme
  * or one for all): code = nearest to v / scale, limited; a NaN becomes int8 0 or the fp8 type's NaN, and a scale that is
  * zero, negative or no finite number gives codes 0.
  *
- * Streams and memory: device-tensor calls are asynchronous on the context's stream and can be captured into a CUDA graph
- * once each entry point (with these types) has run before; calls that need scratch memory are refused while capturing, see
- * the entries. The caller's current device is left as it was. An output may be the same tensor as an input (same address,
+ * Streams and memory: device-tensor calls are asynchronous on the context's stream and can be captured into a CUDA graph, a
+ * process's first calls too. Calls that need the context's scratch memory (see the entries) are refused while capturing, and wait on
+ * the host when they have to enlarge it. The caller's current device is left as it was. An output may be the same tensor as an input (same address,
  * type and strides) where the entry says so; any other overlap is refused. Device tensors may lie between each other's rows
  * (column ranges of one matrix); host tensors, which are staged whole as everywhere else, must not where one is an output. */
 enum { MMEB200_SCALE_ROW = 0, MMEB200_SCALE_GIVEN = 1 };
@@ -393,7 +394,9 @@ enum { MMEB200_SCALE_ROW = 0, MMEB200_SCALE_GIVEN = 1 };
  *   residual's type, and may be the same tensor as x or residual; out may be the same tensor as x or residual.
  *   out: bf16, fp32 (scale must be NULL), or 8-bit codes with `scale` (see above; the codes of h * gamma, whose scale then
  *   carries the factor 1 / sqrt(...); with MMEB200_SCALE_GIVEN the codes of the finished rows).
- *   gamma: dense, one element per column. eps: finite, >= 0. */
+ *   gamma: dense, one element per column. eps: finite, >= 0.
+ * mean(h^2) is a 32-bit number like the rest: elements beyond about 1e19 make it infinite (the row comes out as zeros, with scale 0),
+ * and with eps = 0 rows whose elements all lie below about 1e-23 make it zero (infinities or NaN, and scale infinite). */
 int mmeb200_rms_norm(mmeb200_ctx* ctx, mmeb200_tensor* out, mmeb200_tensor* scale, mmeb200_tensor* sum, const mmeb200_tensor* x,
                      const mmeb200_tensor* residual, const mmeb200_tensor* gamma, float eps, int scale_mode);
 
@@ -420,9 +423,10 @@ int mmeb200_quantize(mmeb200_ctx* ctx, mmeb200_tensor* out, mmeb200_tensor* scal
  * operation), the result to out's type. int8 sums are exact before their rounding, so an int8 product's row has the same bits
  * whatever the other rows, the kernel and the knobs; fp8 sums may differ in their order.
  *   x, w: both int8 (any code, -128 included; the sum is exact, K <= 131071), or both fp8 (1-4-3 'minimal' or 1-5-2 'full', any
- *   exponent bias; fp32 sum on the tensor cores). x_scale, w_scale: dense fp32, one element per row or one for all.
+ *   exponent bias; fp32 sum on the tensor cores, so refused in MMEB200_ACC_CHIP_EXACT mode). x_scale, w_scale: dense fp32, one element per row or one for all.
  *   bias: bf16 or fp32, dense, may be NULL. out: bf16 or fp32, any row pitch. K = 0 gives the bias, or zeros.
- * Operands whose rows do not start on 16-byte boundaries are copied to scratch memory first (refused while capturing). */
+ * Operands whose rows do not start on 16-byte boundaries are copied to scratch memory first, on every call (refused while
+ * capturing). */
 int mmeb200_scaled_gemm(mmeb200_ctx* ctx, mmeb200_tensor* out, const mmeb200_tensor* x, const mmeb200_tensor* x_scale, const mmeb200_tensor* w,
                         const mmeb200_tensor* w_scale, const mmeb200_tensor* bias, int op);
 

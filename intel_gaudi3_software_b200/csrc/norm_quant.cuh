@@ -10,10 +10,15 @@
 //
 // A row takes a warp (up to 1024 columns), a block (32 columns a thread, 64 past 16384), or a loop that reads it twice. Blocks are
 // not kept over rows: the next row's loads come from the block beside it, two of 512 threads per SM. Measured against what has to
-// be read and written at 6549 GB/s: 8192 x 8192 bf16 with residual to int8 70.9 us (101 %), 16384 x 4096 with an fp32 residual to
-// bf16 119 us (103 %), quantisation of 2048 x 28672 bf16 33.4 us (81 %) and 8192 x 8192 fp32 54.8 us (94 %), 8192 x 4999 (odd
-// rows) 61 us (72 %: gamma's words are shifted for every row). 200000 rows of 128 columns take 54 us (22 %): a block lives for
-// four short rows and what bounds it is the rate at which blocks start.
+// be read and written at 6549 GB/s: 8192 x 8192 bf16 with residual to int8 71.8 us (100 %), 16384 x 4096 with an fp32 residual to
+// bf16 121 us (102 %), quantisation of 2048 x 28672 bf16 33.5 us (80 %) and 8192 x 8192 fp32 52.8 us (97 %).
+// Odd rows shift gamma's words for every row, and their block forms of a bf16 stream spill 28 to 108 bytes at 64 registers; beside
+// even rows of about the same length: 8192 x 4999 bf16 with residual to int8 57 us (bf16 gamma) and 61 us (fp32 gamma), 46 us at 5000 columns; without
+// a residual 41 and 31 us; 8192 x 8191 without a residual 72 us (43 %: seven columns of phase make a ninth warp, three blocks per SM
+// in place of four), 48 us at 8192; 2048 x 20001 fp32 without a residual 94 us (33 %), 66 us at 20000.
+// Short rows: 200000 of 128 columns take 54 us (22 %), of 129 columns 93 us (13 %): a block lives for four rows, and at 128 columns
+// half of a warp's lanes have no element. Codes under given scales are divided for, out of line: 8192 x 8192 bf16 with residual to
+// int8 101 us and to fp8 106 us.
 #pragma once
 #include <type_traits>
 
@@ -28,7 +33,7 @@ namespace mmeb200 {
 // but the same distance (the phase) past eight elements in every tensor, as rows of an odd length that lie one behind the other do:
 // columns are counted from the boundary before the row, and all but the pieces at a row's two ends move as with 8. 1: element by
 // element, a lane's elements 32 columns apart so that a warp's accesses stay contiguous. (bf16 rows of 4999 columns to int8 with a
-// residual, 8192 of them: 61 us phased, 83 us one by one; 5000 columns take 47 us.)
+// residual and an fp32 gamma, 8192 of them: 61 us phased, 83 us one by one; 5000 columns take 46 us.)
 template <int TYPE>
 struct RowElem;
 template <> struct RowElem<ROW_BF16> { static constexpr int kBytes = 2; };
@@ -74,7 +79,8 @@ __device__ __forceinline__ void store_element(uint8_t* a, const uint32_t (&w)[W]
 }
 // The eight elements of a lane, packed. Columns from `c0` on (in_row); those outside the span read as zeros, of a phased row once
 // trim_piece has cleared them: there the aligned 16 bytes around a row's ends are read whole (none without a byte of the row), so
-// that no lane goes another way while loads are issued (a branch for the ends: 79 us where this takes 71, 8192 x 4999). Such a word
+// that no lane goes another way while loads are issued (a branch for the ends: 79 us where this took 71, 8192 x 4999 bf16 with a residual to
+// int8 and an fp32 gamma, before gamma was fetched ahead: 61 us since). Such a word
 // lies in the page of the byte it shares with the row. `row` is where column 0 would be.
 template <int TYPE, int VEC, int W>
 __device__ __forceinline__ void load_piece(const void* row, uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[W]) {
@@ -659,7 +665,9 @@ __global__ void __launch_bounds__(1024) norm_long_kernel(const __grid_constant__
 // blocks, ...; every thread keeps the sums of its own columns of dgamma, and the block's partial sums (one row of `partial`)
 // are added in a fixed order by column_sums: results do not depend on timing. HBM bounds it: 16384 x 4096 bf16 67.6 us (91 % of the
 // copy rate), 91 us with the sum's gradient (90 %), 2048 x 16384 54 us (76 %, two blocks of a cluster per row); 8000 rows of 1000
-// columns 19.5 us (38 %), where the block's first row and the second launch weigh most.
+// columns 20 us (37 %), where the block's first row and the second launch weigh most. Odd rows: 8192 x 4999 64 us (59 %; 5000 columns
+// 49 us), 2048 x 16383 with the sum's 93 us (44 %). fp32 forms keep their pieces in registers and, with the sum's gradient, spill 112
+// to 440 bytes: 4096 x 8192 121 us (68 %), 86 us without it (71 %).
 //
 // a (dy * gamma) becomes dx; acc += dy * u.
 template <bool DSUM>
@@ -1023,8 +1031,9 @@ __global__ void __launch_bounds__(256) column_max_kernel(const __grid_constant__
     for (int i = 1; i < 8; ++i) t = max_nan(t, part[i][threadIdx.x]);
     atomicMax(reinterpret_cast<uint32_t*>(p.scale) + mine, __float_as_uint(t) & 0x7FFFFFFFu);
 }
-// Both passes together: 8192 x 8192 bf16 64 us, where reading x twice and writing once is 51 us; 8191 x 8193 112 us (the ends of the
-// result's rows are written byte by byte; in a pass of their own that was 121 us).
+// Both passes together: 8192 x 8192 bf16 64 us, where reading x twice and writing once is 51 us: the first pass covers the whole
+// matrix, so the second reads most of it from HBM again; 4096 x 4096 fp32 30 us; 8191 x 8193 bf16 112 us (the ends of the result's
+// rows are written byte by byte; in a pass of their own that was 121 us).
 // Tiles of 128 rows x 256 columns (248 phased): a warp takes four rows at a time, a lane eight of their columns, whose codes make one
 // word per column. The tile's columns leave as aligned 16-byte words (byte by byte at their ends). Four blocks per SM hide one's
 // loads behind another's stores: 8192 x 8192 bf16 64 us, with three and rows read a step ahead 68 us.

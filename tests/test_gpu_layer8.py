@@ -250,6 +250,22 @@ def test_eps_of_every_finite_size(calc, dev):
         assert (np.abs(dev.get(td) - dx) <= layer8.norm_grad_bounds(v, np.ones(4), v, None, eps, abi.FP32)[0]).all()
 
 
+@pytest.mark.parametrize("cols", [40, 5000])
+def test_norm_of_rows_whose_squares_leave_32_bits(calc, dev, cols):
+    """As the header says: an infinite mean square gives zeros (scale 0), a vanishing one with eps = 0 no numbers (scale infinite).
+    The codes are those of h * gamma all the same."""
+    v = np.ones((2, cols), np.float32)
+    v[0] *= np.float32(1e20)
+    v[1] *= np.float32(1e-30)
+    tx, to = dev.put(v, abi.FP32), dev.put(np.ones_like(v), abi.FP32)
+    tq, ts = dev.put(np.zeros((2, cols), np.int8), abi.INT8), dev.put(np.ones(2, np.float32), abi.FP32)
+    calc.rms_norm(to, tx, None, 0.0)
+    calc.rms_norm(tq, tx, None, 0.0, scale=ts)
+    calc.sync()
+    assert (dev.get(to)[0] == 0).all() and np.isinf(dev.get(to)[1]).all()
+    assert (dev.get(tq) == 127).all() and list(dev.get(ts)[0]) == [0.0, np.inf]
+
+
 @pytest.mark.parametrize("cols", [64, 2056, 9001, 40000])
 def test_norm_in_place(calc, dev, cols):
     """sum over residual, out over x: the same values as with tensors of their own."""
@@ -1053,6 +1069,15 @@ def test_first_calls_of_a_process_inside_a_capture():
     """Nothing that a call sets up once keeps it from being captured."""
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FIRST_CALLS_CAPTURED, root], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+def test_first_products_of_many_tiles_inside_a_capture():
+    """The same with the kernel of many tiles."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    text = FIRST_CALLS_CAPTURED.replace("rows, cols, n = 12, 9104, 136", "rows, cols, n = 520, 1104, 264; calc.set_option('pair', 1)")
+    assert text != FIRST_CALLS_CAPTURED
+    done = subprocess.run([sys.executable, "-c", text, root], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
 
 
