@@ -41,7 +41,8 @@ __device__ __forceinline__ void token_put(const TokenGemmParams& p, uint32_t m, 
     }
 }
 // COUNT consecutive tokens of this lane's channel: acc * (the token's scale, held by lane `place` + j), rounded, then * ws + bias in
-// one operation, as in the CTA-pair kernel (epilogue_scaled). `exist` of them exist. All values first, then all stores: nothing waits between two of them.
+// one operation, as in the CTA-pair kernel (epilogue_scaled). `exist` of them exist. All values first, then all stores: nothing waits
+// between two of them.
 template <int KIND, bool BF16, int COUNT>
 __device__ __forceinline__ void token_put_all(const TokenGemmParams& p, const uint32_t* v, uint32_t m, uint32_t exist, uint32_t n, float scales, uint32_t place, float ws,
                                               float bias) {

@@ -13,9 +13,9 @@
 // be read and written at 6549 GB/s: 8192 x 8192 bf16 with residual to int8 71.8 us (100 %), 16384 x 4096 with an fp32 residual to
 // bf16 121 us (102 %), quantisation of 2048 x 28672 bf16 33.5 us (80 %) and 8192 x 8192 fp32 52.8 us (97 %).
 // Odd rows shift gamma's words for every row, and their block forms of a bf16 stream spill 28 to 108 bytes at 64 registers; beside
-// even rows of about the same length: 8192 x 4999 bf16 with residual to int8 57 us (bf16 gamma) and 61 us (fp32 gamma), 46 us at 5000 columns; without
-// a residual 41 and 31 us; 8192 x 8191 without a residual 72 us (43 %: seven columns of phase make a ninth warp, three blocks per SM
-// in place of four), 48 us at 8192; 2048 x 20001 fp32 without a residual 94 us (33 %), 66 us at 20000.
+// even rows of about the same length: 8192 x 4999 bf16 with residual to int8 57 us (bf16 gamma) and 61 us (fp32 gamma), 46 us at
+// 5000 columns; without a residual 41 and 31 us; 8192 x 8191 without a residual 72 us (43 %: seven columns of phase make a ninth
+// warp, three blocks per SM in place of four), 48 us at 8192; 2048 x 20001 fp32 without a residual 94 us (33 %), 66 us at 20000.
 // Short rows: 200000 of 128 columns take 54 us (22 %), of 129 columns 93 us (13 %): a block lives for four rows, and at 128 columns
 // half of a warp's lanes have no element. Codes under given scales are divided for, out of line: 8192 x 8192 bf16 with residual to
 // int8 101 us and to fp8 106 us.
@@ -79,9 +79,8 @@ __device__ __forceinline__ void store_element(uint8_t* a, const uint32_t (&w)[W]
 }
 // The eight elements of a lane, packed. Columns from `c0` on (in_row); those outside the span read as zeros, of a phased row once
 // trim_piece has cleared them: there the aligned 16 bytes around a row's ends are read whole (none without a byte of the row), so
-// that no lane goes another way while loads are issued (a branch for the ends: 79 us where this took 71, 8192 x 4999 bf16 with a residual to
-// int8 and an fp32 gamma, before gamma was fetched ahead: 61 us since). Such a word
-// lies in the page of the byte it shares with the row. `row` is where column 0 would be.
+// that no lane goes another way while loads are issued (a branch for the ends: 79 us where this took 71, 8192 x 4999 bf16 with a
+// residual to int8 and an fp32 gamma, before gamma was fetched ahead: 61 us since). Such a word lies in the page of the byte it shares with the row. `row` is where column 0 would be.
 template <int TYPE, int VEC, int W>
 __device__ __forceinline__ void load_piece(const void* row, uint32_t c0, const RowSpan<VEC>& span, uint32_t (&w)[W]) {
     constexpr int kBytes = RowElem<TYPE>::kBytes;
